@@ -5,6 +5,8 @@ API (reset / submit / step -> dict / clock / output_schema / counters / state_di
 make_engine("WIFI", ..., NRConfig(wifi=WifiConfig(...))) returns the mean-field 802.11 level
 (isaac_net/core/wifi/engine.py:100-403). Both run the hand-written HIP kernels of csrc/ through the C ABI of
 include/inet_nr.h and include/inet_wifi.h.
+
+delta_rule, delta_rule_step, gated_ffn and block_norm are what a recurrent policy computes beside them (policy.py).
 """
 from .config import NRConfig  # noqa: F401
 from .phy import PhyTables  # noqa: F401
@@ -24,6 +26,9 @@ def __getattr__(name):
     if name in ("HipWifiEngine", "wifi_refusals"):
         from . import wifi_engine
         return getattr(wifi_engine, name)
+    if name in ("delta_rule", "delta_rule_step", "gated_ffn", "block_norm"):
+        from . import policy
+        return getattr(policy, name)
     if name == "WifiConfig":
         from .wifi_config import WifiConfig
         return WifiConfig

@@ -1,5 +1,5 @@
-"""ctypes binding of libinet_nr.so (include/inet_nr.h, include/inet_wifi.h). No torch types cross the ABI: only
-pointers and sizes."""
+"""ctypes bindings of libinet_nr.so (include/inet_nr.h, include/inet_wifi.h) and libinet_policy.so
+(include/inet_policy.h). No torch types cross the ABI: only pointers and sizes."""
 from __future__ import annotations
 
 import ctypes as C
@@ -125,6 +125,39 @@ class InetDcfParams(C.Structure):
                [("fer", f32)]
 
 
+class InetDelta(C.Structure):
+    _fields_ = [(n, i32) for n in ("B", "T", "Hk", "H", "K", "V", "dtype", "gate_dtype")] + \
+               [("scale", f32), ("chunk", i32)] + \
+               [(n, i64 * 3) for n in ("q_s", "k_s", "v_s", "g_s", "beta_s")] + [("reset_s", i64 * 2)] + \
+               [(n, P) for n in ("q", "k", "v", "g", "beta", "reset", "state", "o", "state_out", "chunk_state", "err")]
+
+
+class InetDeltaGrad(C.Structure):
+    _fields_ = [(n, P) for n in ("d_o", "d_state_out", "d_q", "d_k", "d_v", "d_g", "d_beta", "d_state", "chunk_grad",
+                                 "err_grad", "head_grad")]
+
+
+class InetFfn(C.Structure):
+    _fields_ = [("N", i64)] + [(n, i32) for n in ("D", "F", "dtype", "act")] + \
+               [(n, i64) for n in ("x_s", "w_gate_s", "w_up_s", "y_s")] + \
+               [(n, P) for n in ("x", "w_gate", "w_up", "y", "work")]
+
+
+class InetFfnGrad(C.Structure):
+    _fields_ = [("d_y", P), ("d_y_s", i64), ("d_x", P), ("d_w_gate", P), ("d_w_up", P)]
+
+
+class InetNorm(C.Structure):
+    _fields_ = [("N", i64)] + [(n, i32) for n in ("D", "dtype", "gate_kind")] + [("eps", f32)] + \
+               [(n, i64) for n in ("x_s", "f_s", "gate_s")] + \
+               [(n, P) for n in ("x", "f", "gate", "scale", "post_weight", "pre_weight", "y", "n")]
+
+
+class InetNormGrad(C.Structure):
+    _fields_ = [(n, P) for n in ("d_y", "d_n", "d_x", "d_f", "d_gate", "d_scale", "d_post_weight", "d_pre_weight",
+                                 "work")]
+
+
 ROW_DTYPE_FIELDS = ("rel", "nsym_idx", "flags", "re_prb", "rho", "c1", "salt_fade", "salt_bler")   # 8 x 4 bytes
 ERRORS = {-1: "invalid argument (size or pointer)", -2: "unsupported configuration for this build",
           -3: "HIP launch failed"}
@@ -195,6 +228,44 @@ def load(path=LIB_PATH):
         raise RuntimeError(f"{path} was built from other sources (src={built}, the tree's is {source_hash()}): "
                            "rebuild it with `python isaac-net_amd/build.py`")
     _LIB = lib
+    return lib
+
+
+POLICY_LIB_PATH = os.path.join(HERE, "libinet_policy.so")
+POLICY_ABI_VERSION = 1
+_POLICY_LIB = None
+
+
+def load_policy(path=POLICY_LIB_PATH):
+    """Load the policy operators' library; raises if it is missing, of another version or built from other sources."""
+    global _POLICY_LIB
+    if _POLICY_LIB is not None:
+        return _POLICY_LIB
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: build it with `python isaac-net_amd/build.py` (hipcc, gfx950)")
+    import torch  # noqa: F401  (its HIP runtime first, as in load())
+    lib = C.CDLL(path)
+    lib.inet_policy_abi_version.restype = i32
+    lib.inet_policy_build_info.restype = C.c_char_p
+    if lib.inet_policy_abi_version() != POLICY_ABI_VERSION:
+        raise RuntimeError("libinet_policy.so ABI version mismatch; rebuild it")
+    lib.inet_policy_delta_chunk.argtypes = [i32, i32, i32, i32]
+    lib.inet_policy_ffn_work.argtypes = [i64, i32, i32, i32]
+    lib.inet_policy_norm_work.argtypes = [i64, i32]
+    lib.inet_policy_ffn_work.restype = lib.inet_policy_norm_work.restype = i64
+    for name, args in (("delta_forward", (InetDelta,)), ("delta_backward", (InetDelta, InetDeltaGrad)),
+                       ("delta_step", (InetDelta,)), ("ffn_forward", (InetFfn,)),
+                       ("ffn_backward", (InetFfn, InetFfnGrad)), ("norm_forward", (InetNorm,)),
+                       ("norm_backward", (InetNorm, InetNormGrad))):
+        fn = getattr(lib, "inet_policy_" + name)
+        fn.argtypes = [C.POINTER(t) for t in args] + [P]
+        fn.restype = i32
+    from .build import policy_hash
+    built = lib.inet_policy_build_info().decode().rsplit("src=", 1)[-1]
+    if built != policy_hash():
+        raise RuntimeError(f"{path} was built from other sources (src={built}, the tree's is {policy_hash()}): "
+                           "rebuild it with `python isaac-net_amd/build.py`")
+    _POLICY_LIB = lib
     return lib
 
 

@@ -1,0 +1,183 @@
+// One control step of the gated delta rule (a rollout), the state updated in place, and the delta rule's C ABI.
+//
+// What bounds it is the state: 8 K V bytes a head, read and written once, against 6 K V operations. A wave takes one
+// head's block of columns into its registers: LP lanes across the columns, VW each (one 16-byte load), 64 / LP rows at
+// a time, RL such loads a lane; the sums over the rows are taken in the lane and then across the row groups.
+#include "delta.h"
+#include "delta_launch.h"
+
+namespace pol {
+
+template <typename T, int LP, int VW, int RL>
+__global__ __launch_bounds__(256) void delta_step_kernel(InetDelta d, int blocks) {
+    constexpr int RG = 64 / LP;                                  // rows a load
+    typedef float Vec __attribute__((ext_vector_type(VW)));
+    __shared__ float s_k[4][RL * RG], s_q[4][RL * RG];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane % LP, r0 = lane / LP;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + w, heads = (int64_t)d.B * d.H;
+    const int64_t bh = unit / blocks;
+    const bool live = bh < heads;
+    const int b = live ? (int)(bh / d.H) : 0, h = live ? (int)(bh % d.H) : 0, hk = h / (d.H / d.Hk);
+    const int col = ((int)(unit % blocks) * LP + c) * VW;
+    const bool in = live && col < d.V;
+    float* S = d.state_out + (bh * d.K) * d.V + col;
+    Vec x[RL];
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+        const int row = i * RG + r0;
+        x[i] = in && row < d.K ? *(const Vec*)(S + (int64_t)row * d.V) : Vec{};
+    }
+    if (live)
+        for (int i = lane; i < RL * RG; i += 64) {
+            s_k[w][i] = i < d.K ? (float)((const T*)d.k)[b * d.k_s[0] + hk * d.k_s[2] + i] : 0.0f;
+            s_q[w][i] = i < d.K ? (float)((const T*)d.q)[b * d.q_s[0] + hk * d.q_s[2] + i] : 0.0f;
+        }
+    float keep = 1.0f, beta = 0.0f;
+    Vec v = {};
+    if (live) {
+        const float g = gate_load(d.g, b * d.g_s[0] + h * d.g_s[2], d.gate_dtype);
+        beta = gate_load(d.beta, b * d.beta_s[0] + h * d.beta_s[2], d.gate_dtype);
+        keep = (d.reset && d.reset[b * d.reset_s[0]]) || (double)g < DECAY_MIN ? 0.0f : expf(g);
+    }
+    if (in)
+        for (int e = 0; e < VW; ++e) v[e] = (float)((const T*)d.v)[b * d.v_s[0] + h * d.v_s[2] + col + e];
+    __syncthreads();
+    Vec read = {};
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+        const float kk = s_k[w][i * RG + r0];
+        for (int e = 0; e < VW; ++e) {
+            x[i][e] = keep != 0.0f ? keep * x[i][e] : 0.0f;      // (an emptied state is empty whatever it held)
+            read[e] += kk * x[i][e];
+        }
+    }
+#pragma unroll
+    for (int o = LP; o < 64; o <<= 1)
+        for (int e = 0; e < VW; ++e) read[e] += __shfl_xor(read[e], o);
+    Vec out = {};
+    for (int e = 0; e < VW; ++e) v[e] = beta * (v[e] - read[e]);
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+        const int row = i * RG + r0;
+        const float kk = s_k[w][row], qq = s_q[w][row];
+        for (int e = 0; e < VW; ++e) {
+            x[i][e] += kk * v[e];
+            out[e] += qq * x[i][e];
+        }
+        if (in && row < d.K) *(Vec*)(S + (int64_t)row * d.V) = x[i];
+    }
+#pragma unroll
+    for (int o = LP; o < 64; o <<= 1)
+        for (int e = 0; e < VW; ++e) out[e] += __shfl_xor(out[e], o);
+    if (in && r0 == 0)
+        for (int e = 0; e < VW; ++e) ((T*)d.o)[bh * d.V + col + e] = (T)(d.scale * out[e]);
+}
+
+template <typename T, int LP, int VW, int RL> static int launch(const InetDelta& d, hipStream_t st) {
+    const int blocks = (d.V + LP * VW - 1) / (LP * VW);
+    const int64_t units = (int64_t)d.B * d.H * blocks;
+    auto k = delta_step_kernel<T, LP, VW, RL>;
+    hipLaunchKernelGGL(k, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, d, blocks);
+    return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
+}
+
+// rows a lane: the smallest build that holds K
+template <typename T, int LP, int VW> static int rows(const InetDelta& d, hipStream_t st) {
+    constexpr int RG = 64 / LP;
+    const int need = (d.K + RG - 1) / RG;
+    if constexpr (128 / RG > 16)
+        if (need > 16) return launch<T, LP, VW, 32>(d, st);
+    if constexpr (128 / RG > 8)
+        if (need > 8) return launch<T, LP, VW, 16>(d, st);
+    if (need > 4) return launch<T, LP, VW, 8>(d, st);
+    return launch<T, LP, VW, 4>(d, st);
+}
+
+template <typename T> static int widths(const InetDelta& d, hipStream_t st) {
+    // columns a lane: four where rows start on 16 bytes, else one; lanes across: the narrowest that takes all columns,
+    // up to 16 (more rows a load, so a head of 128 columns is two waves' and keeps half the registers)
+    if (d.V % 4 || (uintptr_t)d.state_out % 16) return rows<T, 16, 1>(d, st);
+    if (d.V <= 16) return rows<T, 4, 4>(d, st);
+    return d.V <= 32 ? rows<T, 8, 4>(d, st) : rows<T, 16, 4>(d, st);
+}
+
+int delta_step(const InetDelta& d, hipStream_t st) {
+    if (d.dtype == INET_POLICY_F32) return widths<float>(d, st);
+    if (d.dtype == INET_POLICY_BF16) return widths<__bf16>(d, st);
+    return widths<_Float16>(d, st);
+}
+
+// ------------------------------------------------------------------------------------------------ C ABI
+constexpr int64_t GRID_MAX = (1 << 24) - 1;       // workgroups of 256 lanes a launch
+
+static int elem_size(int dtype) { return dtype == INET_POLICY_F32 ? 4 : 2; }
+
+static int check(const InetDelta* a) {
+    if (!a || a->B < 0 || a->T < 0 || a->Hk < 1 || a->H < 1 || a->K < 1 || a->V < 1) return INET_POLICY_EINVAL;
+    if (a->H % a->Hk || a->dtype < 0 || a->dtype > 2 || a->gate_dtype < 0 || a->gate_dtype > 2)
+        return INET_POLICY_EINVAL;
+    if (a->K > INET_POLICY_MAX_HEAD || a->V > INET_POLICY_MAX_HEAD) return INET_POLICY_EUNSUPPORTED;
+    if ((int64_t)a->B * a->H > GRID_MAX) return INET_POLICY_EUNSUPPORTED;
+    return INET_POLICY_OK;
+}
+
+static int check_window(const InetDelta* a) {
+    if (int rc = check(a)) return rc;
+    if (a->chunk != inet_policy_delta_chunk(a->T, a->K, a->V, a->dtype)) return INET_POLICY_EINVAL;
+    const int64_t chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;
+    if ((int64_t)a->B * a->H * chunks > GRID_MAX) return INET_POLICY_EUNSUPPORTED;
+    return INET_POLICY_OK;
+}
+
+// bit 0, 1, 2: rows of k, of q, and of V contiguous values start on 16 bytes and hold whole groups of eight
+static int aligned(const InetDelta* a) {
+    const int e = elem_size(a->dtype);
+    auto rows = [&](const void* p, const int64_t* s) {
+        return a->K % 8 == 0 && (uintptr_t)p % 16 == 0 && s[0] * e % 16 == 0 && s[1] * e % 16 == 0 && s[2] * e % 16 == 0;
+    };
+    return (rows(a->k, a->k_s) ? 1 : 0) | (rows(a->q, a->q_s) ? 2 : 0);
+}
+
+}  // namespace pol
+
+extern "C" {
+
+int32_t inet_policy_delta_chunk(int32_t T, int32_t K, int32_t V, int32_t dtype) {
+    if (T < 0 || K < 1 || V < 1 || K > INET_POLICY_MAX_HEAD || V > INET_POLICY_MAX_HEAD || dtype < 0 || dtype > 2)
+        return 0;
+    if (dtype == INET_POLICY_F32 || (dtype == INET_POLICY_F16 && K > 64)) return 32;   // (LDS: delta_launch.h)
+    return T <= 32 ? 32 : 64;
+}
+
+int32_t inet_policy_delta_forward(const InetDelta* a, void* stream) {
+    if (int rc = pol::check_window(a)) return rc;
+    if (a->B == 0) return INET_POLICY_OK;
+    if (!a->state_out || a->state == a->state_out) return INET_POLICY_EINVAL;
+    if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o)) return INET_POLICY_EINVAL;
+    return pol::delta_forward(*a, pol::aligned(a), (hipStream_t)stream);
+}
+
+int32_t inet_policy_delta_backward(const InetDelta* a, const InetDeltaGrad* d, void* stream) {
+    if (int rc = pol::check_window(a)) return rc;
+    if (!d) return INET_POLICY_EINVAL;
+    if (a->B == 0 || (a->T == 0 && !d->d_state)) return INET_POLICY_OK;
+    if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->chunk_state || !a->err || !d->d_q || !d->d_k ||
+                     !d->d_v || !d->d_g || !d->d_beta || !d->chunk_grad || !d->err_grad))
+        return INET_POLICY_EINVAL;
+    if (a->H != a->Hk && a->T > 0 && !d->head_grad) return INET_POLICY_EINVAL;
+    int vec = pol::aligned(a);
+    if (a->V % 8 == 0 && (uintptr_t)a->err % 16 == 0 && (uintptr_t)d->err_grad % 16 == 0 && (uintptr_t)d->d_o % 16 == 0 &&
+        (uintptr_t)a->chunk_state % 16 == 0 && (uintptr_t)d->chunk_grad % 16 == 0)
+        vec |= 4;
+    return pol::delta_backward(*a, *d, vec, (hipStream_t)stream);
+}
+
+int32_t inet_policy_delta_step(const InetDelta* a, void* stream) {
+    if (int rc = pol::check(a)) return rc;
+    if (a->T != 1) return INET_POLICY_EINVAL;
+    if (a->B == 0) return INET_POLICY_OK;
+    if (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o || !a->state_out) return INET_POLICY_EINVAL;
+    return pol::delta_step(*a, (hipStream_t)stream);
+}
+
+}  // extern "C"

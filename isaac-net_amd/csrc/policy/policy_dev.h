@@ -1,0 +1,145 @@
+// Device helpers of the policy operators: element types, bfloat16 planes and the matrix instructions' fragments.
+//
+// Products of 32-bit precision on the bfloat16 matrix instructions. A value is held as a sum of planes, each the
+// bfloat16 nearest to what the planes before it leave over: one plane is a bfloat16 value itself, two hold a float16
+// value, three hold a float32 value to its last bit (3 x 8 significand bits). A product of two such sums keeps the
+// plane products whose orders add up to at most ORD: ORD = 2 drops what is below 2^-24 of the product, ORD = 1 what is
+// below 2^-16. The 32-bit matrix instruction has a sixteenth of the bfloat16 one's rate, six plane products (3 x 3
+// planes, ORD = 2) a sixth, and a bfloat16 operand against three planes a third.
+//
+// Fragments of v_mfma_f32_16x16x32_bf16 (lane l, n = l % 16, g = l / 16): A holds row n, B column n, each at the
+// contraction indexes 8 g .. 8 g + 7; the result holds column n at rows 4 g .. 4 g + 3. Two results stacked (rows 0..15
+// and 16..31) are a B fragment of a 32-long contraction in the order perm(): index 16 t + 4 g + i at place
+// 8 g + 4 t + i. Matrices that meet such a fragment are kept in that order, so a state or a row of values goes from one
+// product into the next without leaving its registers.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <stdint.h>
+
+#define DEV __device__ __forceinline__
+
+namespace pol {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Elem;
+template <> struct Elem<float> { static constexpr int planes = 3, ord = 2; };
+template <> struct Elem<__bf16> { static constexpr int planes = 1, ord = 1; };
+template <> struct Elem<_Float16> { static constexpr int planes = 2, ord = 1; };
+
+// eight consecutive elements, the first n of them inside the row (the others read as 0); vec: the row starts are
+// aligned to 16 bytes and rows hold whole groups of eight
+template <typename T> DEV void load8(const T* __restrict__ p, int n, bool vec, float (&x)[8]) {
+    if (vec && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+            for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+        } else {
+            typedef T V8 __attribute__((ext_vector_type(8)));
+            const V8 a = *(const V8*)p;
+            for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+        }
+    } else {
+        for (int i = 0; i < 8; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+
+// the same for four (vec: aligned to four elements)
+template <typename T> DEV void load4(const T* __restrict__ p, int n, bool vec, float (&x)[4]) {
+    if (vec && n >= 4) {
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        const V4 a = *(const V4*)p;
+        for (int i = 0; i < 4; ++i) x[i] = (float)a[i];
+    } else {
+        for (int i = 0; i < 4; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+
+template <int N> struct Frag { bf16x8 p[N]; };
+
+template <int N> DEV Frag<N> split8(const float (&x)[8]) {
+    Frag<N> f;
+    float r[8];
+    for (int e = 0; e < 8; ++e) r[e] = x[e];
+    for (int i = 0; i < N; ++i)
+        for (int e = 0; e < 8; ++e) {
+            const __bf16 h = (__bf16)r[e];
+            f.p[i][e] = h;
+            if (i + 1 < N) r[e] -= (float)h;
+        }
+    return f;
+}
+
+// two stacked 16 x 16 results as a B fragment
+template <int N> DEV Frag<N> split_tiles(f32x4 lo, f32x4 hi) {
+    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return split8<N>(x);
+}
+
+// c + A B over a 32-long contraction; the small plane products first
+template <int ORD, int NA, int NB> DEV f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
+#pragma unroll
+    for (int s = ORD; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], c, 0, 0, 0);
+    return c;
+}
+
+// c + A B over a 16-long contraction in 32 bits: a = A's row n at columns 4 g .. 4 g + 3, b a 16 x 16 result
+DEV f32x4 mma32(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+}
+
+// place of contraction index c in the order of two stacked results
+DEV int perm(int c) { return (c & ~31) | ((c & 12) << 1) | ((c & 16) >> 2) | (c & 3); }
+
+// a matrix of N planes in LDS, rows of ld elements (ld / 8 odd: 16 lanes' 16-byte reads fall on distinct banks)
+template <int N> struct Planes {
+    __bf16* p;
+    int ld, plane;
+    DEV Frag<N> frag(int row, int k8) const {            // eight elements from place k8 of a row
+        Frag<N> f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) f.p[i] = *(const bf16x8*)(p + i * plane + row * ld + k8);
+        return f;
+    }
+    DEV void put(int row, int place, float x) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const __bf16 h = (__bf16)x;
+            p[i * plane + row * ld + place] = h;
+            x -= (float)h;
+        }
+    }
+    DEV void put4(int row, int place, float a, float b, float c, float d) const {
+        float x[4] = {a, b, c, d};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            bf16x4 h;
+            for (int e = 0; e < 4; ++e) { h[e] = (__bf16)x[e]; x[e] -= (float)h[e]; }
+            *(bf16x4*)(p + i * plane + row * ld + place) = h;
+        }
+    }
+};
+
+template <typename T> DEV void store4(T* p, int n, bool vec, const float (&x)[4]) {
+    if (vec && n >= 4) {
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        V4 v;
+        for (int i = 0; i < 4; ++i) v[i] = (T)x[i];
+        *(V4*)p = v;
+    } else {
+        for (int i = 0; i < 4; ++i) if (i < n) p[i] = (T)x[i];
+    }
+}
+
+}  // namespace pol
