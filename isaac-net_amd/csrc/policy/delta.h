@@ -32,11 +32,12 @@ namespace pol {
 constexpr int DELTA_WG = 256;
 constexpr double DECAY_MIN = -104.0;     // e^-104 is 0 in 32 bits: the memory is emptied
 
-// per chunk and head: the gates, in LDS
+// per chunk and head: the gates, in LDS. Gam_ij of a step i and a step j of an earlier tile of 16 is in[i] out[tile of
+// i][j], through the last step before i's tile (for decays both factors are at most 1).
 template <int C> struct alignas(16) Gates {
     double G[C];
+    float a[C], c[C], beta[C], in[C], out[C / 16][C];
     int seg[C];
-    float a[C], c[C], beta[C];
     float a_end;
 };
 
@@ -46,81 +47,256 @@ DEV float gate_load(const void* p, int64_t i, int dtype) {
                                                                                        : gate_at<_Float16>(p, i);
 }
 
-// wave 0: the chunk's gates from step t0 on (steps from T on: no decay, nothing written)
-template <int C> DEV void load_gates(Gates<C>& s, const InetDelta& d, int b, int h, int t0) {
-    const int lane = threadIdx.x & 63, t = t0 + lane;
-    double g = 0.0;
-    float beta = 0.0f;
+// lane i's step of a chunk, as loaded (steps from T on: no decay, nothing written)
+struct Gate {
+    float g = 0.0f, beta = 0.0f;
     int cut = 0;
-    if (lane < C && t < d.T) {
-        const float gf = gate_load(d.g, b * d.g_s[0] + t * d.g_s[1] + h * d.g_s[2], d.gate_dtype);
-        beta = gate_load(d.beta, b * d.beta_s[0] + t * d.beta_s[1] + h * d.beta_s[2], d.gate_dtype);
-        cut = (d.reset && d.reset[b * d.reset_s[0] + t * d.reset_s[1]]) || (double)gf < DECAY_MIN;
-        g = cut ? 0.0 : (double)gf;
+    template <int C> DEV void load(const InetDelta& d, int b, int h, int t0) {
+        const int lane = threadIdx.x & 63, t = t0 + lane;
+        g = beta = 0.0f;
+        cut = 0;
+        if (lane < C && t < d.T) {
+            g = gate_load(d.g, b * d.g_s[0] + t * d.g_s[1] + h * d.g_s[2], d.gate_dtype);
+            beta = gate_load(d.beta, b * d.beta_s[0] + t * d.beta_s[1] + h * d.beta_s[2], d.gate_dtype);
+            if (d.reset) cut = d.reset[b * d.reset_s[0] + t * d.reset_s[1]];
+        }
     }
-    for (int o = 1; o < C; o <<= 1) {
-        const double u = __shfl_up(g, o);
-        const int v = __shfl_up(cut, o);
-        if (lane >= o) { g += u; cut += v; }
-    }
+};
+
+// one wave: the chunk's gates
+template <int C> DEV void put_gates(Gates<C>& s, const Gate& x) {
+    const int lane = threadIdx.x & 63;
+    const bool empty = x.cut != 0 || (double)x.g < DECAY_MIN;
+    const double g = lane_scan(empty ? 0.0 : (double)x.g);
+    const int seg = lane_scan(empty ? 1 : 0);
     const double g_end = __shfl(g, C - 1);
-    const int seg_end = __shfl(cut, C - 1);
+    const int seg_end = __shfl(seg, C - 1), to = (lane & ~15) - 1;
+    const double g_in = __shfl(g, to);                            // (of the first tile: not used)
+    const int seg_in = __shfl(seg, to);
+#pragma unroll
+    for (int r = 1; r < C / 16; ++r) {
+        const double g_r = __shfl(g, 16 * r - 1);
+        const int seg_r = __shfl(seg, 16 * r - 1);
+        if (lane < 16 * r) s.out[r][lane] = seg == seg_r ? expf((float)(g_r - g)) : 0.0f;
+    }
     if (lane < C) {
         s.G[lane] = g;
-        s.seg[lane] = cut;
-        s.beta[lane] = beta;
-        s.a[lane] = cut == 0 ? expf((float)g) : 0.0f;
-        s.c[lane] = cut == seg_end ? expf((float)(g_end - g)) : 0.0f;
+        s.seg[lane] = seg;
+        s.beta[lane] = x.beta;
+        s.a[lane] = seg == 0 ? expf((float)g) : 0.0f;
+        s.c[lane] = seg == seg_end ? expf((float)(g_end - g)) : 0.0f;
+        s.in[lane] = lane >= 16 && seg == seg_in ? expf((float)(g - g_in)) : 0.0f;
         if (lane == 0) s.a_end = seg_end == 0 ? expf((float)g_end) : 0.0f;
     }
 }
 
-// Gam_ij
-template <int C> DEV float decay(const Gates<C>& s, int i, int j) {
-    return s.seg[i] == s.seg[j] ? expf((float)(s.G[i] - s.G[j])) : 0.0f;
+// Gam_ij for step i and steps j .. j + 3, 4 g + e of a tile; DIAG: of the same tile of 16, j <= i alone
+template <int C, bool DIAG> DEV f32x4 decay4(const Gates<C>& s, int i, int j) {
+    f32x4 x;
+    if constexpr (DIAG) {
+        const double gi = s.G[i];
+        const int si = s.seg[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = j + e <= i && s.seg[j + e] == si ? expf((float)(gi - s.G[j + e])) : 0.0f;
+    } else {
+        x = *(const f32x4*)(s.out[i >> 4] + j) * s.in[i];
+    }
+    return x;
 }
 
-// rows t0 .. t0 + C - 1 of x [steps][K] (row stride st) into planes in the order perm(), and, where TR, transposed
-template <typename T, int C, int KP, int N, bool ROWS, bool TR>
-DEV void stage(const T* __restrict__ x, int64_t st, int t0, int t_end, int K, bool vec, const Planes<N>& rows,
-               const Planes<N>& tr) {
-    for (int i = threadIdx.x; i < C * (KP / 8); i += DELTA_WG) {
-        const int r = i / (KP / 8), c = i % (KP / 8) * 8;
-        float v[8] = {};
-        if (t0 + r < t_end && c < K) load8(x + (t0 + r) * st + c, K - c, vec, v);
-        if (ROWS) {
-            rows.put4(r, perm(c), v[0], v[1], v[2], v[3]);
-            rows.put4(r, perm(c + 4), v[4], v[5], v[6], v[7]);
+// C rows of x [steps][K] (row stride st) on their way from memory to LDS: load() and, when the rows of the chunk before
+// are done with, put()
+// (VEC: rows start on 16 bytes and hold whole groups of eight)
+template <typename T, int C, int KP, bool VEC> struct Rows {
+    static constexpr int GR = C * (KP / 8), NL = (GR + DELTA_WG - 1) / DELTA_WG;
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    V8 v[NL];
+    DEV void load(const T* __restrict__ x, int64_t st, int t0, int t_end, int K) {
+#pragma unroll
+        for (int m = 0; m < NL; ++m) {
+            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            v[m] = V8{};
+            if (i < GR && t0 + r < t_end && c < K) {
+                const T* p = x + (t0 + r) * st + c;
+                if constexpr (VEC) v[m] = *(const V8*)p;
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < K) v[m][e] = p[e];
+            }
         }
-        if (TR)
-            for (int e = 0; e < 8; ++e) tr.put(c + e, perm(r), v[e]);
+    }
+    DEV void put(T* s, int ld) const {                            // as they are
+#pragma unroll
+        for (int m = 0; m < NL; ++m) {
+            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            if (GR % DELTA_WG == 0 || i < GR) *(V8*)(s + r * ld + c) = v[m];
+        }
+    }
+    template <int N> DEV void put(const Planes<N>& s) const {
+#pragma unroll
+        for (int m = 0; m < NL; ++m) {
+            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            if (GR % DELTA_WG == 0 || i < GR) {
+                s.put4(r, perm(c), (float)v[m][0], (float)v[m][1], (float)v[m][2], (float)v[m][3]);
+                s.put4(r, perm(c + 4), (float)v[m][4], (float)v[m][5], (float)v[m][6], (float)v[m][7]);
+            }
+        }
+    }
+};
+
+// a 16 x 16 tile of values in LDS (rows of ld, the tile at s) as a matrix instruction's result: lane column n, rows 4 g + e
+template <typename T> DEV f32x4 tile_at(const T* s, int ld, int n, int g) {
+    f32x4 x;
+    if constexpr (sizeof(T) == 2) {
+        typedef T V4 __attribute__((ext_vector_type(4)));
+        const V4 v = __builtin_bit_cast(V4, read_tr((const __bf16*)s + (4 * g + (n >> 2)) * ld + (n & 3) * 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (float)v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = s[(4 * g + e) * ld + n];
+    }
+    return x;
+}
+
+// such a result to LDS, rounded to T
+template <typename T> DEV void tile_put(T* s, int ld, int n, int g, f32x4 x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[(4 * g + e) * ld + n] = (T)x[e];
+}
+
+// C rows of 64 columns from LDS (rows of LV) to out [steps][heads][V], out at the first step, this head and these columns
+constexpr int LV = 64 + 8;
+template <typename T, int C, bool VEC> DEV void store_rows(const T* s, T* __restrict__ out, int64_t st, int steps, int cols) {
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    for (int i = threadIdx.x; i < C * 8; i += DELTA_WG) {
+        const int r = i / 8, c = i % 8 * 8;
+        if (r < steps && c < cols) {
+            const V8 v = *(const V8*)(s + r * LV + c);
+            T* p = out + r * st + c;
+            if constexpr (VEC) *(V8*)p = v;
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < cols) p[e] = v[e];
+        }
     }
 }
 
-// the 16 x 16 diagonal blocks of I + L (L's negative in Ln, row-major, rows of ld) replaced by their inverses: wave w
-// takes block w; lane n of each 16 solves for column n by forward substitution
-template <int C> DEV void invert_blocks(float* Ln, int ld) {
-    const int w = threadIdx.x >> 6, n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-    if (w >= C / 16) return;
-    float* B = Ln + (w * 16) * ld + w * 16;
-    float x[16];
+// the state's tiles of 16 columns, from and to [K][V] at the first of the columns; off: row 4 g, column n
+template <int KT> DEV void state_load(f32x4 (&S)[KT], const float* __restrict__ p, uint32_t off, int V, int K, int g) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float s = i == n ? 1.0f : 0.0f;
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int m4 = 0; m4 < (i + 3) / 4; ++m4) {
-            const f32x4 l = *(const f32x4*)(B + i * ld + 4 * m4);
+        for (int e = 0; e < 4; ++e)
+            S[kt][e] = kt * 16 + 4 * g + e < K ? p[off + (uint32_t)((kt * 16 + e) * V)] : 0.0f;
+}
+template <int KT> DEV void state_store(const f32x4 (&S)[KT], float* __restrict__ p, uint32_t off, int V, int K, int g) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (4 * m4 + e < i) s += l[e] * x[4 * m4 + e];
-        }
-        x[i] = s;
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (kt * 16 + 4 * g + e < K) p[off + (uint32_t)((kt * 16 + e) * V)] = S[kt][e];
+}
+
+// keeps what is computed from x inside the loop: addresses are cheaper to compute again than to hold in registers
+DEV void keep(uint32_t& x) { asm volatile("" : "+v"(x)); }
+
+// tile row it of the triangles: -L (in Ln, f32, rows of ld) from K K^T, or P from Q K^T. The products are taken
+// transposed (K's rows as A), so that a lane holds four steps j of one step i. ROWS_BETA: L_ij takes beta_i, else beta_j.
+template <int C, int KP, int NP, bool ROWS_BETA>
+DEV void triangle_l(const Planes<NP>& Kr, const Gates<C>& gt, float* ln, int ld, int it, int n, int g) {
+    const int i = it * 16 + n;
+#pragma unroll
+    for (int jt = 0; jt < C / 16; ++jt) {
+        if (jt > it) continue;
+        f32x4 acc = {};
+#pragma unroll
+        for (int k8 = 0; k8 < KP; k8 += 32)
+            acc = mma<2>(Kr.frag(jt * 16 + n, k8 + 8 * g), Kr.frag(i, k8 + 8 * g), acc);
+        const int j = jt * 16 + 4 * g;
+        const f32x4 dec = jt == it ? decay4<C, true>(gt, i, j) : decay4<C, false>(gt, i, j);
+        f32x4 b = *(const f32x4*)(gt.beta + j);
+        if (ROWS_BETA) b = f32x4{1, 1, 1, 1} * gt.beta[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = j + e < i ? -acc[e] * dec[e] * b[e] : 0.0f;
+        *(f32x4*)(ln + i * ld + j) = acc;
     }
-    // (the wave's lanes have read the block before any of them writes: one wave, in order)
-    __builtin_amdgcn_wave_barrier();
+}
+template <int C, int KP, int NP, int NO>
+DEV void triangle_p(const Planes<NP>& Kr, const Planes<NP>& Qr, const Planes<NO>& P, const Gates<C>& gt, float scale,
+                    int it, int n, int g) {
+    const int i = it * 16 + n;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if ((i >> 2) == g) B[i * ld + n] = x[i];
+    for (int jt = 0; jt < C / 16; ++jt) {
+        const int j = jt * 16 + 4 * g;
+        if (jt <= it) {
+            f32x4 acc = {};
+#pragma unroll
+            for (int k8 = 0; k8 < KP; k8 += 32)
+                acc = mma<2>(Kr.frag(jt * 16 + n, k8 + 8 * g), Qr.frag(i, k8 + 8 * g), acc);
+            const f32x4 dec = (jt == it ? decay4<C, true>(gt, i, j) : decay4<C, false>(gt, i, j)) * scale;
+            P.put4(i, perm(j), acc[0] * dec[0], acc[1] * dec[1], acc[2] * dec[2], acc[3] * dec[3]);
+        } else if (jt == it + 1 && (jt & 1)) {       // the later tile of a pair that the products take together
+            P.put4(i, perm(j), 0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+}
+
+// the 16 x 16 diagonal blocks of I + L (-L in Ln, rows of ld) replaced by their inverses, by one wave: lanes 16 b .. 16 b
+// + 15 take block b, lane n holds row n and solves for column n by forward substitution, row i's values from lane i
+// s + sum of l[m .. m + 3] of lane I of each 16, times x[m .. m + 3]. (The compiler would take the 120 lane moves of a
+// block first, in as many registers; the wait states are those between a write of l and its read from another lane.)
+template <int I> DEV float sum4(const float (&l)[16], const float (&x)[16], int m, float s) {
+    asm volatile("s_nop 1\n\t"
+                 "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n\t"
+                 "v_fmac_f32_dpp %0, %2, %6 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n\t"
+                 "v_fmac_f32_dpp %0, %3, %7 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n\t"
+                 "v_fmac_f32_dpp %0, %4, %8 row_newbcast:%9 row_mask:0xf bank_mask:0xf"
+                 : "+v"(s)
+                 : "v"(l[m]), "v"(l[m + 1]), "v"(l[m + 2]), "v"(l[m + 3]), "v"(x[m]), "v"(x[m + 1]), "v"(x[m + 2]),
+                   "v"(x[m + 3]), "n"(I));
+    return s;
+}
+// (x[m] is 0 for m >= I, where l holds zeros too)
+template <int I> DEV void substitute(const float (&l)[16], float (&x)[16], int n) {
+    if constexpr (I < 16) {
+        float s = I == n ? 1.0f : 0.0f;
+#pragma unroll
+        for (int m = 0; m < I; m += 4) s = sum4<I>(l, x, m, s);
+        x[I] = s;
+        substitute<I + 1>(l, x, n);
+    }
+}
+template <int C> DEV void invert_blocks(float* ln, int ld) {
+    const int n = threadIdx.x & 15, blk = (threadIdx.x & 63) >> 4;
+    float* B = ln + (blk * 16) * ld + blk * 16;
+    const bool in = blk < C / 16;
+    float l[16] = {}, x[16] = {};
+    if (in)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const f32x4 v = *(const f32x4*)(B + n * ld + 4 * m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[4 * m + e] = v[e];
+        }
+    substitute<0>(l, x, n);
+    if (in)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) B[i * ld + n] = x[i];
+}
+
+// both triangles of a chunk, from K and Q in LDS, and the diagonal blocks' inverses; ends with a barrier
+template <int C, int KP, int NP, int NO, bool ROWS_BETA>
+DEV void triangles(const Planes<NP>& Kr, const Planes<NP>& Qr, const Planes<NO>& P, const Gates<C>& gt, float* ln,
+                   int ld, float scale, int w, int n, int g) {
+    if (w < C / 16) triangle_l<C, KP, NP, ROWS_BETA>(Kr, gt, ln, ld, w, n, g);
+    else if (C == 32) triangle_p<C, KP, NP, NO>(Kr, Qr, P, gt, scale, w - 2, n, g);
+    __syncthreads();
+    if (w == 0) invert_blocks<C>(ln, ld);
+    if (C == 64) triangle_p<C, KP, NP, NO>(Kr, Qr, P, gt, scale, w, n, g);
+    __syncthreads();
 }
 
 }  // namespace pol

@@ -10,120 +10,78 @@ namespace pol {
 template <typename T, int C, int KP> struct ScanLds {
     static constexpr int NP = Elem<T>::planes, LK = KP + 8, LC = C + 8, LL = C + 4;
     Gates<C> gates;
-    alignas(16) __bf16 k[NP * C * LK], kt[NP * KP * LC], qt[NP * KP * LC], pt[3 * C * LC];
+    alignas(16) __bf16 k[NP * C * LK], q[NP * C * LK], p[3 * C * LC];
     alignas(16) float ln[C * LL];
+    alignas(16) T u[C * LV], v[C * LV];
 };
 
 // The state's gradient. One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns.
-template <typename T, int C, int KP>
-__global__ __launch_bounds__(DELTA_WG) void delta_scan_kernel(InetDelta d, InetDeltaGrad gr, int vec) {
+template <typename T, int C, int KP, bool VEC>
+__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
+void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
     constexpr int NP = Elem<T>::planes, RT = C / 16, KT = KP / 16;
     extern __shared__ char lds_raw[];
     typedef ScanLds<T, C, KP> Lds;
     Lds& s = *(Lds*)lds_raw;
-    const Planes<NP> Kr{s.k, Lds::LK, C * Lds::LK}, Kt{s.kt, Lds::LC, KP * Lds::LC}, Qt{s.qt, Lds::LC, KP * Lds::LC};
-    const Planes<3> Pt{s.pt, Lds::LC, C * Lds::LC};
+    const Planes<NP> Kr{s.k, Lds::LK, C * Lds::LK}, Qr{s.q, Lds::LK, C * Lds::LK};
+    const Planes<3> P{s.p, Lds::LC, C * Lds::LC};
     const int b = blockIdx.x / d.H, h = blockIdx.x % d.H, hk = h / (d.H / d.Hk);
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int col = (blockIdx.y * 4 + w) * 16 + n;
-    const bool cols = (blockIdx.y * 4 + w) * 16 < d.V, mine = col < d.V;
+    const int c0 = blockIdx.y * 64, width = d.V - c0 < 64 ? d.V - c0 : 64;      // the workgroup's columns
+    const bool cols = w * 16 < width, mine = w * 16 + n < width;
     const T* q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2];
     const T* k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2];
     const int chunks = (d.T + C - 1) / C;
-    const int64_t bh = (int64_t)b * d.H + h;
+    const int64_t bh = (int64_t)b * d.H + h, row_s = (int64_t)d.H * d.V, rows0 = b * (int64_t)d.T * row_s + h * d.V + c0;
 
+    Rows<T, C, KP, VEC> kr, qr;
+    Rows<T, C, 64, VEC> ur;                              // dO
+    Gate gate;
+    auto fetch = [&](int t0) {
+        kr.load(k, d.k_s[1], t0, d.T, d.K);
+        qr.load(q, d.q_s[1], t0, d.T, d.K);
+        ur.load((const T*)gr.d_o + rows0, row_s, t0, gr.d_o ? d.T : 0, width);
+        if (w == 0) gate.load<C>(d, b, h, t0);
+    };
+    if (chunks) fetch((chunks - 1) * C);
+
+    uint32_t at = (uint32_t)(4 * g * d.V + w * 16 + n), at_err = (uint32_t)(4 * g * row_s + w * 16 + n);
     f32x4 S[KT] = {};                               // the gradient of the state, 16 columns
-    if (mine && gr.d_state_out)
-        for (int kt = 0; kt < KT; ++kt)
-            for (int e = 0; e < 4; ++e) {
-                const int row = kt * 16 + 4 * g + e;
-                if (row < d.K) S[kt][e] = gr.d_state_out[(bh * d.K + row) * d.V + col];
-            }
+    if (mine && gr.d_state_out) state_load(S, gr.d_state_out + bh * d.K * d.V + c0, at, d.V, d.K, g);
 
     for (int ch = chunks - 1; ch >= 0; --ch) {
         const int t0 = ch * C;
-        stage<T, C, KP, NP, true, true>(k, d.k_s[1], t0, d.T, d.K, vec & 1, Kr, Kt);
-        stage<T, C, KP, NP, false, true>(q, d.q_s[1], t0, d.T, d.K, vec & 2, Qt, Qt);
-        if (w == 0) load_gates<C>(s.gates, d, b, h, t0);
+        kr.put(Kr);
+        qr.put(Qr);
+        ur.put(s.u, LV);
+        if (w == 0) put_gates<C>(s.gates, gate);
         __syncthreads();
-        for (int job = w; job < 2 * RT; job += 4) {
-            const bool qk = job >= RT;
-            const int rt = qk ? 2 * RT - 1 - job : job, i_n = rt * 16 + n;
-            f32x4 acc[RT] = {};
-            for (int k8 = 0; k8 < KP; k8 += 32) {
-                Frag<NP> af;
-                if (qk) {                           // row i_n of Q, in the order that K's rows are kept in
-                    float x[8] = {}, y[4];
-                    const int c = k8 + 4 * g;
-                    const bool in = t0 + i_n < d.T;
-                    if (in && c < d.K) {
-                        load4(q + (t0 + i_n) * d.q_s[1] + c, d.K - c, vec & 2, y);
-                        for (int e = 0; e < 4; ++e) x[e] = y[e];
-                    }
-                    if (in && c + 16 < d.K) {
-                        load4(q + (t0 + i_n) * d.q_s[1] + c + 16, d.K - c - 16, vec & 2, y);
-                        for (int e = 0; e < 4; ++e) x[4 + e] = y[e];
-                    }
-                    af = split8<NP>(x);
-                } else {
-                    af = Kr.frag(i_n, k8 + 8 * g);
-                }
-#pragma unroll
-                for (int ct = 0; ct < RT; ++ct)
-                    if (ct <= rt) acc[ct] = mma<2>(af, Kr.frag(ct * 16 + n, k8 + 8 * g), acc[ct]);
-            }
-#pragma unroll
-            for (int ct = 0; ct < RT; ++ct) {
-                const int j = ct * 16 + n;
-                if (ct <= rt) {
-                    if (qk) {
-                        float p[4];
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = rt * 16 + 4 * g + e;
-                            p[e] = i >= j ? acc[ct][e] * d.scale * decay(s.gates, i, j) : 0.0f;
-                        }
-                        Pt.put4(j, perm(rt * 16 + 4 * g), p[0], p[1], p[2], p[3]);
-                    } else {
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = rt * 16 + 4 * g + e;
-                            s.ln[i * Lds::LL + j] = i > j ? -acc[ct][e] * s.gates.beta[i] * decay(s.gates, i, j) : 0.0f;
-                        }
-                    }
-                } else if (qk && ct == rt + 1 && (ct & 1)) {    // steps before the row tile, in the same pair
-                    Pt.put4(j, perm(rt * 16 + 4 * g), 0.0f, 0.0f, 0.0f, 0.0f);
-                }
-            }
-        }
-        __syncthreads();
-        invert_blocks<C>(s.ln, Lds::LL);
-        __syncthreads();
+        keep(at), keep(at_err);
+        triangles<C, KP, NP, 3, true>(Kr, Qr, P, s.gates, s.ln, Lds::LL, d.scale, w, n, g);
+        if (ch) fetch(t0 - C);
         if (cols) {
-            f32x4 u[RT], z[RT];                     // u: dO
-            for (int rt = 0; rt < RT; ++rt)
-                for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + rt * 16 + 4 * g + e;
-                    u[rt][e] = mine && t < d.T && gr.d_o
-                                   ? (float)((const T*)gr.d_o)[(((int64_t)b * d.T + t) * d.H + h) * d.V + col] : 0.0f;
-                }
             // dX = c K dS + P^T dO
-            for (int rt = 0; rt < RT; ++rt) z[rt] = f32x4{};
+            f32x4 z[RT] = {};
 #pragma unroll
             for (int kp = 0; kp < KT / 2; ++kp) {
                 const Frag<3> sf = split_tiles<3>(S[2 * kp], S[2 * kp + 1]);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) z[rt] = mma<2>(Kr.frag(rt * 16 + n, kp * 32 + 8 * g), sf, z[rt]);
             }
-            for (int rt = 0; rt < RT; ++rt)
-                for (int e = 0; e < 4; ++e) {
-                    const float c = s.gates.c[rt * 16 + 4 * g + e];
-                    z[rt][e] = c != 0.0f ? c * z[rt][e] : 0.0f;
-                }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const f32x4 c = *(const f32x4*)(s.gates.c + rt * 16 + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[rt][e] = c[e] != 0.0f ? c[e] * z[rt][e] : 0.0f;
+            }
+            f32x4 u[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) u[rt] = tile_at(s.u + rt * 16 * LV + w * 16, LV, n, g);
 #pragma unroll
             for (int kp = 0; kp < RT / 2; ++kp) {
                 const Frag<NP> uf = split_tiles<NP>(u[2 * kp], u[2 * kp + 1]);
 #pragma unroll
-                for (int rt = 0; rt < 2 * kp + 2; ++rt)
-                    z[rt] = mma<2>(Pt.frag(rt * 16 + n, kp * 32 + 8 * g), uf, z[rt]);
+                for (int rt = 0; rt < 2 * kp + 2; ++rt) z[rt] = mma<2>(P.tr_frag(rt, kp, n, g), uf, z[rt]);
             }
             // Z, block row by block row from the end
 #pragma unroll
@@ -131,66 +89,67 @@ __global__ __launch_bounds__(DELTA_WG) void delta_scan_kernel(InetDelta d, InetD
                 f32x4 acc = z[rt], a;
 #pragma unroll
                 for (int m = rt + 1; m < RT; ++m) {
+#pragma unroll
                     for (int e = 0; e < 4; ++e) a[e] = s.ln[(m * 16 + 4 * g + e) * Lds::LL + rt * 16 + n];
                     acc = mma32(a, z[m], acc);
                 }
+#pragma unroll
                 for (int e = 0; e < 4; ++e) a[e] = s.ln[(rt * 16 + 4 * g + e) * Lds::LL + rt * 16 + n];
                 z[rt] = mma32(a, acc, f32x4{});
             }
             if (mine) {
+                float* zs = gr.err_grad + rows0 + t0 * row_s;
+#pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
-                    for (int e = 0; e < 4; ++e) {
-                        const int t = t0 + rt * 16 + 4 * g + e;
-                        if (t < d.T) {
-                            const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.V + col;
-                            gr.err_grad[at] = z[rt][e];
-                            ((T*)gr.d_v)[at] = (T)(s.gates.beta[rt * 16 + 4 * g + e] * z[rt][e]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (t0 + rt * 16 + 4 * g + e < d.T) zs[at_err + (uint32_t)((rt * 16 + e) * row_s)] = z[rt][e];
+                state_store(S, gr.chunk_grad + (bh * chunks + ch) * d.K * d.V + c0, at, d.V, d.K, g);
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                tile_put(s.v + rt * 16 * LV + w * 16, LV, n, g, z[rt] * *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g));
+            if (ch || gr.d_state) {
+                const float a_end = s.gates.a_end;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
+#pragma unroll
+                for (int kp = 0; kp < RT / 2; ++kp) {
+                    f32x4 o[2], y[2];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const f32x4 a = *(const f32x4*)(s.gates.a + kp * 32 + 16 * m + 4 * g),
+                                    bt = *(const f32x4*)(s.gates.beta + kp * 32 + 16 * m + 4 * g);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[m][e] = d.scale * a[e] * u[2 * kp + m][e];
+                            y[m][e] = a[e] != 0.0f ? -bt[e] * a[e] * z[2 * kp + m][e] : 0.0f;
                         }
                     }
-                for (int kt = 0; kt < KT; ++kt)
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = kt * 16 + 4 * g + e;
-                        if (row < d.K) gr.chunk_grad[((bh * chunks + ch) * d.K + row) * d.V + col] = S[kt][e];
-                    }
-            }
-            const float a_end = s.gates.a_end;
-            for (int kt = 0; kt < KT; ++kt)
-                for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
+                    const Frag<3> of = split_tiles<3>(o[0], o[1]), yf = split_tiles<3>(y[0], y[1]);
 #pragma unroll
-            for (int kp = 0; kp < RT / 2; ++kp) {
-                f32x4 o[2], y[2];
-                for (int m = 0; m < 2; ++m)
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = kp * 32 + 16 * m + 4 * g + e;
-                        const float a = s.gates.a[i];
-                        o[m][e] = d.scale * a * u[2 * kp + m][e];
-                        y[m][e] = a != 0.0f ? -s.gates.beta[i] * a * z[2 * kp + m][e] : 0.0f;
+                    for (int kt = 0; kt < KT; ++kt) {
+                        S[kt] = mma<2>(Qr.tr_frag(kt, kp, n, g), of, S[kt]);
+                        S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), yf, S[kt]);
                     }
-                const Frag<3> of = split_tiles<3>(o[0], o[1]), yf = split_tiles<3>(y[0], y[1]);
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    S[kt] = mma<2>(Qt.frag(kt * 16 + n, kp * 32 + 8 * g), of, S[kt]);
-                    S[kt] = mma<2>(Kt.frag(kt * 16 + n, kp * 32 + 8 * g), yf, S[kt]);
                 }
             }
         }
         __syncthreads();
+        store_rows<T, C, VEC>(s.v, (T*)gr.d_v + rows0 + t0 * row_s, row_s, d.T - t0, width);
     }
-    if (mine && gr.d_state)
-        for (int kt = 0; kt < KT; ++kt)
-            for (int e = 0; e < 4; ++e) {
-                const int row = kt * 16 + 4 * g + e;
-                if (row < d.K) gr.d_state[(bh * d.K + row) * d.V + col] = S[kt][e];
-            }
+    if (mine && gr.d_state) state_store(S, gr.d_state + bh * d.K * d.V + c0, at, d.V, d.K, g);
 }
 
 constexpr int VMAX = INET_POLICY_MAX_HEAD;
 
-// LDS of the chunk kernel in bytes: transposed K and Q, X, Z and dO by rows (of vp + 8), gates and partial sums
+// LDS of the chunk kernel in bytes: K and Q, X, Z and dO by rows (of vp + 8), gates and partial sums
 template <typename T, int C, int KP> constexpr size_t chunk_lds(int vp) {
     constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1;
     return sizeof(Gates<C>) + (5 * 4 * C + 8) * sizeof(float) +
-           sizeof(__bf16) * (2 * NP * KP * (C + 8) + (2 * NO + NP) * C * (vp + 8));
+           sizeof(__bf16) * (2 * NP * C * (KP + 8) + (2 * NO + NP) * C * (vp + 8));
 }
 
 // eight consecutive values of a 32-bit matrix's row as an operand
@@ -202,17 +161,17 @@ template <int N> DEV Frag<N> row_frag(const float* __restrict__ p, bool in, int 
 
 // The gradients of q, k and the gates of one chunk. Wave w takes the steps of tile w % RT as its columns, and the key
 // rows' tiles w / RT, w / RT + 4 / RT, ...
-template <typename T, int C, int KP>
-__global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr, int vec) {
+template <typename T, int C, int KP, bool VEC>
+__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
     constexpr int NP = Elem<T>::planes, ORD = Elem<T>::ord, NO = ORD + 1, RT = C / 16, KT = KP / 16, PARTS = 4 / RT,
-                  LC = C + 8;
+                  LK = KP + 8;
     extern __shared__ char lds_raw[];
     const int vp = (d.V + 31) & ~31, lv = vp + 8;
     Gates<C>& gates = *(Gates<C>*)lds_raw;
     float* sums = (float*)(lds_raw + sizeof(Gates<C>));     // [5][4 parts][C] and the state's share [4], then pad
     __bf16* pool = (__bf16*)(sums + 5 * 4 * C + 8);
-    const Planes<NP> Kt{pool, LC, KP * LC}, Qt{pool + NP * KP * LC, LC, KP * LC};
-    __bf16* rows = pool + 2 * NP * KP * LC;
+    const Planes<NP> Kr{pool, LK, C * LK}, Qr{pool + NP * C * LK, LK, C * LK};
+    __bf16* rows = pool + 2 * NP * C * LK;
     const Planes<NO> X{rows, lv, C * lv}, Z{rows + NO * C * lv, lv, C * lv};
     const Planes<NP> O{rows + 2 * NO * C * lv, lv, C * lv};
     const int chunks = (d.T + C - 1) / C, ch = blockIdx.x % chunks, t0 = ch * C;
@@ -223,11 +182,19 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
     const T* k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2];
     const float* S = d.chunk_state + (bh * chunks + ch) * d.K * d.V;
     const float* dS = gr.chunk_grad + (bh * chunks + ch) * d.K * d.V;
-    const bool vv = vec & 4, vq = vec & 2, vk = vec & 1;    // rows of V, q and k aligned for whole-group loads
 
-    if (w == 0) load_gates<C>(gates, d, b, h, t0);
-    stage<T, C, KP, NP, false, true>(k, d.k_s[1], t0, d.T, d.K, vk, Kt, Kt);
-    stage<T, C, KP, NP, false, true>(q, d.q_s[1], t0, d.T, d.K, vq, Qt, Qt);
+    {
+        Rows<T, C, KP, VEC> kr, qr;
+        Gate gate;
+        kr.load(k, d.k_s[1], t0, d.T, d.K);
+        qr.load(q, d.q_s[1], t0, d.T, d.K);
+        if (w == 0) {
+            gate.load<C>(d, b, h, t0);
+            put_gates<C>(gates, gate);
+        }
+        kr.put(Kr);
+        qr.put(Qr);
+    }
     __syncthreads();
     // X = beta E, Z and dO by rows; dbeta's E . Z and <S, dS> on the way
     for (int i = threadIdx.x; i < C * (vp / 8); i += DELTA_WG) {
@@ -235,9 +202,9 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
         float e[8] = {}, z[8] = {}, o[8] = {};
         if (t < d.T && c < d.V) {
             const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.V + c;
-            load8(d.err + at, d.V - c, vv, e);
-            load8((const float*)gr.err_grad + at, d.V - c, vv, z);
-            if (gr.d_o) load8((const T*)gr.d_o + at, d.V - c, vv, o);
+            load8(d.err + at, d.V - c, VEC, e);
+            load8((const float*)gr.err_grad + at, d.V - c, VEC, z);
+            if (gr.d_o) load8((const T*)gr.d_o + at, d.V - c, VEC, o);
         }
         const float beta = gates.beta[r];
         X.put4(r, c, beta * e[0], beta * e[1], beta * e[2], beta * e[3]);
@@ -286,16 +253,34 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
             }
         }
     }
+    const float beta = gates.beta[i0];
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-        for (int e = 0; e < 4; ++e) {
-            const int i = r * 16 + 4 * g + e;
-            const float before = i <= i0 ? decay(gates, i0, i) : 0.0f, after = i >= i0 ? decay(gates, i, i0) : 0.0f;
-            dt[r][e] = i <= i0 ? dt[r][e] * d.scale * before : 0.0f;
-            mt[r][e] = i < i0 ? -mt[r][e] * gates.beta[i0] * before : 0.0f;
-            dn[r][e] = i >= i0 ? dn[r][e] * d.scale * after : 0.0f;
-            mn[r][e] = i > i0 ? -mn[r][e] * gates.beta[i] * after : 0.0f;
+    for (int r = 0; r < RT; ++r) {
+        const int i = r * 16 + 4 * g;
+        const f32x4 bt = *(const f32x4*)(gates.beta + i);
+        if (r <= tt) {
+            const f32x4 dec = r == tt ? decay4<C, true>(gates, i0, i) : decay4<C, false>(gates, i0, i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                dt[r][e] *= d.scale * dec[e];
+                mt[r][e] = i + e < i0 ? -mt[r][e] * beta * dec[e] : 0.0f;
+            }
         }
+        if (r >= tt) {
+            f32x4 dec;                             // Gam_{i + e, i0}
+            const float out = gates.out[r][i0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                dec[e] = r > tt ? gates.in[i + e] * out
+                                : i + e >= i0 && gates.seg[i + e] == gates.seg[i0]
+                                      ? expf((float)(gates.G[i + e] - gates.G[i0])) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                dn[r][e] *= d.scale * dec[e];
+                mn[r][e] = i + e > i0 ? -mn[r][e] * bt[e] * dec[e] : 0.0f;
+            }
+        }
+    }
     Frag<NO> dtf[RT / 2], dnf[RT / 2], mtf[RT / 2], mnf[RT / 2];
     for (int p = 0; p < RT / 2; ++p) {
         dtf[p] = split_tiles<NO>(dt[2 * p], dt[2 * p + 1]);
@@ -303,7 +288,7 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
         mtf[p] = split_tiles<NO>(mt[2 * p], mt[2 * p + 1]);
         mnf[p] = split_tiles<NO>(mn[2 * p], mn[2 * p + 1]);
     }
-    const float a = gates.a[i0], c = gates.c[i0], ya = -gates.beta[i0] * a, oa = d.scale * a;
+    const float a = gates.a[i0], c = gates.c[i0], ya = -beta * a, oa = d.scale * a;
     const int t = t0 + i0;
     float sq = 0.0f, sp = 0.0f, sn = 0.0f, sc = 0.0f;
     for (int kt = part; kt < KT; kt += PARTS) {
@@ -311,8 +296,8 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
         const int row = kt * 16 + n;
         f32x4 dq = {}, dp = {}, dm = {};
         for (int v = 0; v < vp; v += 32) {
-            const Frag<NO> sf = row_frag<NO>(S + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, vv);
-            const Frag<NO> df = row_frag<NO>(dS + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, vv);
+            const Frag<NO> sf = row_frag<NO>(S + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC);
+            const Frag<NO> df = row_frag<NO>(dS + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC);
             dq = mma<ORD>(sf, O.frag(i0, v + 8 * g), dq);
             dp = mma<ORD>(sf, Z.frag(i0, v + 8 * g), dp);
             dm = mma<ORD>(df, X.frag(i0, v + 8 * g), dm);
@@ -326,7 +311,7 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
         }
 #pragma unroll
         for (int p = 0; p < RT / 2; ++p) {
-            const Frag<NP> kf = Kt.frag(kt * 16 + n, p * 32 + 8 * g), qf = Qt.frag(kt * 16 + n, p * 32 + 8 * g);
+            const Frag<NP> kf = Kr.tr_frag(kt, p, n, g), qf = Qr.tr_frag(kt, p, n, g);
             dq = mma<ORD>(kf, dtf[p], dq);
             dp = mma<ORD>(kf, mtf[p], dp);
             dm = mma<ORD>(qf, dnf[p], dm);
@@ -335,8 +320,8 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
         const int kd = kt * 16 + 4 * g;
         if (t < d.T && kd < d.K) {
             float qv[4], kv[4], dk[4], dqv[4];
-            load4(q + t * d.q_s[1] + kd, d.K - kd, vq, qv);
-            load4(k + t * d.k_s[1] + kd, d.K - kd, vk, kv);
+            load4(q + t * d.q_s[1] + kd, d.K - kd, VEC, qv);
+            load4(k + t * d.k_s[1] + kd, d.K - kd, VEC, kv);
             for (int e = 0; e < 4; ++e) {
                 sq += dq[e] * qv[e];
                 sp += dp[e] * kv[e];
@@ -346,13 +331,12 @@ __global__ __launch_bounds__(DELTA_WG) void delta_chunk_kernel(InetDelta d, Inet
                 dqv[e] = dq[e];
             }
             const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.K + kd;
-            const bool v4 = (d.K & 3) == 0;
             if (d.H == d.Hk) {
-                store4((T*)gr.d_q + at, d.K - kd, v4, dqv);
-                store4((T*)gr.d_k + at, d.K - kd, v4, dk);
+                store4((T*)gr.d_q + at, d.K - kd, VEC, dqv);
+                store4((T*)gr.d_k + at, d.K - kd, VEC, dk);
             } else {
-                store4(gr.head_grad + at, d.K - kd, v4, dqv);
-                store4(gr.head_grad + (int64_t)d.B * d.T * d.H * d.K + at, d.K - kd, v4, dk);
+                store4(gr.head_grad + at, d.K - kd, VEC, dqv);
+                store4(gr.head_grad + (int64_t)d.B * d.T * d.H * d.K + at, d.K - kd, VEC, dk);
             }
         }
     }
@@ -412,19 +396,19 @@ __global__ __launch_bounds__(256) void delta_heads_kernel(const float* __restric
     k[i] = (T)sk;
 }
 
-template <typename T, int C, int KP>
-static int launch(const InetDelta& d, const InetDeltaGrad& g, int vec, hipStream_t st) {
+template <typename T, int C, int KP, bool VEC>
+static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
     const size_t lds = sizeof(ScanLds<T, C, KP>);
     static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && chunk_lds<T, C, KP>(VMAX) <= LDS_MAX, "LDS");
-    auto scan = delta_scan_kernel<T, C, KP>;
-    auto chunk = delta_chunk_kernel<T, C, KP>;
+    auto scan = delta_scan_kernel<T, C, KP, VEC>;
+    auto chunk = delta_chunk_kernel<T, C, KP, VEC>;
     const size_t cl = chunk_lds<T, C, KP>((d.V + 31) & ~31);
     if (allow_lds((const void*)scan, lds) || allow_lds((const void*)chunk, cl)) return INET_POLICY_ELAUNCH;
-    hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g, vec);
+    hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     const int chunks = (d.T + C - 1) / C;
     if (!chunks) return INET_POLICY_OK;
-    hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), cl, st, d, g, vec);
+    hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), cl, st, d, g);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     if (d.H != d.Hk) {
         const int64_t rows = (int64_t)d.B * d.T * d.Hk;
@@ -434,10 +418,11 @@ static int launch(const InetDelta& d, const InetDeltaGrad& g, int vec, hipStream
     return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
 }
 
-int delta_backward(const InetDelta& d, const InetDeltaGrad& g, int vec, hipStream_t st) {
+int delta_backward(const InetDelta& d, const InetDeltaGrad& g, bool vec, hipStream_t st) {
     return delta_dispatch(d, [&](auto t, auto c, auto kp) {
         typedef typename decltype(t)::type T;
-        return launch<T, decltype(c)::value, decltype(kp)::value>(d, g, vec, st);
+        constexpr int C = decltype(c)::value, KP = decltype(kp)::value;
+        return vec ? launch<T, C, KP, true>(d, g, st) : launch<T, C, KP, false>(d, g, st);
     });
 }
 

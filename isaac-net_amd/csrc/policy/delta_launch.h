@@ -41,8 +41,9 @@ template <typename F> int delta_dispatch(const InetDelta& d, F&& f) {
     return delta_dispatch_t(d, Type<_Float16>{}, f);
 }
 
-int delta_forward(const InetDelta& d, int vec, hipStream_t st);
-int delta_backward(const InetDelta& d, const InetDeltaGrad& g, int vec, hipStream_t st);
+// vec: all rows start on 16 bytes and hold whole groups of eight
+int delta_forward(const InetDelta& d, bool vec, hipStream_t st);
+int delta_backward(const InetDelta& d, const InetDeltaGrad& g, bool vec, hipStream_t st);
 int delta_step(const InetDelta& d, hipStream_t st);
 
 }  // namespace pol

@@ -124,18 +124,19 @@ static int check(const InetDelta* a) {
 static int check_window(const InetDelta* a) {
     if (int rc = check(a)) return rc;
     if (a->chunk != inet_policy_delta_chunk(a->T, a->K, a->V, a->dtype)) return INET_POLICY_EINVAL;
+    if ((int64_t)a->H * a->V > 1 << 22) return INET_POLICY_EUNSUPPORTED;      // (a chunk's offsets are 32-bit)
     const int64_t chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;
     if ((int64_t)a->B * a->H * chunks > GRID_MAX) return INET_POLICY_EUNSUPPORTED;
     return INET_POLICY_OK;
 }
 
-// bit 0, 1, 2: rows of k, of q, and of V contiguous values start on 16 bytes and hold whole groups of eight
-static int aligned(const InetDelta* a) {
+// whether the inputs' rows start on 16 bytes and hold whole groups of eight
+static bool aligned(const InetDelta* a) {
     const int e = elem_size(a->dtype);
     auto rows = [&](const void* p, const int64_t* s) {
-        return a->K % 8 == 0 && (uintptr_t)p % 16 == 0 && s[0] * e % 16 == 0 && s[1] * e % 16 == 0 && s[2] * e % 16 == 0;
+        return (uintptr_t)p % 16 == 0 && s[0] * e % 16 == 0 && s[1] * e % 16 == 0 && s[2] * e % 16 == 0;
     };
-    return (rows(a->k, a->k_s) ? 1 : 0) | (rows(a->q, a->q_s) ? 2 : 0);
+    return a->K % 8 == 0 && a->V % 8 == 0 && rows(a->k, a->k_s) && rows(a->q, a->q_s) && rows(a->v, a->v_s);
 }
 
 }  // namespace pol
@@ -154,7 +155,7 @@ int32_t inet_policy_delta_forward(const InetDelta* a, void* stream) {
     if (a->B == 0) return INET_POLICY_OK;
     if (!a->state_out || a->state == a->state_out) return INET_POLICY_EINVAL;
     if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o)) return INET_POLICY_EINVAL;
-    return pol::delta_forward(*a, pol::aligned(a), (hipStream_t)stream);
+    return pol::delta_forward(*a, pol::aligned(a) && (uintptr_t)a->o % 16 == 0, (hipStream_t)stream);
 }
 
 int32_t inet_policy_delta_backward(const InetDelta* a, const InetDeltaGrad* d, void* stream) {
@@ -165,10 +166,11 @@ int32_t inet_policy_delta_backward(const InetDelta* a, const InetDeltaGrad* d, v
                      !d->d_v || !d->d_g || !d->d_beta || !d->chunk_grad || !d->err_grad))
         return INET_POLICY_EINVAL;
     if (a->H != a->Hk && a->T > 0 && !d->head_grad) return INET_POLICY_EINVAL;
-    int vec = pol::aligned(a);
-    if (a->V % 8 == 0 && (uintptr_t)a->err % 16 == 0 && (uintptr_t)d->err_grad % 16 == 0 && (uintptr_t)d->d_o % 16 == 0 &&
-        (uintptr_t)a->chunk_state % 16 == 0 && (uintptr_t)d->chunk_grad % 16 == 0)
-        vec |= 4;
+    bool vec = pol::aligned(a);
+    for (const void* p : {(const void*)a->err, (const void*)a->chunk_state, (const void*)d->err_grad, d->d_o,
+                          (const void*)d->chunk_grad, (const void*)d->d_q, (const void*)d->d_k, (const void*)d->d_v,
+                          (const void*)d->head_grad})
+        vec = vec && (uintptr_t)p % 16 == 0;
     return pol::delta_backward(*a, *d, vec, (hipStream_t)stream);
 }
 

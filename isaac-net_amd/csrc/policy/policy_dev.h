@@ -39,13 +39,16 @@ template <typename T> DEV void load8(const T* __restrict__ p, int n, bool vec, f
     if (vec && n >= 8) {
         if constexpr (sizeof(T) == 4) {
             const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
             for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
         } else {
             typedef T V8 __attribute__((ext_vector_type(8)));
             const V8 a = *(const V8*)p;
+#pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
         }
     } else {
+#pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
@@ -55,8 +58,10 @@ template <typename T> DEV void load4(const T* __restrict__ p, int n, bool vec, f
     if (vec && n >= 4) {
         typedef T V4 __attribute__((ext_vector_type(4)));
         const V4 a = *(const V4*)p;
+#pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = (float)a[i];
     } else {
+#pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = i < n ? (float)p[i] : 0.0f;
     }
 }
@@ -66,8 +71,11 @@ template <int N> struct Frag { bf16x8 p[N]; };
 template <int N> DEV Frag<N> split8(const float (&x)[8]) {
     Frag<N> f;
     float r[8];
+#pragma unroll
     for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
     for (int i = 0; i < N; ++i)
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
             const __bf16 h = (__bf16)r[e];
             f.p[i][e] = h;
@@ -102,6 +110,15 @@ DEV f32x4 mma32(f32x4 a, f32x4 b, f32x4 c) {
 // place of contraction index c in the order of two stacked results
 DEV int perm(int c) { return (c & ~31) | ((c & 12) << 1) | ((c & 16) >> 2) | (c & 3); }
 
+// four rows x 16 columns of 16-bit values in LDS, transposed: lanes 0..15 of a group point to four values each (lane n:
+// row n / 4, columns 4 (n % 4) ..), and lane n receives column n
+DEV bf16x4 read_tr(const __bf16* p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* Lds;
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)p);
+    return __builtin_bit_cast(bf16x4, v);
+}
+
 // a matrix of N planes in LDS, rows of ld elements (ld / 8 odd: 16 lanes' 16-byte reads fall on distinct banks)
 template <int N> struct Planes {
     __bf16* p;
@@ -112,24 +129,48 @@ template <int N> struct Planes {
         for (int i = 0; i < N; ++i) f.p[i] = *(const bf16x8*)(p + i * plane + row * ld + k8);
         return f;
     }
-    DEV void put(int row, int place, float x) const {
+    // the A fragment of the transpose: row 16 ct + n of it, contraction over rows 32 rp .. 32 rp + 31 in the order of two
+    // stacked results. The matrix's columns are in the order perm().
+    DEV Frag<N> tr_frag(int ct, int rp, int n, int g) const {
+        Frag<N> f;
+        const __bf16* at = p + (32 * rp + 4 * g + (n >> 2)) * ld + 32 * (ct >> 1) + (n & 3) * 8 + (ct & 1) * 4;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const __bf16 h = (__bf16)x;
-            p[i * plane + row * ld + place] = h;
-            x -= (float)h;
+            const bf16x4 lo = read_tr(at + i * plane), hi = read_tr(at + i * plane + 16 * ld);
+            f.p[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
+        return f;
     }
     DEV void put4(int row, int place, float a, float b, float c, float d) const {
         float x[4] = {a, b, c, d};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             bf16x4 h;
+#pragma unroll
             for (int e = 0; e < 4; ++e) { h[e] = (__bf16)x[e]; x[e] -= (float)h[e]; }
             *(bf16x4*)(p + i * plane + row * ld + place) = h;
         }
     }
 };
+
+// inclusive sum over the wave's lanes
+template <int CTRL, int ROWS> DEV int lane_shift(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, true);
+}
+template <int CTRL, int ROWS> DEV double lane_shift(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)lane_shift<CTRL, ROWS>((int)(uint32_t)u), hi = (uint32_t)lane_shift<CTRL, ROWS>((int)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <typename T> DEV T lane_scan(T x) {
+    x += lane_shift<0x111, 0xf>(x);          // one, two, four, eight lanes along a row of 16
+    x += lane_shift<0x112, 0xf>(x);
+    x += lane_shift<0x114, 0xf>(x);
+    x += lane_shift<0x118, 0xf>(x);
+    x += lane_shift<0x142, 0xa>(x);          // rows 1 and 3 gain the last lane of the row before
+    x += lane_shift<0x143, 0xc>(x);          // rows 2 and 3 that of row 1
+    return x;
+}
 
 template <typename T> DEV void store4(T* p, int n, bool vec, const float (&x)[4]) {
     if (vec && n >= 4) {
