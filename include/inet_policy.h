@@ -55,8 +55,9 @@ typedef struct InetDelta {
     const float *state;                         /* [B][H][K][V], or NULL: empty */
     void *o;
     float *state_out;                           /* may not overlap state */
-    /* kept by the forward pass for the backward pass (NULL: not kept): the state at each chunk's start
-       [B][H][chunks][K][V], and the prediction errors v_t - (d_t S_{t-1})^T k_t, [B][T][H][V] */
+    /* kept by the forward pass for the backward pass: the prediction errors v_t - (d_t S_{t-1})^T k_t, [B][T][H][V] (NULL:
+       neither is kept), and the state at the start of each chunk but the first, [B][H][chunks - 1][K][V] (NULL where
+       there is one chunk). The backward pass takes `state` too. */
     float *chunk_state, *err;
 } InetDelta;
 
@@ -66,8 +67,8 @@ typedef struct InetDeltaGrad {
     const float *d_state_out;
     void *d_q, *d_k, *d_v, *d_g, *d_beta;
     float *d_state;                             /* or NULL: not wanted */
-    /* workspaces: gradient of each chunk's end state (as chunk_state), of the errors (as err), and where H > Hk the
-       heads' own d_q and d_k in 32 bits, [2][B][T][H][K] */
+    /* workspaces: gradient of the state after each chunk but the last (as chunk_state), of the errors (as err; both NULL
+       where there is one chunk), and where H > Hk the heads' own d_q and d_k in 32 bits, [2][B][T][H][K] */
     float *chunk_grad, *err_grad, *head_grad;
 } InetDeltaGrad;
 

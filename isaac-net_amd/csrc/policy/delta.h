@@ -133,6 +133,16 @@ template <typename T, int C, int KP, bool VEC> struct Rows {
             if (GR % DELTA_WG == 0 || i < GR) *(V8*)(s + r * ld + c) = v[m];
         }
     }
+    template <int N> DEV void put_natural(const Planes<N>& s) const {       // columns in their own order
+#pragma unroll
+        for (int m = 0; m < NL; ++m) {
+            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            if (GR % DELTA_WG == 0 || i < GR) {
+                s.put4(r, c, (float)v[m][0], (float)v[m][1], (float)v[m][2], (float)v[m][3]);
+                s.put4(r, c + 4, (float)v[m][4], (float)v[m][5], (float)v[m][6], (float)v[m][7]);
+            }
+        }
+    }
     template <int N> DEV void put(const Planes<N>& s) const {
 #pragma unroll
         for (int m = 0; m < NL; ++m) {

@@ -1,18 +1,118 @@
-// Backward pass of the gated delta rule over windows (the mathematics: delta.h), in two kernels: the state's gradient
-// goes backwards through a window chunk by chunk, column tile by column tile, as the forward pass goes forwards, and
-// leaves each chunk's dS and Z; with those, every chunk's gradients of q, k and the gates are independent, and one
-// workgroup a chunk computes them.
+// Backward pass of the gated delta rule over windows (the mathematics: delta.h). A window of one chunk is one kernel's
+// (delta_window_kernel). Longer ones take two: the state's gradient goes backwards through a window chunk by chunk, column
+// tile by column tile, as the forward pass goes forwards, and leaves each chunk's dS and Z (delta_scan_kernel); with
+// those, every chunk's gradients of q, k and the gates are independent, and one workgroup a chunk computes them
+// (delta_chunk_kernel).
 #include "delta.h"
 #include "delta_launch.h"
 
 namespace pol {
+
+// 16 columns (from c0 on) of a chunk's dO from its rows' planes
+template <int N> DEV f32x4 plane_tile(const Planes<N>& s, int row0, int c0, int n, int g) {
+    f32x4 x = {};
+#pragma unroll
+    for (int m = N - 1; m >= 0; --m)
+        x += tile_at<__bf16>(s.p + m * s.plane + row0 * s.ld + c0, s.ld, n, g);
+    return x;
+}
+
+// rows of values [steps][V] into planes in their own order, zeros up to vp columns
+template <typename T, int C, bool VEC, int N>
+DEV void stage_rows(const T* __restrict__ x, int64_t row0, int64_t row_s, int steps, int V, int vp, const Planes<N>& s) {
+    for (int i = threadIdx.x; i < C * (vp / 8); i += DELTA_WG) {
+        const int r = i / (vp / 8), c = i % (vp / 8) * 8;
+        float o[8] = {};
+        if (x && r < steps && c < V) load8(x + row0 + r * row_s + c, V - c, VEC, o);
+        s.put4(r, c, o[0], o[1], o[2], o[3]);
+        s.put4(r, c + 4, o[4], o[5], o[6], o[7]);
+    }
+}
+
+// 16 columns of a chunk: Z from the gradient S of the state after the chunk (has_s; else zero) and dO (u, read here)
+template <int C, int KP, int NP>
+DEV void column_gradients(const f32x4 (&S)[KP / 16], bool has_s, f32x4 (&z)[C / 16], f32x4 (&u)[C / 16],
+                          const Gates<C>& gates, const float* ln, int ld, const Planes<NP>& Kr, const Planes<3>& P,
+                          const Planes<NP>& O, int c0, int n, int g) {
+    constexpr int RT = C / 16, KT = KP / 16;
+    // dX = c K dS + P^T dO
+    if (has_s) {
+#pragma unroll
+        for (int kp = 0; kp < KT / 2; ++kp) {
+            const Frag<3> sf = split_tiles<3>(S[2 * kp], S[2 * kp + 1]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) z[rt] = mma<2>(Kr.frag(rt * 16 + n, kp * 32 + 8 * g), sf, z[rt]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const f32x4 c = *(const f32x4*)(gates.c + rt * 16 + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[rt][e] = c[e] != 0.0f ? c[e] * z[rt][e] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) u[rt] = plane_tile(O, rt * 16, c0, n, g);
+#pragma unroll
+    for (int kp = 0; kp < RT / 2; ++kp) {
+        const Frag<NP> uf = split_tiles<NP>(u[2 * kp], u[2 * kp + 1]);
+#pragma unroll
+        for (int rt = 0; rt < 2 * kp + 2; ++rt) z[rt] = mma<2>(P.tr_frag(rt, kp, n, g), uf, z[rt]);
+    }
+    // Z, block row by block row from the end
+#pragma unroll
+    for (int rt = RT - 1; rt >= 0; --rt) {
+        f32x4 acc = z[rt], a;
+#pragma unroll
+        for (int m = rt + 1; m < RT; ++m) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = ln[(m * 16 + 4 * g + e) * ld + rt * 16 + n];
+            acc = mma32(a, z[m], acc);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = ln[(rt * 16 + 4 * g + e) * ld + rt * 16 + n];
+        z[rt] = mma32(a, acc, f32x4{});
+    }
+}
+
+// S, the gradient of the state after a chunk, to that of the state before it: a_C S + Q^T (scale a dO) - K^T (a beta Z)
+template <int C, int KP, int NP>
+DEV void state_gradient(f32x4 (&S)[KP / 16], const f32x4 (&z)[C / 16], const f32x4 (&u)[C / 16], const Gates<C>& gates,
+                        float scale, const Planes<NP>& Kr, const Planes<NP>& Qr, int n, int g) {
+    constexpr int RT = C / 16, KT = KP / 16;
+    const float a_end = gates.a_end;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
+#pragma unroll
+    for (int kp = 0; kp < RT / 2; ++kp) {
+        f32x4 o[2], y[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const f32x4 a = *(const f32x4*)(gates.a + kp * 32 + 16 * m + 4 * g),
+                        bt = *(const f32x4*)(gates.beta + kp * 32 + 16 * m + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[m][e] = scale * a[e] * u[2 * kp + m][e];
+                y[m][e] = a[e] != 0.0f ? -bt[e] * a[e] * z[2 * kp + m][e] : 0.0f;
+            }
+        }
+        const Frag<3> of = split_tiles<3>(o[0], o[1]), yf = split_tiles<3>(y[0], y[1]);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            S[kt] = mma<2>(Qr.tr_frag(kt, kp, n, g), of, S[kt]);
+            S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), yf, S[kt]);
+        }
+    }
+}
 
 template <typename T, int C, int KP> struct ScanLds {
     static constexpr int NP = Elem<T>::planes, LK = KP + 8, LC = C + 8, LL = C + 4;
     Gates<C> gates;
     alignas(16) __bf16 k[NP * C * LK], q[NP * C * LK], p[3 * C * LC];
     alignas(16) float ln[C * LL];
-    alignas(16) T u[C * LV], v[C * LV];
+    alignas(16) __bf16 u[NP * C * LV];
+    alignas(16) T v[C * LV];
 };
 
 // The state's gradient. One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns.
@@ -25,6 +125,7 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
     Lds& s = *(Lds*)lds_raw;
     const Planes<NP> Kr{s.k, Lds::LK, C * Lds::LK}, Qr{s.q, Lds::LK, C * Lds::LK};
     const Planes<3> P{s.p, Lds::LC, C * Lds::LC};
+    const Planes<NP> O{s.u, LV, C * LV};
     const int b = blockIdx.x / d.H, h = blockIdx.x % d.H, hk = h / (d.H / d.Hk);
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int c0 = blockIdx.y * 64, width = d.V - c0 < 64 ? d.V - c0 : 64;      // the workgroup's columns
@@ -53,50 +154,15 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
         const int t0 = ch * C;
         kr.put(Kr);
         qr.put(Qr);
-        ur.put(s.u, LV);
+        ur.put_natural(O);
         if (w == 0) put_gates<C>(s.gates, gate);
         __syncthreads();
         keep(at), keep(at_err);
         triangles<C, KP, NP, 3, true>(Kr, Qr, P, s.gates, s.ln, Lds::LL, d.scale, w, n, g);
         if (ch) fetch(t0 - C);
         if (cols) {
-            // dX = c K dS + P^T dO
-            f32x4 z[RT] = {};
-#pragma unroll
-            for (int kp = 0; kp < KT / 2; ++kp) {
-                const Frag<3> sf = split_tiles<3>(S[2 * kp], S[2 * kp + 1]);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) z[rt] = mma<2>(Kr.frag(rt * 16 + n, kp * 32 + 8 * g), sf, z[rt]);
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const f32x4 c = *(const f32x4*)(s.gates.c + rt * 16 + 4 * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) z[rt][e] = c[e] != 0.0f ? c[e] * z[rt][e] : 0.0f;
-            }
-            f32x4 u[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) u[rt] = tile_at(s.u + rt * 16 * LV + w * 16, LV, n, g);
-#pragma unroll
-            for (int kp = 0; kp < RT / 2; ++kp) {
-                const Frag<NP> uf = split_tiles<NP>(u[2 * kp], u[2 * kp + 1]);
-#pragma unroll
-                for (int rt = 0; rt < 2 * kp + 2; ++rt) z[rt] = mma<2>(P.tr_frag(rt, kp, n, g), uf, z[rt]);
-            }
-            // Z, block row by block row from the end
-#pragma unroll
-            for (int rt = RT - 1; rt >= 0; --rt) {
-                f32x4 acc = z[rt], a;
-#pragma unroll
-                for (int m = rt + 1; m < RT; ++m) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) a[e] = s.ln[(m * 16 + 4 * g + e) * Lds::LL + rt * 16 + n];
-                    acc = mma32(a, z[m], acc);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = s.ln[(rt * 16 + 4 * g + e) * Lds::LL + rt * 16 + n];
-                z[rt] = mma32(a, acc, f32x4{});
-            }
+            f32x4 z[RT] = {}, u[RT];
+            column_gradients<C, KP, NP>(S, true, z, u, s.gates, s.ln, Lds::LL, Kr, P, O, w * 16, n, g);
             if (mine) {
                 float* zs = gr.err_grad + rows0 + t0 * row_s;
 #pragma unroll
@@ -104,38 +170,13 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (t0 + rt * 16 + 4 * g + e < d.T) zs[at_err + (uint32_t)((rt * 16 + e) * row_s)] = z[rt][e];
-                state_store(S, gr.chunk_grad + (bh * chunks + ch) * d.K * d.V + c0, at, d.V, d.K, g);
+                if (ch + 1 < chunks)
+                    state_store(S, gr.chunk_grad + (bh * (chunks - 1) + ch) * d.K * d.V + c0, at, d.V, d.K, g);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
                 tile_put(s.v + rt * 16 * LV + w * 16, LV, n, g, z[rt] * *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g));
-            if (ch || gr.d_state) {
-                const float a_end = s.gates.a_end;
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
-#pragma unroll
-                for (int kp = 0; kp < RT / 2; ++kp) {
-                    f32x4 o[2], y[2];
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const f32x4 a = *(const f32x4*)(s.gates.a + kp * 32 + 16 * m + 4 * g),
-                                    bt = *(const f32x4*)(s.gates.beta + kp * 32 + 16 * m + 4 * g);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            o[m][e] = d.scale * a[e] * u[2 * kp + m][e];
-                            y[m][e] = a[e] != 0.0f ? -bt[e] * a[e] * z[2 * kp + m][e] : 0.0f;
-                        }
-                    }
-                    const Frag<3> of = split_tiles<3>(o[0], o[1]), yf = split_tiles<3>(y[0], y[1]);
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        S[kt] = mma<2>(Qr.tr_frag(kt, kp, n, g), of, S[kt]);
-                        S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), yf, S[kt]);
-                    }
-                }
-            }
+            if (ch || gr.d_state) state_gradient<C, KP, NP>(S, z, u, s.gates, d.scale, Kr, Qr, n, g);
         }
         __syncthreads();
         store_rows<T, C, VEC>(s.v, (T*)gr.d_v + rows0 + t0 * row_s, row_s, d.T - t0, width);
@@ -143,96 +184,68 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
     if (mine && gr.d_state) state_store(S, gr.d_state + bh * d.K * d.V + c0, at, d.V, d.K, g);
 }
 
-constexpr int VMAX = INET_POLICY_MAX_HEAD;
+// the rows' sums that the log-decays' gradients are made of: q . dQ, k . dK+, k . dK-, the state's share of k . dK- (each by
+// the key rows' part), E . Z, and <S, dS> by wave
+template <int C> struct Sums {
+    float q[4][C], kp[4][C], km[4][C], ks[4][C], ez[C], ss[4];
+};
 
-// LDS of the chunk kernel in bytes: K and Q, X, Z and dO by rows (of vp + 8), gates and partial sums
+// LDS of the chunk kernel in bytes: K and Q, X, Z and dO by rows (of vp + 8), gates and sums
 template <typename T, int C, int KP> constexpr size_t chunk_lds(int vp) {
     constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1;
-    return sizeof(Gates<C>) + (5 * 4 * C + 8) * sizeof(float) +
-           sizeof(__bf16) * (2 * NP * C * (KP + 8) + (2 * NO + NP) * C * (vp + 8));
+    return sizeof(Gates<C>) + sizeof(Sums<C>) + sizeof(__bf16) * (2 * NP * C * (KP + 8) + (2 * NO + NP) * C * (vp + 8));
 }
 
-// eight consecutive values of a 32-bit matrix's row as an operand
-template <int N> DEV Frag<N> row_frag(const float* __restrict__ p, bool in, int v, int V, bool vec) {
-    float x[8] = {};
+// X = beta E and dbeta's E . Z by rows, Z from memory (err_grad) where z_in, else as it is in LDS already
+template <typename T, int C, bool VEC, int NO>
+DEV void stage_errors(const InetDelta& d, const float* z_in, int64_t row0, int64_t row_s, int steps, int vp,
+                      const Gates<C>& gates, const Planes<NO>& X, const Planes<NO>& Z, Sums<C>& sums) {
+    const int lanes = vp <= 32 ? 4 : vp <= 64 ? 8 : 16;             // a row
+    for (int i = threadIdx.x; i < C * lanes; i += DELTA_WG) {
+        const int r = i / lanes, c = i % lanes * 8;
+        float e[8] = {}, z[8] = {}, x = 0.0f;
+        if (r < steps && c < d.V) load8(d.err + row0 + r * row_s + c, d.V - c, VEC, e);
+        if (c < vp) {
+            if (z_in) {
+                if (r < steps && c < d.V) load8(z_in + row0 + r * row_s + c, d.V - c, VEC, z);
+                Z.put4(r, c, z[0], z[1], z[2], z[3]);
+                Z.put4(r, c + 4, z[4], z[5], z[6], z[7]);
+            } else {
+                const Frag<NO> f = Z.frag(r, c);
+#pragma unroll
+                for (int m = 0; m < NO; ++m)
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) z[u] += (float)f.p[m][u];
+            }
+            const float beta = gates.beta[r];
+            X.put4(r, c, beta * e[0], beta * e[1], beta * e[2], beta * e[3]);
+            X.put4(r, c + 4, beta * e[4], beta * e[5], beta * e[6], beta * e[7]);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x += e[u] * z[u];
+        for (int o = 1; o < lanes; o <<= 1) x += __shfl_xor(x, o);
+        if (c == 0) sums.ez[r] = x;
+    }
+}
+
+// eight consecutive values of a 32-bit matrix's row
+DEV void row8(const float* __restrict__ p, bool in, int v, int V, bool vec, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.0f;
     if (in && v < V) load8(p + v, V - v, vec, x);
-    return split8<N>(x);
 }
 
-// The gradients of q, k and the gates of one chunk. Wave w takes the steps of tile w % RT as its columns, and the key
-// rows' tiles w / RT, w / RT + 4 / RT, ...
-template <typename T, int C, int KP, bool VEC>
-__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
-    constexpr int NP = Elem<T>::planes, ORD = Elem<T>::ord, NO = ORD + 1, RT = C / 16, KT = KP / 16, PARTS = 4 / RT,
-                  LK = KP + 8;
-    extern __shared__ char lds_raw[];
-    const int vp = (d.V + 31) & ~31, lv = vp + 8;
-    Gates<C>& gates = *(Gates<C>*)lds_raw;
-    float* sums = (float*)(lds_raw + sizeof(Gates<C>));     // [5][4 parts][C] and the state's share [4], then pad
-    __bf16* pool = (__bf16*)(sums + 5 * 4 * C + 8);
-    const Planes<NP> Kr{pool, LK, C * LK}, Qr{pool + NP * C * LK, LK, C * LK};
-    __bf16* rows = pool + 2 * NP * C * LK;
-    const Planes<NO> X{rows, lv, C * lv}, Z{rows + NO * C * lv, lv, C * lv};
-    const Planes<NP> O{rows + 2 * NO * C * lv, lv, C * lv};
-    const int chunks = (d.T + C - 1) / C, ch = blockIdx.x % chunks, t0 = ch * C;
-    const int64_t bh = blockIdx.x / chunks;
-    const int b = (int)(bh / d.H), h = (int)(bh % d.H), hk = h / (d.H / d.Hk);
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+// The gradients of q, k and the gates of one chunk, from K, Q, X, Z and dO in LDS and the state S before the chunk and its
+// gradient dS after it (NULL: zero). Wave w takes the steps of tile w % RT as its columns, and the key rows' tiles
+// w / RT, w / RT + 4 / RT, ...
+template <typename T, int C, int KP, bool VEC, int NP, int NO>
+DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int h, int t0, const float* __restrict__ S,
+                         const float* __restrict__ dS, const Gates<C>& gates, Sums<C>& sums, const Planes<NP>& Kr,
+                         const Planes<NP>& Qr, const Planes<NO>& X, const Planes<NO>& Z, const Planes<NP>& O, int vp) {
+    constexpr int ORD = Elem<T>::ord, RT = C / 16, KT = KP / 16, PARTS = 4 / RT;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, hk = h / (d.H / d.Hk);
     const T* q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2];
     const T* k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2];
-    const float* S = d.chunk_state + (bh * chunks + ch) * d.K * d.V;
-    const float* dS = gr.chunk_grad + (bh * chunks + ch) * d.K * d.V;
-
-    {
-        Rows<T, C, KP, VEC> kr, qr;
-        Gate gate;
-        kr.load(k, d.k_s[1], t0, d.T, d.K);
-        qr.load(q, d.q_s[1], t0, d.T, d.K);
-        if (w == 0) {
-            gate.load<C>(d, b, h, t0);
-            put_gates<C>(gates, gate);
-        }
-        kr.put(Kr);
-        qr.put(Qr);
-    }
-    __syncthreads();
-    // X = beta E, Z and dO by rows; dbeta's E . Z and <S, dS> on the way
-    for (int i = threadIdx.x; i < C * (vp / 8); i += DELTA_WG) {
-        const int r = i / (vp / 8), c = i % (vp / 8) * 8, t = t0 + r;
-        float e[8] = {}, z[8] = {}, o[8] = {};
-        if (t < d.T && c < d.V) {
-            const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.V + c;
-            load8(d.err + at, d.V - c, VEC, e);
-            load8((const float*)gr.err_grad + at, d.V - c, VEC, z);
-            if (gr.d_o) load8((const T*)gr.d_o + at, d.V - c, VEC, o);
-        }
-        const float beta = gates.beta[r];
-        X.put4(r, c, beta * e[0], beta * e[1], beta * e[2], beta * e[3]);
-        X.put4(r, c + 4, beta * e[4], beta * e[5], beta * e[6], beta * e[7]);
-        Z.put4(r, c, z[0], z[1], z[2], z[3]);
-        Z.put4(r, c + 4, z[4], z[5], z[6], z[7]);
-        O.put4(r, c, o[0], o[1], o[2], o[3]);
-        O.put4(r, c + 4, o[4], o[5], o[6], o[7]);
-    }
-    float ss = 0.0f;
-    if (gates.a_end != 0.0f)
-        for (int i = threadIdx.x; i < d.K * d.V; i += DELTA_WG) ss += S[i] * dS[i];
-    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
-    if (lane == 0) sums[5 * 4 * C + w] = ss;
-    // dbeta: four lanes a step
-    {
-        const int r = threadIdx.x >> 2, part = threadIdx.x & 3, t = t0 + r;
-        float x = 0.0f;
-        if (r < C && t < d.T) {
-            const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.V;
-            for (int c = part; c < d.V; c += 4) x += d.err[at + c] * gr.err_grad[at + c];
-        }
-        x += __shfl_xor(x, 1);
-        x += __shfl_xor(x, 2);
-        if (r < C && part == 0) sums[4 * 4 * C + r] = x;
-    }
-    __syncthreads();
-
     const int tt = w % RT, part = w / RT, i0 = tt * 16 + n;         // the wave's steps; this lane's
     // the triangles' columns of this wave's steps, as operands: dt: D^T[j][i0]; dn: D[i][i0]; mt: M^T[i][i0] ([i < i0]:
     // M[i0][i]); mn: M[i][i0]
@@ -290,19 +303,29 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_c
     }
     const float a = gates.a[i0], c = gates.c[i0], ya = -beta * a, oa = d.scale * a;
     const int t = t0 + i0;
-    float sq = 0.0f, sp = 0.0f, sn = 0.0f, sc = 0.0f;
+    float sq = 0.0f, sp = 0.0f, sn = 0.0f, sc = 0.0f, ss = 0.0f;
     for (int kt = part; kt < KT; kt += PARTS) {
         if (kt * 16 >= d.K) continue;
         const int row = kt * 16 + n;
         f32x4 dq = {}, dp = {}, dm = {};
         for (int v = 0; v < vp; v += 32) {
-            const Frag<NO> sf = row_frag<NO>(S + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC);
-            const Frag<NO> df = row_frag<NO>(dS + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC);
-            dq = mma<ORD>(sf, O.frag(i0, v + 8 * g), dq);
-            dp = mma<ORD>(sf, Z.frag(i0, v + 8 * g), dp);
-            dm = mma<ORD>(df, X.frag(i0, v + 8 * g), dm);
+            float x[8], y[8];
+            if (S) {
+                row8(S + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC, x);
+                const Frag<NO> sf = split8<NO>(x);
+                dq = mma<ORD>(sf, O.frag(i0, v + 8 * g), dq);
+                dp = mma<ORD>(sf, Z.frag(i0, v + 8 * g), dp);
+            }
+            if (dS) {
+                row8(dS + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC, y);
+                dm = mma<ORD>(split8<NO>(y), X.frag(i0, v + 8 * g), dm);
+            }
+            if (S && dS && tt == 0)
+#pragma unroll
+                for (int u = 0; u < 8; ++u) ss += x[u] * y[u];
         }
         f32x4 dc;
+#pragma unroll
         for (int e = 0; e < 4; ++e) {
             dq[e] = a != 0.0f ? dq[e] * oa : 0.0f;
             dp[e] = a != 0.0f ? dp[e] * ya : 0.0f;
@@ -322,6 +345,7 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_c
             float qv[4], kv[4], dk[4], dqv[4];
             load4(q + t * d.q_s[1] + kd, d.K - kd, VEC, qv);
             load4(k + t * d.k_s[1] + kd, d.K - kd, VEC, kv);
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
                 sq += dq[e] * qv[e];
                 sp += dp[e] * kv[e];
@@ -340,12 +364,14 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_c
             }
         }
     }
-    float* p[4] = {&sq, &sp, &sn, &sc};
-    for (int m = 0; m < 4; ++m) {
-        *p[m] += __shfl_xor(*p[m], 16);
-        *p[m] += __shfl_xor(*p[m], 32);
-        if (g == 0) sums[(m * 4 + part) * C + i0] = *p[m];
-    }
+    auto give = [&](float x, float (&to)[4][C]) {
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        if (g == 0) to[part][i0] = x;
+    };
+    give(sq, sums.q), give(sp, sums.kp), give(sn, sums.km), give(sc, sums.ks);
+    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
+    if (lane == 0) sums.ss[w] = ss;
     __syncthreads();
     if (w == 0) {
         const int step = t0 + lane;
@@ -353,17 +379,16 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_c
         int seg = -1;
         if (lane < C) {
             seg = gates.seg[lane];
+#pragma unroll
             for (int m = 0; m < PARTS; ++m) {
-                x += sums[(0 + m) * C + lane] + sums[(4 + m) * C + lane] - sums[(8 + m) * C + lane];
-                e += sums[(12 + m) * C + lane];
+                x += sums.q[m][lane] + sums.kp[m][lane] - sums.km[m][lane];
+                e += sums.ks[m][lane];
             }
         }
         // the state's share, at the last step
         for (int o = 32; o; o >>= 1) e += __shfl_xor(e, o);
-        if (lane == C - 1) {
-            const float* sh = sums + 5 * 4 * C;
-            x += e + (gates.a_end != 0.0f ? gates.a_end * (sh[0] + sh[1] + sh[2] + sh[3]) : 0.0f);
-        }
+        if (lane == C - 1)
+            x += e + (gates.a_end != 0.0f ? gates.a_end * (sums.ss[0] + sums.ss[1] + sums.ss[2] + sums.ss[3]) : 0.0f);
         for (int o = 1; o < C; o <<= 1) {
             const float u = __shfl_down(x, o);
             const int sg = __shfl_down(seg, o);
@@ -372,12 +397,143 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_c
         if (lane < C && step < d.T) {
             const bool cut = lane ? gates.seg[lane] != gates.seg[lane - 1] : gates.seg[0] != 0;
             const int64_t at = ((int64_t)b * d.T + step) * d.H + h;
-            const float dg = cut ? 0.0f : x, db = sums[4 * 4 * C + lane];
-            if (d.gate_dtype == INET_POLICY_F32) { ((float*)gr.d_g)[at] = dg; ((float*)gr.d_beta)[at] = db; }
-            else if (d.gate_dtype == INET_POLICY_BF16) { ((__bf16*)gr.d_g)[at] = (__bf16)dg; ((__bf16*)gr.d_beta)[at] = (__bf16)db; }
-            else { ((_Float16*)gr.d_g)[at] = (_Float16)dg; ((_Float16*)gr.d_beta)[at] = (_Float16)db; }
+            const float dg = cut ? 0.0f : x, db = sums.ez[lane];
+            if (d.gate_dtype == INET_POLICY_F32) {
+                ((float*)gr.d_g)[at] = dg;
+                ((float*)gr.d_beta)[at] = db;
+            } else if (d.gate_dtype == INET_POLICY_BF16) {
+                ((__bf16*)gr.d_g)[at] = (__bf16)dg;
+                ((__bf16*)gr.d_beta)[at] = (__bf16)db;
+            } else {
+                ((_Float16*)gr.d_g)[at] = (_Float16)dg;
+                ((_Float16*)gr.d_beta)[at] = (_Float16)db;
+            }
         }
     }
+}
+
+template <typename T, int C, int KP, bool VEC>
+__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
+void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
+    constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1, LK = KP + 8;
+    extern __shared__ char lds_raw[];
+    const int vp = (d.V + 31) & ~31, lv = vp + 8;
+    Gates<C>& gates = *(Gates<C>*)lds_raw;
+    Sums<C>& sums = *(Sums<C>*)(lds_raw + sizeof(Gates<C>));
+    __bf16* pool = (__bf16*)(lds_raw + sizeof(Gates<C>) + sizeof(Sums<C>));
+    const Planes<NP> Kr{pool, LK, C * LK}, Qr{pool + NP * C * LK, LK, C * LK};
+    __bf16* rows = pool + 2 * NP * C * LK;
+    const Planes<NO> X{rows, lv, C * lv}, Z{rows + NO * C * lv, lv, C * lv};
+    const Planes<NP> O{rows + 2 * NO * C * lv, lv, C * lv};
+    const int chunks = (d.T + C - 1) / C, ch = blockIdx.x % chunks, t0 = ch * C;
+    const int64_t bh = blockIdx.x / chunks, row_s = (int64_t)d.H * d.V;
+    const int b = (int)(bh / d.H), h = (int)(bh % d.H), hk = h / (d.H / d.Hk), steps = d.T - t0;
+    const int64_t row0 = ((int64_t)b * d.T + t0) * row_s + h * d.V;
+    {
+        Rows<T, C, KP, VEC> kr, qr;
+        Gate gate;
+        kr.load((const T*)d.k + b * d.k_s[0] + hk * d.k_s[2], d.k_s[1], t0, d.T, d.K);
+        qr.load((const T*)d.q + b * d.q_s[0] + hk * d.q_s[2], d.q_s[1], t0, d.T, d.K);
+        if (threadIdx.x < 64) {
+            gate.load<C>(d, b, h, t0);
+            put_gates<C>(gates, gate);
+        }
+        kr.put(Kr);
+        qr.put(Qr);
+    }
+    stage_rows<T, C, VEC, NP>((const T*)gr.d_o, row0, row_s, steps, d.V, vp, O);
+    __syncthreads();
+    stage_errors<T, C, VEC, NO>(d, gr.err_grad, row0, row_s, steps, vp, gates, X, Z, sums);
+    __syncthreads();
+    const int64_t kv = (int64_t)d.K * d.V, at = bh * (chunks - 1) + ch;
+    const float* S = ch ? d.chunk_state + (at - 1) * kv : d.state ? d.state + bh * kv : nullptr;
+    const float* dS = ch + 1 < chunks ? gr.chunk_grad + at * kv : gr.d_state_out ? gr.d_state_out + bh * kv : nullptr;
+    chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, t0, S, dS, gates, sums, Kr, Qr, X, Z, O, vp);
+}
+
+// LDS of the one-chunk kernel: the chunk kernel's, with X where the triangles and 64 columns of dV on their way out were
+// until the errors' gradients were known
+template <typename T, int C> constexpr size_t triangles_lds() {
+    return sizeof(__bf16) * 3 * C * (C + 8) + sizeof(float) * C * (C + 4) + sizeof(T) * C * LV;
+}
+template <typename T, int C, int KP> constexpr size_t window_lds(int vp) {
+    const size_t x = sizeof(__bf16) * (Elem<T>::ord + 1) * C * (vp + 8), t = triangles_lds<T, C>();
+    return chunk_lds<T, C, KP>(vp) + (t > x ? t - x : 0);
+}
+
+// The whole backward pass of a window of at most C steps, one workgroup a robot and head.
+template <typename T, int C, int KP, bool VEC>
+__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
+void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
+    constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1, LK = KP + 8, LC = C + 8, LL = C + 4, RT = C / 16,
+                  KT = KP / 16;
+    extern __shared__ char lds_raw[];
+    const int vp = (d.V + 31) & ~31, lv = vp + 8;
+    Gates<C>& gates = *(Gates<C>*)lds_raw;
+    Sums<C>& sums = *(Sums<C>*)(lds_raw + sizeof(Gates<C>));
+    __bf16* pool = (__bf16*)(lds_raw + sizeof(Gates<C>) + sizeof(Sums<C>));
+    const Planes<NP> Kr{pool, LK, C * LK}, Qr{pool + NP * C * LK, LK, C * LK};
+    __bf16* rows = pool + 2 * NP * C * LK;
+    const Planes<NO> Z{rows, lv, C * lv}, X{rows + (NO + NP) * C * lv, lv, C * lv};
+    const Planes<NP> O{rows + NO * C * lv, lv, C * lv};
+    const Planes<3> P{X.p, LC, C * LC};             // (X's place, until it is staged)
+    float* ln = (float*)(P.p + 3 * C * LC);
+    T* out = (T*)(ln + C * LL);
+    const int64_t bh = blockIdx.x, row_s = (int64_t)d.H * d.V, kv = (int64_t)d.K * d.V;
+    const int b = blockIdx.x / d.H, h = blockIdx.x % d.H, hk = h / (d.H / d.Hk);
+    const int64_t row0 = (int64_t)b * d.T * row_s + h * d.V;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    {
+        Rows<T, C, KP, VEC> kr, qr;
+        Gate gate;
+        kr.load((const T*)d.k + b * d.k_s[0] + hk * d.k_s[2], d.k_s[1], 0, d.T, d.K);
+        qr.load((const T*)d.q + b * d.q_s[0] + hk * d.q_s[2], d.q_s[1], 0, d.T, d.K);
+        if (w == 0) {
+            gate.load<C>(d, b, h, 0);
+            put_gates<C>(gates, gate);
+        }
+        kr.put(Kr);
+        qr.put(Qr);
+    }
+    stage_rows<T, C, VEC, NP>((const T*)gr.d_o, row0, row_s, d.T, d.V, vp, O);
+    __syncthreads();
+    triangles<C, KP, NP, 3, true>(Kr, Qr, P, gates, ln, LL, d.scale, w, n, g);
+    for (int c0 = 0; c0 < d.V; c0 += 64) {
+        const int width = d.V - c0 < 64 ? d.V - c0 : 64;
+        const bool mine = w * 16 + n < width;
+        const uint32_t at = (uint32_t)(4 * g * d.V + w * 16 + n);
+        if (c0 + w * 16 < vp) {                     // (columns from V up to vp: zeros)
+            f32x4 z[RT] = {}, u[RT], S[KT] = {};
+            if (mine && gr.d_state_out) state_load(S, gr.d_state_out + bh * kv + c0, at, d.V, d.K, g);
+            column_gradients<C, KP, NP>(S, gr.d_state_out != nullptr, z, u, gates, ln, LL, Kr, P, O, c0 + w * 16, n, g);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                tile_put(out + rt * 16 * LV + w * 16, LV, n, g, z[rt] * *(const f32x4*)(gates.beta + rt * 16 + 4 * g));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = z[rt][e];
+#pragma unroll
+                    for (int m = 0; m < NO; ++m) {
+                        const __bf16 y = (__bf16)x;
+                        Z.p[m * Z.plane + (rt * 16 + 4 * g + e) * lv + c0 + w * 16 + n] = y;
+                        x -= (float)y;
+                    }
+                }
+            }
+            if (gr.d_state) {
+                state_gradient<C, KP, NP>(S, z, u, gates, d.scale, Kr, Qr, n, g);
+                if (mine) state_store(S, gr.d_state + bh * kv + c0, at, d.V, d.K, g);
+            }
+        }
+        __syncthreads();
+        store_rows<T, C, VEC>(out, (T*)gr.d_v + row0 + c0, row_s, d.T, width);
+        __syncthreads();
+    }
+    stage_errors<T, C, VEC, NO>(d, nullptr, row0, row_s, d.T, vp, gates, X, Z, sums);
+    __syncthreads();
+    chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, 0, d.state ? d.state + bh * kv : nullptr,
+                                           gr.d_state_out ? gr.d_state_out + bh * kv : nullptr, gates, sums, Kr, Qr, X,
+                                           Z, O, vp);
 }
 
 // gradients of shared query and key heads: the value heads' own, summed in head order
@@ -398,18 +554,26 @@ __global__ __launch_bounds__(256) void delta_heads_kernel(const float* __restric
 
 template <typename T, int C, int KP, bool VEC>
 static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
-    const size_t lds = sizeof(ScanLds<T, C, KP>);
-    static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && chunk_lds<T, C, KP>(VMAX) <= LDS_MAX, "LDS");
-    auto scan = delta_scan_kernel<T, C, KP, VEC>;
-    auto chunk = delta_chunk_kernel<T, C, KP, VEC>;
-    const size_t cl = chunk_lds<T, C, KP>((d.V + 31) & ~31);
-    if (allow_lds((const void*)scan, lds) || allow_lds((const void*)chunk, cl)) return INET_POLICY_ELAUNCH;
-    hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
-    if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
-    const int chunks = (d.T + C - 1) / C;
-    if (!chunks) return INET_POLICY_OK;
-    hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), cl, st, d, g);
-    if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
+    const int chunks = (d.T + C - 1) / C, vp = (d.V + 31) & ~31;
+    constexpr int V_MOST = std::is_same<T, _Float16>::value && C == 64 ? 64 : INET_POLICY_MAX_HEAD;
+    static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && window_lds<T, C, KP>(V_MOST) <= LDS_MAX, "LDS");
+    if (chunks == 1) {
+        auto window = delta_window_kernel<T, C, KP, VEC>;
+        const size_t lds = window_lds<T, C, KP>(vp);
+        if (allow_lds((const void*)window, lds)) return INET_POLICY_ELAUNCH;
+        hipLaunchKernelGGL(window, dim3(d.B * d.H), dim3(DELTA_WG), lds, st, d, g);
+        if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
+    } else {
+        const size_t lds = sizeof(ScanLds<T, C, KP>), cl = chunk_lds<T, C, KP>(vp);
+        auto scan = delta_scan_kernel<T, C, KP, VEC>;
+        auto chunk = delta_chunk_kernel<T, C, KP, VEC>;
+        if (allow_lds((const void*)scan, lds) || allow_lds((const void*)chunk, cl)) return INET_POLICY_ELAUNCH;
+        hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
+        if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
+        if (!chunks) return INET_POLICY_OK;
+        hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), cl, st, d, g);
+        if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
+    }
     if (d.H != d.Hk) {
         const int64_t rows = (int64_t)d.B * d.T * d.Hk;
         hipLaunchKernelGGL(delta_heads_kernel<T>, dim3((unsigned)((rows * d.K + 255) / 256)), dim3(256), 0, st,

@@ -57,8 +57,8 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_f
         triangles<C, KP, NP, NO, false>(Kr, Qr, P, s.gates, s.ln, Lds::LL, d.scale, w, n, g);
         if (ch + 1 < chunks) fetch(t0 + C);
         if (cols) {
-            if (d.chunk_state && mine)
-                state_store(S, d.chunk_state + (bh * chunks + ch) * d.K * d.V + c0, at, d.V, d.K, g);
+            if (d.chunk_state && ch && mine)
+                state_store(S, d.chunk_state + (bh * (chunks - 1) + ch - 1) * d.K * d.V + c0, at, d.V, d.K, g);
             // K S to the last bits of 32, since the state goes on with it; Q S to the output's
             f32x4 x[RT] = {}, o[RT] = {};
 #pragma unroll

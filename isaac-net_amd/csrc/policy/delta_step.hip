@@ -146,7 +146,7 @@ extern "C" {
 int32_t inet_policy_delta_chunk(int32_t T, int32_t K, int32_t V, int32_t dtype) {
     if (T < 0 || K < 1 || V < 1 || K > INET_POLICY_MAX_HEAD || V > INET_POLICY_MAX_HEAD || dtype < 0 || dtype > 2)
         return 0;
-    if (dtype == INET_POLICY_F32 || (dtype == INET_POLICY_F16 && K > 64)) return 32;   // (LDS: delta_launch.h)
+    if (dtype == INET_POLICY_F32 || (dtype == INET_POLICY_F16 && (K > 64 || V > 64))) return 32;   // (LDS: delta_launch.h)
     return T <= 32 ? 32 : 64;
 }
 
@@ -155,6 +155,7 @@ int32_t inet_policy_delta_forward(const InetDelta* a, void* stream) {
     if (a->B == 0) return INET_POLICY_OK;
     if (!a->state_out || a->state == a->state_out) return INET_POLICY_EINVAL;
     if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o)) return INET_POLICY_EINVAL;
+    if (a->T > a->chunk && !a->err != !a->chunk_state) return INET_POLICY_EINVAL;
     return pol::delta_forward(*a, pol::aligned(a) && (uintptr_t)a->o % 16 == 0, (hipStream_t)stream);
 }
 
@@ -162,14 +163,15 @@ int32_t inet_policy_delta_backward(const InetDelta* a, const InetDeltaGrad* d, v
     if (int rc = pol::check_window(a)) return rc;
     if (!d) return INET_POLICY_EINVAL;
     if (a->B == 0 || (a->T == 0 && !d->d_state)) return INET_POLICY_OK;
-    if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->chunk_state || !a->err || !d->d_q || !d->d_k ||
-                     !d->d_v || !d->d_g || !d->d_beta || !d->chunk_grad || !d->err_grad))
+    if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->err || !d->d_q || !d->d_k || !d->d_v || !d->d_g ||
+                     !d->d_beta))
         return INET_POLICY_EINVAL;
+    if (a->T > a->chunk && (!a->chunk_state || !d->chunk_grad || !d->err_grad)) return INET_POLICY_EINVAL;
     if (a->H != a->Hk && a->T > 0 && !d->head_grad) return INET_POLICY_EINVAL;
     bool vec = pol::aligned(a);
     for (const void* p : {(const void*)a->err, (const void*)a->chunk_state, (const void*)d->err_grad, d->d_o,
                           (const void*)d->chunk_grad, (const void*)d->d_q, (const void*)d->d_k, (const void*)d->d_v,
-                          (const void*)d->head_grad})
+                          (const void*)d->head_grad, (const void*)a->state, (const void*)d->d_state_out})
         vec = vec && (uintptr_t)p % 16 == 0;
     return pol::delta_backward(*a, *d, vec, (hipStream_t)stream);
 }

@@ -125,19 +125,20 @@ class _DeltaRule(torch.autograd.Function):
         a.state, a.o, a.state_out = _ptr(state), o.data_ptr(), out.data_ptr()
         chunk_state = err = None
         if keep:
-            chunk_state = torch.empty(B, H, -(-T // a.chunk), K, V, dtype=torch.float32, device=v.device)
             err = torch.empty(B, T, H, V, dtype=torch.float32, device=v.device)
-            a.chunk_state, a.err = chunk_state.data_ptr(), err.data_ptr()
+            if T > a.chunk:
+                chunk_state = torch.empty(B, H, (T - 1) // a.chunk, K, V, dtype=torch.float32, device=v.device)
+            a.chunk_state, a.err = _ptr(chunk_state), err.data_ptr()
         _call(lib.inet_policy_delta_forward, v.device, "delta_rule", C.byref(a))
-        ctx.save_for_backward(q, k, v, g, beta, reset, chunk_state, err)
-        ctx.scale, ctx.has_state = scale, state is not None
+        ctx.save_for_backward(q, k, v, g, beta, state, reset, chunk_state, err)
+        ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_o, d_out):
-        q, k, v, g, beta, reset, chunk_state, err = ctx.saved_tensors
+        q, k, v, g, beta, state, reset, chunk_state, err = ctx.saved_tensors
         if d_o is None and d_out is None:
             return (None,) * 9
         lib = _lib.load_policy()
@@ -145,17 +146,18 @@ class _DeltaRule(torch.autograd.Function):
         Hk, K = q.shape[-2:]
         a = _delta_args(q, k, v, g, beta, reset, ctx.scale, 2)
         a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
-        a.chunk_state, a.err = chunk_state.data_ptr(), err.data_ptr()
+        a.state, a.chunk_state, a.err = _ptr(state), _ptr(chunk_state), err.data_ptr()
         new = lambda *s, dtype=q.dtype: torch.empty(*s, dtype=dtype, device=q.device)  # noqa: E731
         d_o = None if d_o is None else d_o.contiguous()
         d_out = None if d_out is None else d_out.contiguous()
         dq, dk, dv = new(B, T, Hk, K), new(B, T, Hk, K), new(B, T, H, V)
         dg, db = new(B, T, H, dtype=g.dtype), new(B, T, H, dtype=g.dtype)
-        ds = new(B, H, K, V, dtype=torch.float32) if ctx.has_state and ctx.needs_input_grad[5] else None
-        chunk_grad, err_grad = torch.empty_like(chunk_state), torch.empty_like(err)
+        ds = new(B, H, K, V, dtype=torch.float32) if ctx.needs_input_grad[5] else None
+        chunk_grad, err_grad = (None, None) if chunk_state is None else (torch.empty_like(chunk_state),
+                                                                         torch.empty_like(err))
         heads = new(2, B, T, H, K, dtype=torch.float32) if H != Hk else None
         d = _lib.InetDeltaGrad(_ptr(d_o), _ptr(d_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
-                               db.data_ptr(), _ptr(ds), chunk_grad.data_ptr(), err_grad.data_ptr(), _ptr(heads))
+                               db.data_ptr(), _ptr(ds), _ptr(chunk_grad), _ptr(err_grad), _ptr(heads))
         _call(lib.inet_policy_delta_backward, q.device, "delta_rule backward", C.byref(a), C.byref(d))
         return dq, dk, dv, dg, db, ds, None, None, None
 

@@ -140,6 +140,20 @@ def test_window_emptied_memory_is_empty():
         assert torch.equal(x, y), n
 
 
+@pytest.mark.parametrize("T", [20, 90])
+@pytest.mark.parametrize("used", ["o", "state"])
+def test_window_one_output_used(T, used):
+    ins, reset, d_o, d_s = delta_inputs(2, T, 1, 2, 32, 48, torch.float32, seed=14, end=0.02)
+    (d_s if used == "o" else d_o).zero_()
+    want = delta_both(ins, reset, d_o, d_s)[1]
+    x = [t.to(DEV).requires_grad_(True) for t in ins]
+    o, s = P.delta_rule(*x, reset=reset.to(DEV))
+    got = torch.autograd.grad([o if used == "o" else s], x, [(d_o if used == "o" else d_s).to(DEV)], allow_unused=True)
+    for n, a, b in zip(NAMES[2:], got, want[2:]):
+        terms = sum((ins[i].double() * want[2 + i].double()).sum(-1).norm().item() for i in (0, 1))
+        close(n, torch.zeros_like(b) if a is None else a, b, T + 80, size=terms if n == "dg" else 0.0)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_window_layouts(dt):
     """Views of one projection, step-major storage, a last axis that is not contiguous, rows off the 16-byte grid."""
