@@ -59,6 +59,8 @@ typedef struct InetDelta {
        neither is kept), and the state at the start of each chunk but the first, [B][H][chunks - 1][K][V] (NULL where
        there is one chunk). The backward pass takes `state` too. */
     float *chunk_state, *err;
+    void *work;                                 /* inet_policy_delta_work() bytes for the direction; err and chunk_state
+                                                   have to be there too where that is more than 0 */
 } InetDelta;
 
 /* The backward pass: gradients of the inputs from those of o and of state_out (NULL: zero). */
@@ -77,6 +79,8 @@ const char *inet_policy_build_info(void);
 
 /* steps a chunk for these sizes (0: unsupported) */
 int32_t inet_policy_delta_chunk(int32_t T, int32_t K, int32_t V, int32_t dtype);
+/* workspace of a window's forward or backward pass in bytes (sizes, type and chunk are read from a; -1: invalid) */
+int64_t inet_policy_delta_work(const InetDelta *a, int32_t backward);
 int32_t inet_policy_delta_forward(const InetDelta *a, void *stream);
 int32_t inet_policy_delta_backward(const InetDelta *a, const InetDeltaGrad *d, void *stream);
 /* one step, the state updated in place: T = 1, state_out is the state (state itself is ignored); strides of step unused */

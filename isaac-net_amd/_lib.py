@@ -129,7 +129,8 @@ class InetDelta(C.Structure):
     _fields_ = [(n, i32) for n in ("B", "T", "Hk", "H", "K", "V", "dtype", "gate_dtype")] + \
                [("scale", f32), ("chunk", i32)] + \
                [(n, i64 * 3) for n in ("q_s", "k_s", "v_s", "g_s", "beta_s")] + [("reset_s", i64 * 2)] + \
-               [(n, P) for n in ("q", "k", "v", "g", "beta", "reset", "state", "o", "state_out", "chunk_state", "err")]
+               [(n, P) for n in ("q", "k", "v", "g", "beta", "reset", "state", "o", "state_out", "chunk_state", "err",
+                            "work")]
 
 
 class InetDeltaGrad(C.Structure):
@@ -250,6 +251,8 @@ def load_policy(path=POLICY_LIB_PATH):
     if lib.inet_policy_abi_version() != POLICY_ABI_VERSION:
         raise RuntimeError("libinet_policy.so ABI version mismatch; rebuild it")
     lib.inet_policy_delta_chunk.argtypes = [i32, i32, i32, i32]
+    lib.inet_policy_delta_work.argtypes = [C.POINTER(InetDelta), i32]
+    lib.inet_policy_delta_work.restype = i64
     lib.inet_policy_ffn_work.argtypes = [i64, i32, i32, i32]
     lib.inet_policy_norm_work.argtypes = [i64, i32]
     lib.inet_policy_ffn_work.restype = lib.inet_policy_norm_work.restype = i64

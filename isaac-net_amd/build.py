@@ -27,7 +27,7 @@ UNITS = [f"nr_step_mc{c}.hip" for c in (7, 6, 5, 4)] + \
 POLICY_CSRC = os.path.join(CSRC, "policy")
 POLICY_LIB = os.path.join(HERE, "libinet_policy.so")
 POLICY_HEADER = "inet_policy.h"
-POLICY_UNITS = ["delta_forward.hip", "delta_backward.hip", "delta_step.hip", "ffn.hip", "norm.hip", "policy.hip"]
+POLICY_UNITS = ["delta_backward.hip", "delta_split.hip", "delta_forward.hip", "delta_step.hip", "ffn.hip", "norm.hip", "policy.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wall", "-Wno-unused-function"]

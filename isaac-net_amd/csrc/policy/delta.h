@@ -170,6 +170,15 @@ template <typename T> DEV f32x4 tile_at(const T* s, int ld, int n, int g) {
     return x;
 }
 
+// 16 x 16 values from planes (columns in their own order) as a result's tile
+template <int N> DEV f32x4 plane_tile(const Planes<N>& s, int row0, int c0, int n, int g) {
+    f32x4 x = {};
+#pragma unroll
+    for (int m = N - 1; m >= 0; --m)
+        x += tile_at<__bf16>(s.p + m * s.plane + row0 * s.ld + c0, s.ld, n, g);
+    return x;
+}
+
 // such a result to LDS, rounded to T
 template <typename T> DEV void tile_put(T* s, int ld, int n, int g, f32x4 x) {
 #pragma unroll
@@ -295,6 +304,32 @@ template <int C> DEV void invert_blocks(float* ln, int ld) {
     if (in)
 #pragma unroll
         for (int i = 0; i < 16; ++i) B[i * ld + n] = x[i];
+}
+
+// x <- (I + L)^-1 x for 16 columns, or (I + L)^-T x (from the last block row up); ln as invert_blocks leaves it
+template <int C> DEV void solve_down(f32x4 (&x)[C / 16], const float* ln, int ld, int n, int g) {
+#pragma unroll
+    for (int rt = 0; rt < C / 16; ++rt) {
+        f32x4 acc = x[rt];
+#pragma unroll
+        for (int m = 0; m < rt; ++m) acc = mma32(*(const f32x4*)(ln + (rt * 16 + n) * ld + m * 16 + 4 * g), x[m], acc);
+        x[rt] = mma32(*(const f32x4*)(ln + (rt * 16 + n) * ld + rt * 16 + 4 * g), acc, f32x4{});
+    }
+}
+template <int C> DEV void solve_up(f32x4 (&z)[C / 16], const float* ln, int ld, int n, int g) {
+#pragma unroll
+    for (int rt = C / 16 - 1; rt >= 0; --rt) {
+        f32x4 acc = z[rt], a;
+#pragma unroll
+        for (int m = rt + 1; m < C / 16; ++m) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = ln[(m * 16 + 4 * g + e) * ld + rt * 16 + n];
+            acc = mma32(a, z[m], acc);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = ln[(rt * 16 + 4 * g + e) * ld + rt * 16 + n];
+        z[rt] = mma32(a, acc, f32x4{});
+    }
 }
 
 // both triangles of a chunk, from K and Q in LDS, and the diagonal blocks' inverses; ends with a barrier

@@ -8,15 +8,6 @@
 
 namespace pol {
 
-// 16 columns (from c0 on) of a chunk's dO from its rows' planes
-template <int N> DEV f32x4 plane_tile(const Planes<N>& s, int row0, int c0, int n, int g) {
-    f32x4 x = {};
-#pragma unroll
-    for (int m = N - 1; m >= 0; --m)
-        x += tile_at<__bf16>(s.p + m * s.plane + row0 * s.ld + c0, s.ld, n, g);
-    return x;
-}
-
 // rows of values [steps][V] into planes in their own order, zeros up to vp columns
 template <typename T, int C, bool VEC, int N>
 DEV void stage_rows(const T* __restrict__ x, int64_t row0, int64_t row_s, int steps, int V, int vp, const Planes<N>& s) {
@@ -58,20 +49,7 @@ DEV void column_gradients(const f32x4 (&S)[KP / 16], bool has_s, f32x4 (&z)[C / 
 #pragma unroll
         for (int rt = 0; rt < 2 * kp + 2; ++rt) z[rt] = mma<2>(P.tr_frag(rt, kp, n, g), uf, z[rt]);
     }
-    // Z, block row by block row from the end
-#pragma unroll
-    for (int rt = RT - 1; rt >= 0; --rt) {
-        f32x4 acc = z[rt], a;
-#pragma unroll
-        for (int m = rt + 1; m < RT; ++m) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = ln[(m * 16 + 4 * g + e) * ld + rt * 16 + n];
-            acc = mma32(a, z[m], acc);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = ln[(rt * 16 + 4 * g + e) * ld + rt * 16 + n];
-        z[rt] = mma32(a, acc, f32x4{});
-    }
+    solve_up<C>(z, ln, ld, n, g);                   // Z
 }
 
 // S, the gradient of the state after a chunk, to that of the state before it: a_C S + Q^T (scale a dO) - K^T (a beta Z)
@@ -112,7 +90,6 @@ template <typename T, int C, int KP> struct ScanLds {
     alignas(16) __bf16 k[NP * C * LK], q[NP * C * LK], p[3 * C * LC];
     alignas(16) float ln[C * LL];
     alignas(16) __bf16 u[NP * C * LV];
-    alignas(16) T v[C * LV];
 };
 
 // The state's gradient. One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns.
@@ -173,13 +150,9 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
                 if (ch + 1 < chunks)
                     state_store(S, gr.chunk_grad + (bh * (chunks - 1) + ch) * d.K * d.V + c0, at, d.V, d.K, g);
             }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                tile_put(s.v + rt * 16 * LV + w * 16, LV, n, g, z[rt] * *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g));
             if (ch || gr.d_state) state_gradient<C, KP, NP>(S, z, u, s.gates, d.scale, Kr, Qr, n, g);
         }
         __syncthreads();
-        store_rows<T, C, VEC>(s.v, (T*)gr.d_v + rows0 + t0 * row_s, row_s, d.T - t0, width);
     }
     if (mine && gr.d_state) state_store(S, gr.d_state + bh * d.K * d.V + c0, at, d.V, d.K, g);
 }
@@ -196,20 +169,28 @@ template <typename T, int C, int KP> constexpr size_t chunk_lds(int vp) {
     return sizeof(Gates<C>) + sizeof(Sums<C>) + sizeof(__bf16) * (2 * NP * C * (KP + 8) + (2 * NO + NP) * C * (vp + 8));
 }
 
-// X = beta E and dbeta's E . Z by rows, Z from memory (err_grad) where z_in, else as it is in LDS already
+// X = beta E and dbeta's E . Z by rows; Z from memory (err_grad), and dV = beta Z to there, where z_in, else as it is in
+// LDS already
 template <typename T, int C, bool VEC, int NO>
-DEV void stage_errors(const InetDelta& d, const float* z_in, int64_t row0, int64_t row_s, int steps, int vp,
+DEV void stage_errors(const InetDelta& d, const float* z_in, T* dv, int64_t row0, int64_t row_s, int steps, int vp,
                       const Gates<C>& gates, const Planes<NO>& X, const Planes<NO>& Z, Sums<C>& sums) {
     const int lanes = vp <= 32 ? 4 : vp <= 64 ? 8 : 16;             // a row
     for (int i = threadIdx.x; i < C * lanes; i += DELTA_WG) {
         const int r = i / lanes, c = i % lanes * 8;
         float e[8] = {}, z[8] = {}, x = 0.0f;
         if (r < steps && c < d.V) load8(d.err + row0 + r * row_s + c, d.V - c, VEC, e);
+        const float beta = gates.beta[r];
         if (c < vp) {
             if (z_in) {
                 if (r < steps && c < d.V) load8(z_in + row0 + r * row_s + c, d.V - c, VEC, z);
                 Z.put4(r, c, z[0], z[1], z[2], z[3]);
                 Z.put4(r, c + 4, z[4], z[5], z[6], z[7]);
+                if (r < steps && c < d.V) {
+                    const float lo[4] = {beta * z[0], beta * z[1], beta * z[2], beta * z[3]},
+                                hi[4] = {beta * z[4], beta * z[5], beta * z[6], beta * z[7]};
+                    store4(dv + row0 + r * row_s + c, d.V - c, VEC, lo);
+                    store4(dv + row0 + r * row_s + c + 4, d.V - c - 4, VEC, hi);
+                }
             } else {
                 const Frag<NO> f = Z.frag(r, c);
 #pragma unroll
@@ -217,7 +198,6 @@ DEV void stage_errors(const InetDelta& d, const float* z_in, int64_t row0, int64
 #pragma unroll
                     for (int u = 0; u < 8; ++u) z[u] += (float)f.p[m][u];
             }
-            const float beta = gates.beta[r];
             X.put4(r, c, beta * e[0], beta * e[1], beta * e[2], beta * e[3]);
             X.put4(r, c + 4, beta * e[4], beta * e[5], beta * e[6], beta * e[7]);
         }
@@ -443,7 +423,7 @@ void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
     }
     stage_rows<T, C, VEC, NP>((const T*)gr.d_o, row0, row_s, steps, d.V, vp, O);
     __syncthreads();
-    stage_errors<T, C, VEC, NO>(d, gr.err_grad, row0, row_s, steps, vp, gates, X, Z, sums);
+    stage_errors<T, C, VEC, NO>(d, gr.err_grad, (T*)gr.d_v, row0, row_s, steps, vp, gates, X, Z, sums);
     __syncthreads();
     const int64_t kv = (int64_t)d.K * d.V, at = bh * (chunks - 1) + ch;
     const float* S = ch ? d.chunk_state + (at - 1) * kv : d.state ? d.state + bh * kv : nullptr;
@@ -510,15 +490,7 @@ void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
             for (int rt = 0; rt < RT; ++rt) {
                 tile_put(out + rt * 16 * LV + w * 16, LV, n, g, z[rt] * *(const f32x4*)(gates.beta + rt * 16 + 4 * g));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = z[rt][e];
-#pragma unroll
-                    for (int m = 0; m < NO; ++m) {
-                        const __bf16 y = (__bf16)x;
-                        Z.p[m * Z.plane + (rt * 16 + 4 * g + e) * lv + c0 + w * 16 + n] = y;
-                        x -= (float)y;
-                    }
-                }
+                for (int e = 0; e < 4; ++e) Z.put1(rt * 16 + 4 * g + e, c0 + w * 16 + n, z[rt][e]);
             }
             if (gr.d_state) {
                 state_gradient<C, KP, NP>(S, z, u, gates, d.scale, Kr, Qr, n, g);
@@ -529,7 +501,7 @@ void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
         store_rows<T, C, VEC>(out, (T*)gr.d_v + row0 + c0, row_s, d.T, width);
         __syncthreads();
     }
-    stage_errors<T, C, VEC, NO>(d, nullptr, row0, row_s, d.T, vp, gates, X, Z, sums);
+    stage_errors<T, C, VEC, NO>(d, nullptr, (T*)nullptr, row0, row_s, d.T, vp, gates, X, Z, sums);
     __syncthreads();
     chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, 0, d.state ? d.state + bh * kv : nullptr,
                                            gr.d_state_out ? gr.d_state_out + bh * kv : nullptr, gates, sums, Kr, Qr, X,
@@ -568,8 +540,12 @@ static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
         auto scan = delta_scan_kernel<T, C, KP, VEC>;
         auto chunk = delta_chunk_kernel<T, C, KP, VEC>;
         if (allow_lds((const void*)scan, lds) || allow_lds((const void*)chunk, cl)) return INET_POLICY_ELAUNCH;
-        hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
-        if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
+        if (d.work) {
+            if (int rc = delta_split(d, &g, VEC, st)) return rc;
+        } else {
+            hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
+            if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
+        }
         if (!chunks) return INET_POLICY_OK;
         hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), cl, st, d, g);
         if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;

@@ -70,21 +70,17 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_f
                     o[rt] = mma<ORD>(Qr.frag(rt * 16 + n, kp * 32 + 8 * g), sf, o[rt]);
                 }
             }
-            // the errors, block row by block row; then X = beta E
+            // the errors; then X = beta E
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const f32x4 a = *(const f32x4*)(s.gates.a + rt * 16 + 4 * g);
-                f32x4 acc = tile_at(s.v + rt * 16 * LV + w * 16, LV, n, g);
+                const f32x4 a = *(const f32x4*)(s.gates.a + rt * 16 + 4 * g), vt = tile_at(s.v + rt * 16 * LV + w * 16, LV, n, g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    acc[e] -= a[e] != 0.0f ? a[e] * x[rt][e] : 0.0f;
+                    x[rt][e] = vt[e] - (a[e] != 0.0f ? a[e] * x[rt][e] : 0.0f);
                     o[rt][e] = a[e] != 0.0f ? d.scale * a[e] * o[rt][e] : 0.0f;
                 }
-#pragma unroll
-                for (int m = 0; m < rt; ++m)
-                    acc = mma32(*(const f32x4*)(s.ln + (rt * 16 + n) * Lds::LL + m * 16 + 4 * g), x[m], acc);
-                x[rt] = mma32(*(const f32x4*)(s.ln + (rt * 16 + n) * Lds::LL + rt * 16 + 4 * g), acc, f32x4{});
             }
+            solve_down<C>(x, s.ln, Lds::LL, n, g);
             if (d.err && mine) {
                 float* err = d.err + rows0 + t0 * row_s;
 #pragma unroll
@@ -134,6 +130,7 @@ template <typename T, int C, int KP, bool VEC> static int launch(const InetDelta
 }
 
 int delta_forward(const InetDelta& d, bool vec, hipStream_t st) {
+    if (d.work) return delta_split(d, nullptr, vec, st);
     return delta_dispatch(d, [&](auto t, auto c, auto kp) {
         typedef typename decltype(t)::type T;
         constexpr int C = decltype(c)::value, KP = decltype(kp)::value;

@@ -45,5 +45,8 @@ template <typename F> int delta_dispatch(const InetDelta& d, F&& f) {
 int delta_forward(const InetDelta& d, bool vec, hipStream_t st);
 int delta_backward(const InetDelta& d, const InetDeltaGrad& g, bool vec, hipStream_t st);
 int delta_step(const InetDelta& d, hipStream_t st);
+// the long-window forms (delta_split.hip), taken where d.work is given
+int delta_split(const InetDelta& d, const InetDeltaGrad* g, bool vec, hipStream_t st);
+size_t delta_split_bytes(const InetDelta& d, bool back);
 
 }  // namespace pol

@@ -130,6 +130,12 @@ static int check_window(const InetDelta* a) {
     return INET_POLICY_OK;
 }
 
+// whether a window goes by delta_split.hip: several chunks, and too few robots and heads for the chip's compute units
+static bool split(const InetDelta* a) {
+    const int64_t groups = (int64_t)a->B * a->H * ((a->V + 63) / 64), chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;
+    return chunks >= 4 && groups < 256;
+}
+
 // whether the inputs' rows start on 16 bytes and hold whole groups of eight
 static bool aligned(const InetDelta* a) {
     const int e = elem_size(a->dtype);
@@ -150,12 +156,19 @@ int32_t inet_policy_delta_chunk(int32_t T, int32_t K, int32_t V, int32_t dtype) 
     return T <= 32 ? 32 : 64;
 }
 
+int64_t inet_policy_delta_work(const InetDelta* a, int32_t backward) {
+    if (pol::check_window(a)) return -1;
+    return a->B && pol::split(a) ? (int64_t)pol::delta_split_bytes(*a, backward != 0) : 0;
+}
+
 int32_t inet_policy_delta_forward(const InetDelta* a, void* stream) {
     if (int rc = pol::check_window(a)) return rc;
     if (a->B == 0) return INET_POLICY_OK;
     if (!a->state_out || a->state == a->state_out) return INET_POLICY_EINVAL;
     if (a->T > 0 && (!a->q || !a->k || !a->v || !a->g || !a->beta || !a->o)) return INET_POLICY_EINVAL;
     if (a->T > a->chunk && !a->err != !a->chunk_state) return INET_POLICY_EINVAL;
+    if (pol::split(a) != (a->work != nullptr) || (a->work && (!a->err || (uintptr_t)a->work % 16)))
+        return INET_POLICY_EINVAL;
     return pol::delta_forward(*a, pol::aligned(a) && (uintptr_t)a->o % 16 == 0, (hipStream_t)stream);
 }
 
@@ -167,6 +180,7 @@ int32_t inet_policy_delta_backward(const InetDelta* a, const InetDeltaGrad* d, v
                      !d->d_beta))
         return INET_POLICY_EINVAL;
     if (a->T > a->chunk && (!a->chunk_state || !d->chunk_grad || !d->err_grad)) return INET_POLICY_EINVAL;
+    if (pol::split(a) != (a->work != nullptr) || (uintptr_t)a->work % 16) return INET_POLICY_EINVAL;
     if (a->H != a->Hk && a->T > 0 && !d->head_grad) return INET_POLICY_EINVAL;
     bool vec = pol::aligned(a);
     for (const void* p : {(const void*)a->err, (const void*)a->chunk_state, (const void*)d->err_grad, d->d_o,

@@ -141,6 +141,26 @@ template <int N> struct Planes {
         }
         return f;
     }
+    // rows 16 rt .. and columns 16 ct .. (columns in the order perm()) as a result's tile: lane column n, rows 4 g + e
+    DEV f32x4 tr_tile(int ct, int rt, int n, int g) const {
+        f32x4 x = {};
+        const __bf16* at = p + (16 * rt + 4 * g + (n >> 2)) * ld + 32 * (ct >> 1) + (n & 3) * 8 + (ct & 1) * 4;
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) {
+            const bf16x4 v = read_tr(at + i * plane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] += (float)v[e];
+        }
+        return x;
+    }
+    DEV void put1(int row, int place, float x) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const __bf16 h = (__bf16)x;
+            p[i * plane + row * ld + place] = h;
+            x -= (float)h;
+        }
+    }
     DEV void put4(int row, int place, float a, float b, float c, float d) const {
         float x[4] = {a, b, c, d};
 #pragma unroll

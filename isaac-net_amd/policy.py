@@ -109,6 +109,13 @@ def _delta_args(q, k, v, g, beta, reset, scale, lead):
     return a
 
 
+def _delta_work(lib, a, dev, backward):
+    n = lib.inet_policy_delta_work(C.byref(a), backward)
+    work = torch.empty(n, dtype=torch.uint8, device=dev) if n > 0 else None
+    a.work = _ptr(work)
+    return work
+
+
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, reset, scale, keep):
@@ -124,13 +131,15 @@ class _DeltaRule(torch.autograd.Function):
         out = torch.empty(B, H, K, V, dtype=torch.float32, device=v.device)
         a.state, a.o, a.state_out = _ptr(state), o.data_ptr(), out.data_ptr()
         chunk_state = err = None
-        if keep:
+        work = _delta_work(lib, a, v.device, 0)
+        if keep or work is not None:
             err = torch.empty(B, T, H, V, dtype=torch.float32, device=v.device)
             if T > a.chunk:
                 chunk_state = torch.empty(B, H, (T - 1) // a.chunk, K, V, dtype=torch.float32, device=v.device)
             a.chunk_state, a.err = _ptr(chunk_state), err.data_ptr()
         _call(lib.inet_policy_delta_forward, v.device, "delta_rule", C.byref(a))
-        ctx.save_for_backward(q, k, v, g, beta, state, reset, chunk_state, err)
+        if keep:
+            ctx.save_for_backward(q, k, v, g, beta, state, reset, chunk_state, err)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, out
@@ -147,6 +156,7 @@ class _DeltaRule(torch.autograd.Function):
         a = _delta_args(q, k, v, g, beta, reset, ctx.scale, 2)
         a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
         a.state, a.chunk_state, a.err = _ptr(state), _ptr(chunk_state), err.data_ptr()
+        work = _delta_work(lib, a, q.device, 1)  # noqa: F841  (held until the call is enqueued)
         new = lambda *s, dtype=q.dtype: torch.empty(*s, dtype=dtype, device=q.device)  # noqa: E731
         d_o = None if d_o is None else d_o.contiguous()
         d_out = None if d_out is None else d_out.contiguous()

@@ -27,7 +27,7 @@ def lib():
 
 def test_library_exports_every_declared_symbol(lib):
     names = re.findall(r"^\s*(?:int32_t|int64_t|const char \*)\s*(inet_policy_\w+)\s*\(", open(HEADER).read(), re.M)
-    assert len(names) == 12
+    assert len(names) == 13
     for n in names:
         assert hasattr(lib, n), n
     assert lib.inet_policy_abi_version() == _lib.POLICY_ABI_VERSION
