@@ -1,13 +1,15 @@
 // The gated feed-forward (include/inet_policy.h): y = act(x Wg^T) * (x Wu^T), forward and backward, on the 16-bit matrix
 // instructions with sums in 32 bits.
 //
-// Forward: a workgroup computes a 128 x 128 tile of both projections from one pass over its rows of x, and the
-// activation and the product in registers; neither projection goes to memory. Backward: the same tile again from x (the
-// two projections would cost a write and a read of 2 N F values, more than the products at the widths measured), then
-// da = dy u act'(a) and du = dy act(a), rounded to the type, as they are and transposed; then
-//     dx = [da du] [Wg; Wu]        a product over 2 F,        dWg = da^T x,  dWu = du^T x     products over N
-// all with both operands' rows along the sum (W and x transposed once). The products over N are split where the tiles of
-// dW are fewer than the chip's compute units; the parts are added in order, so results do not vary from run to run.
+// Forward: a workgroup computes a tile of both projections from one pass over its rows of x, and the activation and the
+// product in registers; neither projection goes to memory. Backward: the same tile again from x, then da = dy u act'(a)
+// and du = dy act(a), rounded to the type; then
+//     dx = [da du] [Wg; Wu]        a product over 2 F,        dWg = da^T x,  dWu = du^T x     products over N.
+// All are one product (Product): tiles of 64 along the sum go to LDS, the next one on its way from memory while the present
+// one is computed with, and a matrix whose rows lie across the sum (W for dx, x and da for dW) is transposed by the LDS
+// reads.
+// The products over N are split where the tiles of dW are fewer than the chip's compute units; the parts are added in
+// order, so results do not vary from run to run.
 #include <type_traits>
 
 #include "policy_dev.h"
@@ -15,7 +17,7 @@
 
 namespace pol {
 
-constexpr int FFN_WG = 256, BM = 128, BN = 128, BK = 64, LDK = BK + 8;
+constexpr int BK = 64;                       // along the sum, a step
 
 template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 
@@ -24,66 +26,202 @@ template <typename T> DEV f32x4 mfma16(typename Vec8<T>::type a, typename Vec8<T
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// rows r0 .. r0 + 127 of p (row stride st, rows valid rows), columns k0 .. k0 + 63 of `cols` (a multiple of 8), one
-// 16-byte load a thread and pass; outside: 0
-template <typename T> struct Tile {
-    typename Vec8<T>::type v[4];
-    DEV void load(const T* __restrict__ p, int64_t st, int64_t r0, int64_t rows, int64_t k0, int64_t cols) {
+// 16 bytes of zeros, where a tile reaches past its matrix
+__device__ __attribute__((aligned(16))) const uint32_t zero16[4] = {0, 0, 0, 0};
+
+// 64 lanes' 16 bytes each from memory to LDS, lane after lane from `to` on (the same in all lanes)
+DEV void load_lds(const void* from, void* to) {
+    typedef __attribute__((address_space(1))) const uint32_t* Mem;
+    typedef __attribute__((address_space(3))) uint32_t* Lds;
+    __builtin_amdgcn_global_load_lds((Mem)from, (Lds)to, 16, 0, 0);
+}
+
+// A matrix of a product: element (i, k) for index i of the result and k of the sum.
+// ALONG: rows along the sum, p[i * st + k], i < rows. TWO: a second matrix p2 of the same shape, where the tile's second
+// half of indexes comes from.
+// else across: p[k * st + i], i < rows (rows a multiple of eight).
+template <typename T, bool ALONG> struct Operand {
+    const T *p, *p2;
+    int64_t st, st2, rows;
+};
+
+// A tile of R indexes x 64 of the sum on its way to LDS. The lanes' places in memory are 32-bit offsets from a place that
+// moves along the sum; indexes past the matrix read its last (their results are not stored), what is past the sum is zero.
+// DIRECT (ALONG alone): memory to LDS without registers, row i's group c of eight at place c ^ (i % 8) of the row's eight,
+// so that a read's lanes fall on distinct banks. Else through registers, to rows with a gap: ALONG 64 + 8 by index, across
+// R + 16 by the sum, and a read's places are one address and constants.
+template <typename T, bool ALONG, int R, int THREADS, bool TWO, bool DIRECT> struct Tile {
+    static constexpr int LOADS = R * 8 / THREADS, LD = DIRECT ? 64 : ALONG ? 72 : R + 16,
+                         SIZE = (ALONG ? R : BK) * LD;
+    typedef typename Vec8<T>::type V8;
+    const char *base, *base2;
+    uint32_t off[LOADS];
+    int64_t step;
+    V8 v[DIRECT ? 1 : LOADS];
+    // load j of this thread: its row of the tile and its group of eight in the row
+    static DEV int row_at(int j) { return (j * THREADS + (int)threadIdx.x) / (ALONG ? 8 : R / 8); }
+    static DEV int group_at(int j) {
+        const int at = (j * THREADS + (int)threadIdx.x) % (ALONG ? 8 : R / 8);
+        return DIRECT ? at ^ (row_at(j) & 7) : at;
+    }
+    static constexpr bool second(int j) { return TWO && j >= LOADS / 2; }     // (half the loads are half the rows)
+    DEV void start(const Operand<T, ALONG>& m, int64_t r0, int64_t k0) {
+        base = (const char*)(ALONG ? m.p + r0 * m.st + k0 : m.p + k0 * m.st + r0);
+        base2 = TWO ? (const char*)(m.p2 + r0 * m.st2 + k0) : nullptr;
+        step = BK * (ALONG ? 1 : m.st) * (int64_t)sizeof(T);
+        const int64_t last = m.rows - 1 - r0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = threadIdx.x + i * FFN_WG;
-            const int64_t r = r0 + at / 8, k = k0 + at % 8 * 8;
-            if (r < rows && k < cols) v[i] = *(const typename Vec8<T>::type*)(p + r * st + k);
-            else v[i] = typename Vec8<T>::type{};
+        for (int j = 0; j < LOADS; ++j) {
+            const int r = row_at(j), c = group_at(j) * 8;
+            if constexpr (ALONG) {
+                int64_t i = second(j) ? r - R / 2 : r;
+                i = i < last ? i : last;
+                off[j] = (uint32_t)((i * (second(j) ? m.st2 : m.st) + c) * (int64_t)sizeof(T));
+            } else {
+                off[j] = (uint32_t)((r * m.st + (c < last - 7 ? c : last - 7)) * (int64_t)sizeof(T));
+            }
         }
     }
-    DEV void put(T* s) const {
+    DEV void next() {
+        base += step;
+        if (TWO) base2 += step;
+    }
+    // the tile of the next 64, `left` of them inside the sum: straight to LDS
+    DEV void fetch(int64_t left, T* lds) {
+        const int w = threadIdx.x >> 6;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = threadIdx.x + i * FFN_WG;
-            *(typename Vec8<T>::type*)(s + at / 8 * LDK + at % 8 * 8) = v[i];
+        for (int j = 0; j < LOADS; ++j) {
+            const char* from = (second(j) ? base2 : base) + off[j];
+            if (left < BK && group_at(j) * 8 >= left) from = (const char*)zero16;
+            load_lds(from, lds + (j * (THREADS / 64) + w) * 512);
+        }
+        next();
+    }
+    // or into registers, and put() when the buffer is free
+    DEV void load(int64_t left) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            v[j] = V8{};
+            if ((ALONG ? group_at(j) * 8 : row_at(j)) < left) v[j] = *(const V8*)((second(j) ? base2 : base) + off[j]);
+        }
+        next();
+    }
+    DEV void put(T* lds) const {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) *(V8*)(lds + row_at(j) * LD + group_at(j) * 8) = v[j];
+    }
+    // indexes i0 + n, 8 g .. 8 g + 7 of the 32 from kk on
+    static DEV V8 frag(const T* lds, int i0, int kk, int n, int g) {
+        if constexpr (DIRECT) {
+            const int r = i0 + n, c = (kk >> 3) + g;
+            return *(const V8*)(lds + r * 64 + ((c ^ (r & 7)) << 3));
+        } else if constexpr (ALONG) {
+            return *(const V8*)(lds + (i0 + n) * LD + kk + 8 * g);
+        } else {
+            const __bf16* p = (const __bf16*)lds + (kk + 8 * g + (n >> 2)) * LD + i0 + (n & 3) * 4;
+            return __builtin_bit_cast(V8, __builtin_shufflevector(read_tr(p), read_tr(p + 4 * LD), 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
 };
 
-// acc[m] (64 x 64 a wave) of A [rows][k] against NB matrices B_m [cols][k], both along k
-template <typename T, int NB>
-DEV void product(const T* __restrict__ A, int64_t as, int64_t r0, int64_t rows, const T* const (&B)[NB],
-                 const int64_t (&bs)[NB], int64_t c0, int64_t cols, int64_t k_from, int64_t k_to, T* lds,
-                 f32x4 (&acc)[NB][4][4]) {
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wr = (w >> 1) * 64, wc = (w & 1) * 64;
-    Tile<T> ta, tb[NB];
-    ta.load(A, as, r0, rows, k_from, k_to);
-#pragma unroll
-    for (int m = 0; m < NB; ++m) tb[m].load(B[m], bs[m], c0, cols, k_from, k_to);
-    for (int64_t k = k_from; k < k_to; k += BK) {
-        __syncthreads();
-        ta.put(lds);
-#pragma unroll
-        for (int m = 0; m < NB; ++m) tb[m].put(lds + (1 + m) * BM * LDK);
-        __syncthreads();
-        if (k + BK < k_to) {
-            ta.load(A, as, r0, rows, k + BK, k_to);
-#pragma unroll
-            for (int m = 0; m < NB; ++m) tb[m].load(B[m], bs[m], c0, cols, k + BK, k_to);
+// acc[c][r] += tiles of the product of `rows` (BM indexes) and `cols` (BN), over k_from .. k_to - 1; WR x WC waves. A lane
+// holds four columns (16 c + 4 g + e of the wave's) of one row (16 r + n). The columns come in two halves where HALVES:
+// the wave's first CT / 2 tiles from the first half of the tile's columns, the others from the second.
+template <typename T, int BM_, int BN_, int WR_, int WC_, bool ROWS_ALONG, bool COLS_ALONG, bool HALVES> struct Product {
+    static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, THREADS = 64 * WR * WC, RT = BM / WR / 16,
+                         CT = BN / WC / 16;
+    // straight to LDS where no read of LDS transposes: the compiler has those wait for all of memory
+    static constexpr bool DIRECT = ROWS_ALONG && COLS_ALONG;
+    typedef Tile<T, ROWS_ALONG, BM, THREADS, false, DIRECT> TR;
+    typedef Tile<T, COLS_ALONG, BN, THREADS, HALVES, DIRECT> TC;
+    static constexpr int BUF = TR::SIZE + TC::SIZE, LDS = 2 * BUF * (int)sizeof(T);
+    // the first column of the wave's tile c
+    static DEV int col(int wc, int c) {
+        return HALVES ? (c < CT / 2 ? 0 : BN / 2) + wc * (BN / 2 / WC) + (c % (CT / 2)) * 16 : wc * (BN / WC) + c * 16;
+    }
+    // (rows2 and cols2: a second pair, added where rows2.p is there)
+    static DEV void run(const Operand<T, ROWS_ALONG>& rows1, const Operand<T, COLS_ALONG>& cols1,
+                        const Operand<T, ROWS_ALONG>& rows2, const Operand<T, COLS_ALONG>& cols2, int64_t r0, int64_t c0,
+                        int64_t k_from, int64_t k_to, T* lds, f32x4 (&acc)[CT][RT]) {
+        const int pairs = rows2.p ? 2 : 1;
+#pragma nounroll
+        for (int m = 0; m < pairs; ++m) one(m ? rows2 : rows1, m ? cols2 : cols1, r0, c0, k_from, k_to, lds, acc);
+    }
+    static DEV void one(const Operand<T, ROWS_ALONG>& rows, const Operand<T, COLS_ALONG>& cols, int64_t r0, int64_t c0,
+                        int64_t k_from, int64_t k_to, T* lds, f32x4 (&acc)[CT][RT]) {
+        const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = w / WC, wc = w % WC;
+        if (k_from >= k_to) return;
+        TR tr;
+        TC tc;
+        tr.start(rows, r0, k_from);
+        tc.start(cols, c0, k_from);
+        __syncthreads();                     // (a product before this one has been computed with its buffers)
+        if constexpr (DIRECT) {
+            tr.fetch(k_to - k_from, lds);
+            tc.fetch(k_to - k_from, lds + TR::SIZE);
+        } else {
+            tr.load(k_to - k_from);
+            tc.load(k_to - k_from);
         }
-#pragma unroll
-        for (int kk = 0; kk < BK; kk += 32) {
-            typename Vec8<T>::type a[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                a[i] = *(const typename Vec8<T>::type*)(lds + (wr + i * 16 + n) * LDK + kk + 8 * g);
-#pragma unroll
-            for (int m = 0; m < NB; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const auto b = *(const typename Vec8<T>::type*)(lds + (1 + m) * BM * LDK +
-                                                                   (wc + j * 16 + n) * LDK + kk + 8 * g);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][i][j] = mfma16<T>(a[i], b, acc[m][i][j]);
+        int cur = 0;
+        for (int64_t k = k_from; k < k_to; k += BK, cur ^= 1) {
+            if constexpr (DIRECT) {
+                // this step's tiles have arrived, and nobody reads the other buffer any more
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (k + BK < k_to) {
+                    tr.fetch(k_to - k - BK, lds + (cur ^ 1) * BUF);
+                    tc.fetch(k_to - k - BK, lds + (cur ^ 1) * BUF + TR::SIZE);
                 }
+            } else {
+                tr.put(lds + cur * BUF);
+                tc.put(lds + cur * BUF + TR::SIZE);
+                __syncthreads();
+                if (k + BK < k_to) {
+                    tr.load(k_to - k - BK);
+                    tc.load(k_to - k - BK);
+                }
+            }
+            const T *lr = lds + cur * BUF, *lc = lr + TR::SIZE;      // (offsets, not two pointers: the reads stay LDS reads)
+#pragma unroll
+            for (int kk = 0; kk < BK; kk += 32) {
+                typename Vec8<T>::type b[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) b[r] = TR::frag(lr, wr * (BM / WR) + r * 16, kk, n, g);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const auto x = TC::frag(lc, col(wc, c), kk, n, g);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) acc[c][r] = mfma16<T>(x, b[r], acc[c][r]);
+                }
+            }
         }
+    }
+};
+
+// The tiles (and shares of the sum) in an order in which the workgroups that run together on one of the eight dies, each
+// with an L2 of its own, share what they read: die d takes a stretch of the sequence of all shares, of each share's row
+// tiles, and of each row tile's column tiles.
+DEV void tile_order(int64_t row_tiles, int col_tiles, int64_t& r, int& c, int& share) {
+    const int64_t total = gridDim.x, at = blockIdx.x, die = at % 8, per = total / 8, rest = total % 8;
+    const int64_t mine = die * per + (die < rest ? die : rest) + at / 8, tile = mine / col_tiles;
+    c = (int)(mine % col_tiles);
+    r = tile % row_tiles;
+    share = (int)(tile / row_tiles);
+}
+
+// four values of a row from column col on, of `cols`
+template <typename O> DEV void put_row4(O* p, int64_t col, int64_t cols, bool vec, f32x4 x) {
+    if (vec && col + 4 <= cols) {
+        typedef O V4 __attribute__((ext_vector_type(4)));
+        V4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (O)x[e];
+        *(V4*)(p + col) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < cols) p[col + e] = (O)x[e];
     }
 }
 
@@ -106,98 +244,83 @@ DEV void activation(int act, float a, float& h, float& dh) {
 }
 
 struct FfnShape {
-    int64_t N, x_s, wg_s, wu_s, y_s;
-    int D, D8, F, F8, act;
-    int64_t N8;
+    int64_t N, y_s;
+    int D8, F, F8, act;
+    bool vec_y;                              // y (or dy) by four values at a time
 };
 
-template <typename T, bool BACK>
-__global__ __launch_bounds__(FFN_WG) void ffn_gates_kernel(FfnShape p, const T* __restrict__ x,
-                                                           const T* __restrict__ wg, const T* __restrict__ wu,
-                                                           T* __restrict__ y, const T* __restrict__ dy, int64_t dy_s,
-                                                           T* __restrict__ da, T* __restrict__ dat) {
-    __shared__ alignas(16) T lds[3 * BM * LDK];
-    const int64_t r0 = (int64_t)blockIdx.y * BM;
-    const int c0 = blockIdx.x * BN;
-    f32x4 acc[2][4][4] = {};
-    const T* const B[2] = {wg, wu};
-    const int64_t bs[2] = {p.wg_s, p.wu_s};
-    product<T, 2>(x, p.x_s, r0, p.N, B, bs, c0, p.F, 0, p.D8, lds, acc);
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wr = (w >> 1) * 64, wc = (w & 1) * 64;
+// y, or (BACK) da and du side by side in da [N][2 F8]
+template <typename T, typename P, bool BACK>
+__global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
+void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __restrict__ y, const T* __restrict__ dy,
+                      int64_t dy_s, T* __restrict__ da) {
+    extern __shared__ char lds_raw[];
+    constexpr int COLS = P::BN / 2;
+    int64_t rt;
+    int ct, all;
+    tile_order((p.N + P::BM - 1) / P::BM, (p.F + COLS - 1) / COLS, rt, ct, all);
+    const int64_t r0 = rt * P::BM, c0 = (int64_t)ct * COLS;
+    f32x4 acc[P::CT][P::RT] = {};
+    P::one(x, w, r0, c0, 0, p.D8, (T*)lds_raw, acc);
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = wv / P::WC, wc = wv % P::WC;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int r = 0; r < P::RT; ++r) {
+        const int64_t row = r0 + wr * (P::BM / P::WR) + r * 16 + n;
+        if (row >= p.N) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = c0 + wc + j * 16 + n;
-            float a_out[4], u_out[4];
+        for (int c = 0; c < P::CT / 2; ++c) {
+            const int64_t col = c0 + P::col(wc, c) + 4 * g;
+            const f32x4 a = acc[c][r], u = acc[c + P::CT / 2][r];
+            f32x4 h, dh;
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int64_t row = r0 + wr + i * 16 + 4 * g + e;
-                const bool in = row < p.N && col < p.F;
-                float h, dh;
-                activation(p.act, acc[0][i][j][e], h, dh);
-                if (!BACK) {
-                    if (in) y[row * p.y_s + col] = (T)(h * acc[1][i][j][e]);
-                } else {
-                    const float d = in ? (float)dy[row * dy_s + col] : 0.0f;
-                    a_out[e] = d * acc[1][i][j][e] * dh;
-                    u_out[e] = d * h;
-                    if (row < p.N && col < p.F8) {
-                        da[row * 2 * p.F8 + col] = (T)a_out[e];
-                        da[row * 2 * p.F8 + p.F8 + col] = (T)u_out[e];
-                    }
-                }
+                float x, y2;
+                activation(p.act, a[e], x, y2);
+                h[e] = x;
+                dh[e] = y2;
             }
-            if (BACK && col < p.F) {
-                const int64_t row = r0 + wr + i * 16 + 4 * g;
-                for (int e = 0; e < 4; ++e)
-                    if (row + e < p.N8) {
-                        dat[(int64_t)col * p.N8 + row + e] = (T)a_out[e];
-                        dat[(int64_t)(p.F + col) * p.N8 + row + e] = (T)u_out[e];
-                    }
+            if constexpr (!BACK) {
+                put_row4(y + row * p.y_s, col, p.F, p.vec_y, h * u);
+            } else if (col < p.F8) {
+                float d[4] = {};
+                if (col < p.F) load4(dy + row * dy_s + col, (int)(p.F - col), p.vec_y, d);
+                f32x4 x1, x2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x1[e] = col + e < p.F ? d[e] * u[e] * dh[e] : 0.0f;
+                    x2[e] = col + e < p.F ? d[e] * h[e] : 0.0f;
+                }
+                put_row4(da + row * 2 * p.F8, col, p.F8, true, x1);
+                put_row4(da + row * 2 * p.F8 + p.F8, col, p.F8, true, x2);
             }
         }
-}
-
-// C [rows][cols] = A [rows][k] B [cols][k]^T; blockIdx.z: a share of k, each to its own C in 32 bits
-template <typename T, typename O>
-__global__ __launch_bounds__(FFN_WG) void ffn_product_kernel(const T* __restrict__ A, int64_t as, int64_t rows,
-                                                             const T* __restrict__ B, int64_t b_s, int64_t cols,
-                                                             int64_t K, int64_t share, O* __restrict__ C, int64_t cs) {
-    __shared__ alignas(16) T lds[2 * BM * LDK];
-    const int64_t r0 = (int64_t)blockIdx.y * BM, c0 = (int64_t)blockIdx.x * BN;
-    f32x4 acc[1][4][4] = {};
-    const T* const Bm[1] = {B};
-    const int64_t bs[1] = {b_s}, from = blockIdx.z * share, to = from + share < K ? from + share : K;
-    product<T, 1>(A, as, r0, rows, Bm, bs, c0, cols, from, to, lds, acc);
-    C += blockIdx.z * rows * cs;
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wr = (w >> 1) * 64, wc = (w & 1) * 64;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            for (int e = 0; e < 4; ++e) {
-                const int64_t row = r0 + wr + i * 16 + 4 * g + e, col = c0 + wc + j * 16 + n;
-                if (row < rows && col < cols) C[row * cs + col] = (O)acc[0][i][j][e];
-            }
-}
-
-// out [cols][rows8] = in [rows][cols] transposed, zeros in rows .. rows8 - 1; 64 x 64 tiles
-template <typename T>
-__global__ __launch_bounds__(256) void ffn_transpose_kernel(const T* __restrict__ in, int64_t in_s, int64_t rows,
-                                                            int64_t cols, T* __restrict__ out, int64_t out_s,
-                                                            int64_t rows8) {
-    __shared__ T s[64][66];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int64_t r = r0 + i / 64, c = c0 + i % 64;
-        s[i / 64][i % 64] = r < rows && c < cols ? in[r * in_s + c] : (T)0.0f;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int64_t c = c0 + i / 64, r = r0 + i % 64;
-        if (c < cols && r < rows8) out[c * out_s + r] = s[i % 64][i / 64];
+}
+
+// C [rows][cols] = a b (+ a2 b2 where there are such), or shares of the sum each to a C of its own
+template <typename T, typename P, bool RA, bool CA, typename O>
+__global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
+void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, Operand<T, CA> b2, int64_t K,
+                        int64_t share, O* __restrict__ C, int64_t rows, int64_t cols, bool vec) {
+    extern __shared__ char lds_raw[];
+    int64_t rt;
+    int ct, part;
+    tile_order((rows + P::BM - 1) / P::BM, (int)((cols + P::BN - 1) / P::BN), rt, ct, part);
+    const int64_t r0 = rt * P::BM, c0 = (int64_t)ct * P::BN;
+    const int64_t from = part * share, to = from + share < K ? from + share : K;
+    f32x4 acc[P::CT][P::RT] = {};
+    P::run(a, b, a2, b2, r0, c0, from, to, (T*)lds_raw, acc);
+    C += part * rows * cols;
+    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = wv / P::WC, wc = wv % P::WC;
+#pragma unroll
+    for (int r = 0; r < P::RT; ++r) {
+        const int64_t row = r0 + wr * (P::BM / P::WR) + r * 16 + n;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int c = 0; c < P::CT; ++c) {
+            const int64_t col = c0 + P::col(wc, c) + 4 * g;
+            if (col < cols) put_row4(C + row * cols, col, cols, vec, acc[c][r]);
+        }
     }
 }
 
@@ -212,33 +335,50 @@ __global__ __launch_bounds__(256) void ffn_pad_kernel(const T* __restrict__ in, 
     out[i] = c < D ? in[r * in_s + c] : (T)0.0f;
 }
 
-// the shares of a product over N added up in order: out [n]
+// the shares of a product over N added up in order: out [rows][D] of parts [count][.][cols]
 template <typename T>
-__global__ __launch_bounds__(256) void ffn_add_kernel(const float* __restrict__ parts, int count, int64_t n,
-                                                      T* __restrict__ out, int64_t stride) {
+__global__ __launch_bounds__(256) void ffn_add_kernel(const float* __restrict__ parts, int count, int64_t stride,
+                                                      int64_t rows, int D, int cols, T* __restrict__ out) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+    if (i >= rows * D) return;
+    const float* p = parts + i / D * cols + i % D;
     float x = 0.0f;
-    for (int s = 0; s < count; ++s) x += parts[s * stride + i];
+    for (int s = 0; s < count; ++s) x += p[s * stride];
     out[i] = (T)x;
 }
 
 static int64_t up8(int64_t x) { return (x + 7) & ~(int64_t)7; }
-static int64_t tiles(int64_t x) { return (x + BM - 1) / BM; }
+static int64_t tiles(int64_t x, int t) { return (x + t - 1) / t; }
 static unsigned blocks256(int64_t n) { return (unsigned)((n + 255) / 256); }
 
-// shares of a product over N: enough workgroups for the chip's 256 compute units twice over, no share under 512 rows
-static int shares(int64_t N, int D, int F) {
-    const int64_t t = tiles(F) * tiles(D) * 2, want = (512 + t - 1) / t, most = (N + 511) / 512;
+// The tile of a product by how many of the largest it has: 256 x 256 (eight waves, a compute unit's LDS to itself) where
+// they fill the chip's 256 compute units, else 128 x 128, else 64 x 64.
+static int size_for(int64_t rows, int64_t cols) {
+    return tiles(rows, 256) * tiles(cols, 256) >= 256 ? 2 : tiles(rows, 128) * tiles(cols, 128) >= 256 ? 1 : 0;
+}
+template <typename F> static int by_size(int size, F&& f) {
+    return size == 2 ? f(std::integral_constant<int, 2>{}) : size == 1 ? f(std::integral_constant<int, 1>{})
+                                                                      : f(std::integral_constant<int, 0>{});
+}
+template <typename T, int SIZE, bool RA, bool CA, bool HALVES>
+using Sized = typename std::conditional<SIZE == 2, Product<T, 256, 256, 2, 4, RA, CA, HALVES>,
+              typename std::conditional<SIZE == 1, Product<T, 128, 128, 2, 2, RA, CA, HALVES>,
+                                        Product<T, 64, 64, 2, 2, RA, CA, HALVES>>::type>::type;
+
+// the weights' gradients: the tile, and shares of the sum over N, at least 512 rows each, until the chip is full twice over
+static int dw_size(int64_t D8, int64_t F8) { return tiles(2 * F8, 256) * tiles(D8, 256) >= 16 ? 2 : 1; }
+static int shares(int64_t N, int64_t D8, int64_t F8) {
+    const int size = dw_size(D8, F8), b = size == 2 ? 256 : 128;
+    const int64_t t = tiles(2 * F8, b) * tiles(D8, b), want = ((size == 2 ? 256 : 512) + t - 1) / t, most = tiles(N, 512);
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s);
 }
 
 // the workspace's parts, in bytes from its start
 struct Work {
-    int64_t x, wg, wu, da, dat, xt, wt, parts, bytes;
+    int64_t x, wg, wu, da, parts, bytes;
     Work(int64_t N, int64_t D, int64_t F, bool back) {
-        const int64_t D8 = up8(D), F8 = up8(F), N8 = up8(N);
+        const int64_t D8 = up8(D), F8 = up8(F);
         int64_t at = 0;
         auto take = [&](int64_t n) {
             const int64_t p = at;
@@ -250,10 +390,7 @@ struct Work {
         wg = take(pad ? F * D8 * 2 : 0);
         wu = take(pad ? F * D8 * 2 : 0);
         da = take(back ? N * 2 * F8 * 2 : 0);
-        dat = take(back ? 2 * F * N8 * 2 : 0);
-        xt = take(back ? D * N8 * 2 : 0);
-        wt = take(back ? D * 2 * F8 * 2 : 0);
-        parts = take(back ? (int64_t)shares(N, (int)D, (int)F) * 2 * F * D * 4 : 0);
+        parts = take(back ? (int64_t)shares(N, D8, F8) * 2 * F8 * D8 * 4 : 0);
         bytes = at;
     }
 };
@@ -263,64 +400,82 @@ struct Work {
         if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH; \
     } while (0)
 
+static bool allow_lds(const void* kernel, int bytes) {
+    return bytes <= 64 * 1024 ||
+           hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+}
+
+template <typename T, bool BACK>
+static int gates(const FfnShape& p, const Operand<T, true>& x, const Operand<T, true>& w, T* y, const T* dy, int64_t dy_s,
+                 T* da, hipStream_t st) {
+    return by_size(size_for(p.N, 2 * (int64_t)p.F), [&](auto size) {
+        typedef Sized<T, decltype(size)::value, true, true, true> P;
+        auto k = ffn_gates_kernel<T, P, BACK>;
+        if (!allow_lds((const void*)k, P::LDS)) return INET_POLICY_ELAUNCH;
+        const int64_t grid = tiles(p.N, P::BM) * tiles(p.F, P::BN / 2);
+        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(P::THREADS), P::LDS, st, p, x, w, y, dy, dy_s, da);
+        LAUNCHED;
+        return INET_POLICY_OK;
+    });
+}
+
+template <typename T, bool RA, bool CA, typename O>
+static int product(int size, const Operand<T, RA>& a, const Operand<T, CA>& b, const Operand<T, RA>& a2,
+                   const Operand<T, CA>& b2, int64_t K, int count, int64_t share, O* C,
+                   int64_t rows, int64_t cols, bool vec, hipStream_t st) {
+    return by_size(size, [&](auto sz) {
+        typedef Sized<T, decltype(sz)::value, RA, CA, false> P;
+        auto k = ffn_product_kernel<T, P, RA, CA, O>;
+        if (!allow_lds((const void*)k, P::LDS)) return INET_POLICY_ELAUNCH;
+        const int64_t grid = tiles(rows, P::BM) * tiles(cols, P::BN);
+        hipLaunchKernelGGL(k, dim3((unsigned)(grid * count)), dim3(P::THREADS), P::LDS, st, a, b, a2, b2, K, share, C, rows, cols, vec);
+        LAUNCHED;
+        return INET_POLICY_OK;
+    });
+}
+
 template <typename T> static int run(const InetFfn& a, const InetFfnGrad* d, hipStream_t st) {
     const Work at(a.N, a.D, a.F, d != nullptr);
     char* work = (char*)a.work;
-    FfnShape p{a.N, a.x_s, a.w_gate_s, a.w_up_s, a.y_s, a.D, (int)up8(a.D), a.F, (int)up8(a.F), a.act, up8(a.N)};
-    const T *x = (const T*)a.x, *wg = (const T*)a.w_gate, *wu = (const T*)a.w_up;
-    if (p.D8 != p.D) {
-        struct { const T* in; int64_t s, rows; T* out; } pads[3] = {{x, a.x_s, a.N, (T*)(work + at.x)},
-                                                                    {wg, a.w_gate_s, a.F, (T*)(work + at.wg)},
-                                                                    {wu, a.w_up_s, a.F, (T*)(work + at.wu)}};
+    const int D8 = (int)up8(a.D), F8 = (int)up8(a.F);
+    Operand<T, true> x{(const T*)a.x, nullptr, a.x_s, 0, a.N};
+    Operand<T, true> w{(const T*)a.w_gate, (const T*)a.w_up, a.w_gate_s, a.w_up_s, a.F};
+    if (D8 != a.D) {
+        struct { const T* in; int64_t s, rows; T* out; } pads[3] = {{x.p, a.x_s, a.N, (T*)(work + at.x)},
+                                                                    {w.p, a.w_gate_s, a.F, (T*)(work + at.wg)},
+                                                                    {w.p2, a.w_up_s, a.F, (T*)(work + at.wu)}};
         for (auto& q : pads) {
-            hipLaunchKernelGGL(ffn_pad_kernel<T>, dim3(blocks256(q.rows * p.D8)), dim3(256), 0, st, q.in, q.s, q.rows,
-                               p.D, q.out, p.D8);
+            hipLaunchKernelGGL(ffn_pad_kernel<T>, dim3(blocks256(q.rows * D8)), dim3(256), 0, st, q.in, q.s, q.rows,
+                               a.D, q.out, D8);
             LAUNCHED;
         }
-        x = pads[0].out, wg = pads[1].out, wu = pads[2].out;
-        p.x_s = p.wg_s = p.wu_s = p.D8;
+        x.p = pads[0].out, w.p = pads[1].out, w.p2 = pads[2].out;
+        x.st = w.st = w.st2 = D8;
     }
-    const dim3 grid((unsigned)tiles(a.F), (unsigned)tiles(a.N));
-    if (!d) {
-        hipLaunchKernelGGL((ffn_gates_kernel<T, false>), grid, dim3(FFN_WG), 0, st, p, x, wg, wu, (T*)a.y,
-                           (const T*)nullptr, (int64_t)0, (T*)nullptr, (T*)nullptr);
-        LAUNCHED;
-        return INET_POLICY_OK;
-    }
-    T *da = (T*)(work + at.da), *dat = (T*)(work + at.dat), *xt = (T*)(work + at.xt), *wt = (T*)(work + at.wt);
-    hipLaunchKernelGGL((ffn_gates_kernel<T, true>), grid, dim3(FFN_WG), 0, st, p, x, wg, wu, (T*)nullptr,
-                       (const T*)d->d_y, d->d_y_s, da, dat);
-    LAUNCHED;
+    auto by4 = [](const void* p, int64_t s) { return (uintptr_t)p % 8 == 0 && s % 4 == 0; };
+    FfnShape p{a.N, a.y_s, D8, a.F, F8, a.act, d ? by4(d->d_y, d->d_y_s) : by4(a.y, a.y_s)};
+    if (!d) return gates<T, false>(p, x, w, (T*)a.y, nullptr, 0, nullptr, st);
+    T* da = (T*)(work + at.da);
+    if (int rc = gates<T, true>(p, x, w, nullptr, (const T*)d->d_y, d->d_y_s, da, st)) return rc;
     if (d->d_x) {
-        for (int m = 0; m < 2; ++m) {
-            hipLaunchKernelGGL(ffn_transpose_kernel<T>, dim3((a.F + 63) / 64, (a.D + 63) / 64), dim3(256), 0, st,
-                               m ? wu : wg, m ? p.wu_s : p.wg_s, (int64_t)a.F, (int64_t)a.D, wt + m * p.F8,
-                               (int64_t)2 * p.F8, (int64_t)p.F8);
-            LAUNCHED;
-        }
-        hipLaunchKernelGGL((ffn_product_kernel<T, T>), dim3((unsigned)tiles(a.D), (unsigned)tiles(a.N)), dim3(FFN_WG),
-                           0, st, da, (int64_t)2 * p.F8, a.N, wt, (int64_t)2 * p.F8, (int64_t)a.D, (int64_t)2 * p.F8,
-                           (int64_t)2 * p.F8, (T*)d->d_x, (int64_t)a.D);
-        LAUNCHED;
+        const Operand<T, true> dg{da, nullptr, 2 * F8, 0, a.N}, du{da + F8, nullptr, 2 * F8, 0, a.N};
+        const Operand<T, false> wg{w.p, nullptr, w.st, 0, D8}, wu{w.p2, nullptr, w.st2, 0, D8};
+        if (int rc = product<T, true, false, T>(size_for(a.N, D8), dg, wg, du, wu, a.F, 1, F8, (T*)d->d_x, a.N, a.D,
+                                                by4(d->d_x, a.D), st))
+            return rc;
     }
     if (d->d_w_gate || d->d_w_up) {
-        hipLaunchKernelGGL(ffn_transpose_kernel<T>, dim3((unsigned)((a.N + 63) / 64), (a.D + 63) / 64), dim3(256), 0,
-                           st, x, p.x_s, a.N, (int64_t)a.D, xt, p.N8, p.N8);
-        LAUNCHED;
-        const int s = shares(a.N, a.D, a.F);
-        const int64_t share = ((p.N8 + s - 1) / s + BK - 1) / BK * BK;
+        const Operand<T, false> dat{da, nullptr, 2 * F8, 0, 2 * F8}, xt{x.p, nullptr, x.st, 0, D8}, no{};
+        const int s = shares(a.N, D8, F8);
+        const int64_t share = (tiles(a.N, s) + BK - 1) / BK * BK, one = (int64_t)2 * F8 * D8;
         float* parts = (float*)(work + at.parts);
-        hipLaunchKernelGGL((ffn_product_kernel<T, float>), dim3((unsigned)tiles(a.D), (unsigned)tiles(2 * (int64_t)a.F), s),
-                           dim3(FFN_WG), 0, st, dat, p.N8, (int64_t)2 * a.F, xt, p.N8, (int64_t)a.D, p.N8, share, parts,
-                           (int64_t)a.D);
-        LAUNCHED;
-        // (the shares of both matrices lie one after the other: [share][2 F][D])
-        const int64_t one = (int64_t)a.F * a.D;
+        if (int rc = product<T, false, false, float>(dw_size(D8, F8), dat, xt, no, no, a.N, s, share, parts, 2 * F8, D8, true, st))
+            return rc;
         for (int m = 0; m < 2; ++m) {
             T* out = (T*)(m ? d->d_w_up : d->d_w_gate);
             if (!out) continue;
-            hipLaunchKernelGGL(ffn_add_kernel<T>, dim3(blocks256(one)), dim3(256), 0, st, parts + m * one, s, one, out,
-                               2 * one);
+            hipLaunchKernelGGL(ffn_add_kernel<T>, dim3(blocks256((int64_t)a.F * a.D)), dim3(256), 0, st,
+                               parts + (int64_t)m * F8 * D8, s, one, (int64_t)a.F, a.D, D8, out);
             LAUNCHED;
         }
     }
@@ -331,7 +486,11 @@ static int check(const InetFfn* a) {
     if (!a || a->N < 0 || a->D < 1 || a->F < 1 || a->act < 0 || a->act > 2 || a->dtype < 0 || a->dtype > 2)
         return INET_POLICY_EINVAL;
     if (a->dtype == INET_POLICY_F32 || a->D > 1 << 20 || a->F > 1 << 20) return INET_POLICY_EUNSUPPORTED;
-    if (tiles(a->N) > 65535) return INET_POLICY_EUNSUPPORTED;
+    for (int64_t s : {a->x_s, a->w_gate_s, a->w_up_s})       // (a tile's offsets are 32-bit)
+        if (s < 0 || s > (int64_t)1 << 22) return INET_POLICY_EUNSUPPORTED;
+    if (a->N > (int64_t)1 << 23) return INET_POLICY_EUNSUPPORTED;
+    if (tiles(a->N, 64) * tiles(a->F, 32) > (1 << 24) - 1 || tiles(a->N, 64) * tiles(a->D, 64) > (1 << 24) - 1)
+        return INET_POLICY_EUNSUPPORTED;     // (workgroups a launch)
     if (a->N == 0) return INET_POLICY_OK;
     if (!a->x || !a->w_gate || !a->w_up) return INET_POLICY_EINVAL;
     if (a->D % 8 == 0) {                      // rows are read 16 bytes at a time; other widths are padded first
@@ -348,8 +507,8 @@ template <typename T> static int zero_weights(const InetFfn& a, const InetFfnGra
     const int64_t one = (int64_t)a.F * a.D;
     for (void* out : {d.d_w_gate, d.d_w_up})
         if (out) {
-            hipLaunchKernelGGL(ffn_add_kernel<T>, dim3(blocks256(one)), dim3(256), 0, st, (const float*)nullptr, 0, one,
-                               (T*)out, one);
+            hipLaunchKernelGGL(ffn_add_kernel<T>, dim3(blocks256(one)), dim3(256), 0, st, (const float*)nullptr, 0,
+                               (int64_t)0, (int64_t)a.F, a.D, a.D, (T*)out);
             LAUNCHED;
         }
     return INET_POLICY_OK;

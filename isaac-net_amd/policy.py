@@ -212,9 +212,10 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
 
 # ------------------------------------------------------------------------------------------------ the feed-forward
 def _aligned_rows(x):
-    """x [rows, D] with its rows contiguous, and on 16 bytes where D holds whole groups of eight."""
+    """x [rows, D] with its rows contiguous, not too far apart, and on 16 bytes where D holds whole groups of eight."""
     x = _rows(x)
-    if x.shape[1] % 8 == 0 and (x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8)):
+    far = x.shape[0] > 1 and x.stride(0) > 1 << 22
+    if far or (x.shape[1] % 8 == 0 and (x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8))):
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -283,8 +284,8 @@ def gated_ffn(x, w_gate, w_up, activation="silu"):
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise HipUnsupported(f"gated_ffn of {x.dtype}: bfloat16 and float16 are implemented")
     rows = x.reshape(-1, x.shape[-1])
-    if rows.shape[0] > 65535 * 128:
-        raise HipUnsupported(f"gated_ffn of {rows.shape[0]} rows: up to {65535 * 128}")
+    if rows.shape[0] > 1 << 23:
+        raise HipUnsupported(f"gated_ffn of {rows.shape[0]} rows: up to {1 << 23}")
     y = _GatedFfn.apply(rows, w_gate, w_up, ACTIVATIONS.index(activation))
     return y.view(*x.shape[:-1], w_gate.shape[0])
 
