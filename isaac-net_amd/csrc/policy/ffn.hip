@@ -225,18 +225,19 @@ template <typename O> DEV void put_row4(O* p, int64_t col, int64_t cols, bool ve
     }
 }
 
-// act(a) and its derivative
-DEV void activation(int act, float a, float& h, float& dh) {
-    if (act == INET_POLICY_SILU) {
-        const float s = 1.0f / (1.0f + __expf(-a));
+// 1 / (1 + e^-x) (the reciprocal to one unit in the last place; x of any size: e^-x may be infinite, the result then 0)
+DEV float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+
+// act(a) and its derivative; gelu's 0.5 (1 + tanh u) is logistic(2 u)
+template <int ACT> DEV void activation(float a, float& h, float& dh) {
+    if constexpr (ACT == INET_POLICY_SILU) {
+        const float s = logistic(a);
         h = a * s;
-        dh = s * (1.0f + a * (1.0f - s));
-    } else if (act == INET_POLICY_GELU) {
-        // 0.5 (1 + tanh u) = 1 / (1 + e^{-2 u})
-        const float a2 = a * a, u = 0.7978845608028654f * a * (1.0f + 0.044715f * a2);
-        const float s = 1.0f / (1.0f + __expf(-2.0f * u));
+        dh = s + h * (1.0f - s);
+    } else if constexpr (ACT == INET_POLICY_GELU) {
+        const float a2 = a * a, s = logistic(1.5957691216057308f * a * (1.0f + 0.044715f * a2));
         h = a * s;
-        dh = s + a * s * (1.0f - s) * 2.0f * 0.7978845608028654f * (1.0f + 0.134145f * a2);
+        dh = s + h * (1.0f - s) * (1.5957691216057308f + 0.21406440f * a2);
     } else {
         h = a > 0.0f ? a : 0.0f;
         dh = a > 0.0f ? 1.0f : 0.0f;
@@ -245,12 +246,12 @@ DEV void activation(int act, float a, float& h, float& dh) {
 
 struct FfnShape {
     int64_t N, y_s;
-    int D8, F, F8, act;
+    int D8, F, F8;
     bool vec_y;                              // y (or dy) by four values at a time
 };
 
 // y, or (BACK) da and du side by side in da [N][2 F8]
-template <typename T, typename P, bool BACK>
+template <typename T, typename P, int ACT, bool BACK>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __restrict__ y, const T* __restrict__ dy,
                       int64_t dy_s, T* __restrict__ da) {
@@ -275,7 +276,7 @@ void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __r
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float x, y2;
-                activation(p.act, a[e], x, y2);
+                activation<ACT>(a[e], x, y2);
                 h[e] = x;
                 dh[e] = y2;
             }
@@ -405,18 +406,22 @@ static bool allow_lds(const void* kernel, int bytes) {
            hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
 }
 
-template <typename T, bool BACK>
+template <typename T, int ACT, bool BACK>
 static int gates(const FfnShape& p, const Operand<T, true>& x, const Operand<T, true>& w, T* y, const T* dy, int64_t dy_s,
                  T* da, hipStream_t st) {
     return by_size(size_for(p.N, 2 * (int64_t)p.F), [&](auto size) {
         typedef Sized<T, decltype(size)::value, true, true, true> P;
-        auto k = ffn_gates_kernel<T, P, BACK>;
+        auto k = ffn_gates_kernel<T, P, ACT, BACK>;
         if (!allow_lds((const void*)k, P::LDS)) return INET_POLICY_ELAUNCH;
         const int64_t grid = tiles(p.N, P::BM) * tiles(p.F, P::BN / 2);
         hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(P::THREADS), P::LDS, st, p, x, w, y, dy, dy_s, da);
         LAUNCHED;
         return INET_POLICY_OK;
     });
+}
+template <typename T, bool BACK, typename... A> static int gates_for(int act, const A&... a) {
+    return act == INET_POLICY_SILU ? gates<T, INET_POLICY_SILU, BACK>(a...)
+           : act == INET_POLICY_GELU ? gates<T, INET_POLICY_GELU, BACK>(a...) : gates<T, INET_POLICY_RELU, BACK>(a...);
 }
 
 template <typename T, bool RA, bool CA, typename O>
@@ -453,10 +458,10 @@ template <typename T> static int run(const InetFfn& a, const InetFfnGrad* d, hip
         x.st = w.st = w.st2 = D8;
     }
     auto by4 = [](const void* p, int64_t s) { return (uintptr_t)p % 8 == 0 && s % 4 == 0; };
-    FfnShape p{a.N, a.y_s, D8, a.F, F8, a.act, d ? by4(d->d_y, d->d_y_s) : by4(a.y, a.y_s)};
-    if (!d) return gates<T, false>(p, x, w, (T*)a.y, nullptr, 0, nullptr, st);
+    FfnShape p{a.N, a.y_s, D8, a.F, F8, d ? by4(d->d_y, d->d_y_s) : by4(a.y, a.y_s)};
+    if (!d) return gates_for<T, false>(a.act, p, x, w, (T*)a.y, (const T*)nullptr, 0, (T*)nullptr, st);
     T* da = (T*)(work + at.da);
-    if (int rc = gates<T, true>(p, x, w, nullptr, (const T*)d->d_y, d->d_y_s, da, st)) return rc;
+    if (int rc = gates_for<T, true>(a.act, p, x, w, (T*)nullptr, (const T*)d->d_y, d->d_y_s, da, st)) return rc;
     if (d->d_x) {
         const Operand<T, true> dg{da, nullptr, 2 * F8, 0, a.N}, du{da + F8, nullptr, 2 * F8, 0, a.N};
         const Operand<T, false> wg{w.p, nullptr, w.st, 0, D8}, wu{w.p2, nullptr, w.st2, 0, D8};
