@@ -149,7 +149,6 @@ template <typename T, int BM_, int BN_, int WR_, int WC_, bool ROWS_ALONG, bool 
     }
     static DEV void one(const Operand<T, ROWS_ALONG>& rows, const Operand<T, COLS_ALONG>& cols, int64_t r0, int64_t c0,
                         int64_t k_from, int64_t k_to, T* lds, f32x4 (&acc)[CT][RT]) {
-        const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = w / WC, wc = w % WC;
         if (k_from >= k_to) return;
         TR tr;
         TC tc;
@@ -182,18 +181,23 @@ template <typename T, int BM_, int BN_, int WR_, int WC_, bool ROWS_ALONG, bool 
                     tc.load(k_to - k - BK);
                 }
             }
-            const T *lr = lds + cur * BUF, *lc = lr + TR::SIZE;      // (offsets, not two pointers: the reads stay LDS reads)
+            step(lds + cur * BUF, acc);
+        }
+    }
+    // one tile along the sum
+    static DEV void step(const T* lr, f32x4 (&acc)[CT][RT]) {
+        const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = w / WC, wc = w % WC;
+        const T* lc = lr + TR::SIZE;
 #pragma unroll
-            for (int kk = 0; kk < BK; kk += 32) {
-                typename Vec8<T>::type b[RT];
+        for (int kk = 0; kk < BK; kk += 32) {
+            typename Vec8<T>::type b[RT];
 #pragma unroll
-                for (int r = 0; r < RT; ++r) b[r] = TR::frag(lr, wr * (BM / WR) + r * 16, kk, n, g);
+            for (int r = 0; r < RT; ++r) b[r] = TR::frag(lr, wr * (BM / WR) + r * 16, kk, n, g);
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const auto x = TC::frag(lc, col(wc, c), kk, n, g);
+            for (int c = 0; c < CT; ++c) {
+                const auto x = TC::frag(lc, col(wc, c), kk, n, g);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) acc[c][r] = mfma16<T>(x, b[r], acc[c][r]);
-                }
+                for (int r = 0; r < RT; ++r) acc[c][r] = mfma16<T>(x, b[r], acc[c][r]);
             }
         }
     }
@@ -202,8 +206,8 @@ template <typename T, int BM_, int BN_, int WR_, int WC_, bool ROWS_ALONG, bool 
 // The tiles (and shares of the sum) in an order in which the workgroups that run together on one of the eight dies, each
 // with an L2 of its own, share what they read: die d takes a stretch of the sequence of all shares, of each share's row
 // tiles, and of each row tile's column tiles.
-DEV void tile_order(int64_t row_tiles, int col_tiles, int64_t& r, int& c, int& share) {
-    const int64_t total = gridDim.x, at = blockIdx.x, die = at % 8, per = total / 8, rest = total % 8;
+DEV void tile_order(int64_t at, int64_t total, int64_t row_tiles, int col_tiles, int64_t& r, int& c, int& share) {
+    const int64_t die = at % 8, per = total / 8, rest = total % 8;
     const int64_t mine = die * per + (die < rest ? die : rest) + at / 8, tile = mine / col_tiles;
     c = (int)(mine % col_tiles);
     r = tile % row_tiles;
@@ -211,8 +215,8 @@ DEV void tile_order(int64_t row_tiles, int col_tiles, int64_t& r, int& c, int& s
 }
 
 // four values of a row from column col on, of `cols`
-template <typename O> DEV void put_row4(O* p, int64_t col, int64_t cols, bool vec, f32x4 x) {
-    if (vec && col + 4 <= cols) {
+template <bool WHOLE, typename O> DEV void put_row4(O* p, int col, int cols, bool vec, f32x4 x) {
+    if (WHOLE || (vec && col + 4 <= cols)) {
         typedef O V4 __attribute__((ext_vector_type(4)));
         V4 v;
 #pragma unroll
@@ -250,51 +254,91 @@ struct FfnShape {
     bool vec_y;                              // y (or dy) by four values at a time
 };
 
-// y, or (BACK) da and du side by side in da [N][2 F8]
+// y, or (BACK) da and du side by side in da [N][2 F8]. A workgroup takes tile after tile: the next one's first step is on
+// its way, and dy has come during the last step, while the results are stored.
 template <typename T, typename P, int ACT, bool BACK>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __restrict__ y, const T* __restrict__ dy,
                       int64_t dy_s, T* __restrict__ da) {
     extern __shared__ char lds_raw[];
-    constexpr int COLS = P::BN / 2;
-    int64_t rt;
-    int ct, all;
-    tile_order((p.N + P::BM - 1) / P::BM, (p.F + COLS - 1) / COLS, rt, ct, all);
-    const int64_t r0 = rt * P::BM, c0 = (int64_t)ct * COLS;
-    f32x4 acc[P::CT][P::RT] = {};
-    P::one(x, w, r0, c0, 0, p.D8, (T*)lds_raw, acc);
+    constexpr int COLS = P::BN / 2, RT = P::RT, CT = P::CT;
+    T* const lds = (T*)lds_raw;
+    const int64_t row_tiles = (p.N + P::BM - 1) / P::BM;
+    const int col_tiles = (p.F + COLS - 1) / COLS, steps = (p.D8 + BK - 1) / BK;
+    const int64_t total = row_tiles * col_tiles;
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = wv / P::WC, wc = wv % P::WC;
-#pragma unroll
-    for (int r = 0; r < P::RT; ++r) {
-        const int64_t row = r0 + wr * (P::BM / P::WR) + r * 16 + n;
-        if (row >= p.N) continue;
-#pragma unroll
-        for (int c = 0; c < P::CT / 2; ++c) {
-            const int64_t col = c0 + P::col(wc, c) + 4 * g;
-            const f32x4 a = acc[c][r], u = acc[c + P::CT / 2][r];
-            f32x4 h, dh;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x, y2;
-                activation<ACT>(a[e], x, y2);
-                h[e] = x;
-                dh[e] = y2;
+    typename P::TR tr;
+    typename P::TC tc;
+    int64_t rt;
+    int ct, all, buf = 0;
+    auto begin = [&](int64_t at) {
+        tile_order(at, total, row_tiles, col_tiles, rt, ct, all);
+        tr.start(x, rt * P::BM, 0);
+        tc.start(w, (int64_t)ct * COLS, 0);
+        tr.fetch(p.D8, lds + buf * P::BUF);
+        tc.fetch(p.D8, lds + buf * P::BUF + P::TR::SIZE);
+    };
+    begin(blockIdx.x);
+    for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
+        const int64_t r0 = rt * P::BM, c0 = (int64_t)ct * COLS;
+        const int rows = (int)(p.N - r0 < P::BM ? p.N - r0 : P::BM), cols = (int)(p.F - c0), cols8 = (int)(p.F8 - c0);
+        f32x4 acc[CT][RT] = {};
+        for (int k = 0; k < steps; ++k, buf ^= 1) {
+            // this step's tiles have arrived, and nobody reads the other buffer any more
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (k + 1 < steps) {
+                tr.fetch(p.D8 - (k + 1) * BK, lds + (buf ^ 1) * P::BUF);
+                tc.fetch(p.D8 - (k + 1) * BK, lds + (buf ^ 1) * P::BUF + P::TR::SIZE);
             }
-            if constexpr (!BACK) {
-                put_row4(y + row * p.y_s, col, p.F, p.vec_y, h * u);
-            } else if (col < p.F8) {
-                float d[4] = {};
-                if (col < p.F) load4(dy + row * dy_s + col, (int)(p.F - col), p.vec_y, d);
-                f32x4 x1, x2;
+            P::step(lds + buf * P::BUF, acc);
+        }
+        if (at + gridDim.x < total) begin(at + gridDim.x);
+    // WHOLE: the tile inside the matrices, four values at a time; offsets from the tile's corner
+    auto finish = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        T* const out = BACK ? da + r0 * 2 * p.F8 + c0 : y + r0 * p.y_s + c0;
+        const T* const in = BACK ? dy + r0 * dy_s + c0 : nullptr;
+#pragma unroll
+        for (int r = 0; r < P::RT; ++r) {
+            const int row = wr * (P::BM / P::WR) + r * 16 + n;
+            if (!WHOLE && row >= rows) continue;
+            f32x4 d[P::CT / 2];
+            if constexpr (BACK)
+#pragma unroll
+                for (int c = 0; c < P::CT / 2; ++c) {
+                    const int col = P::col(wc, c) + 4 * g;
+                    float v[4] = {};
+                    if (WHOLE || col < cols) load4(in + (int64_t)row * dy_s + col, cols - col, WHOLE || p.vec_y, v);
+                    d[c] = f32x4{v[0], v[1], v[2], v[3]};
+                }
+#pragma unroll
+            for (int c = 0; c < P::CT / 2; ++c) {
+                const int col = P::col(wc, c) + 4 * g;
+                const f32x4 a = acc[c][r], u = acc[c + P::CT / 2][r];
+                f32x4 h, dh;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    x1[e] = col + e < p.F ? d[e] * u[e] * dh[e] : 0.0f;
-                    x2[e] = col + e < p.F ? d[e] * h[e] : 0.0f;
+                    float x, y2;
+                    activation<ACT>(a[e], x, y2);
+                    h[e] = x;
+                    dh[e] = y2;
                 }
-                put_row4(da + row * 2 * p.F8, col, p.F8, true, x1);
-                put_row4(da + row * 2 * p.F8 + p.F8, col, p.F8, true, x2);
+                if constexpr (!BACK) {
+                    put_row4<WHOLE>(out + row * p.y_s, col, cols, p.vec_y, h * u);
+                } else if (WHOLE || col < cols8) {
+                    f32x4 x1 = d[c] * u * dh, x2 = d[c] * h;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!WHOLE && col + e >= cols) x1[e] = x2[e] = 0.0f;
+                    put_row4<WHOLE>(out + (int64_t)row * 2 * p.F8, col, cols8, true, x1);
+                    put_row4<WHOLE>(out + (int64_t)row * 2 * p.F8 + p.F8, col, cols8, true, x2);
+                }
             }
         }
+    };
+    if (rows == P::BM && COLS <= cols && p.vec_y) finish(std::true_type{});
+    else finish(std::false_type{});
     }
 }
 
@@ -306,23 +350,30 @@ void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, O
     extern __shared__ char lds_raw[];
     int64_t rt;
     int ct, part;
-    tile_order((rows + P::BM - 1) / P::BM, (int)((cols + P::BN - 1) / P::BN), rt, ct, part);
+    tile_order(blockIdx.x, gridDim.x, (rows + P::BM - 1) / P::BM, (int)((cols + P::BN - 1) / P::BN), rt, ct, part);
     const int64_t r0 = rt * P::BM, c0 = (int64_t)ct * P::BN;
     const int64_t from = part * share, to = from + share < K ? from + share : K;
     f32x4 acc[P::CT][P::RT] = {};
     P::run(a, b, a2, b2, r0, c0, from, to, (T*)lds_raw, acc);
     C += part * rows * cols;
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = wv / P::WC, wc = wv % P::WC;
+    auto finish = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        O* const out = C + r0 * cols + c0;
+        const int left = (int)(cols - c0 < P::BN ? cols - c0 : P::BN);
 #pragma unroll
-    for (int r = 0; r < P::RT; ++r) {
-        const int64_t row = r0 + wr * (P::BM / P::WR) + r * 16 + n;
-        if (row >= rows) continue;
+        for (int r = 0; r < P::RT; ++r) {
+            const int row = wr * (P::BM / P::WR) + r * 16 + n;
+            if (!WHOLE && r0 + row >= rows) continue;
 #pragma unroll
-        for (int c = 0; c < P::CT; ++c) {
-            const int64_t col = c0 + P::col(wc, c) + 4 * g;
-            if (col < cols) put_row4(C + row * cols, col, cols, vec, acc[c][r]);
+            for (int c = 0; c < P::CT; ++c) {
+                const int col = P::col(wc, c) + 4 * g;
+                if (WHOLE || col < left) put_row4<WHOLE>(out + row * cols, col, left, vec, acc[c][r]);
+            }
         }
-    }
+    };
+    if (r0 + P::BM <= rows && c0 + P::BN <= cols && vec) finish(std::true_type{});
+    else finish(std::false_type{});
 }
 
 // rows padded to a multiple of eight with zeros
@@ -413,7 +464,7 @@ static int gates(const FfnShape& p, const Operand<T, true>& x, const Operand<T, 
         typedef Sized<T, decltype(size)::value, true, true, true> P;
         auto k = ffn_gates_kernel<T, P, ACT, BACK>;
         if (!allow_lds((const void*)k, P::LDS)) return INET_POLICY_ELAUNCH;
-        const int64_t grid = tiles(p.N, P::BM) * tiles(p.F, P::BN / 2);
+        const int64_t all = tiles(p.N, P::BM) * tiles(p.F, P::BN / 2), grid = P::THREADS == 512 && all > 256 ? 256 : all;
         hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(P::THREADS), P::LDS, st, p, x, w, y, dy, dy_s, da);
         LAUNCHED;
         return INET_POLICY_OK;
