@@ -22,28 +22,28 @@ from .engine import HipUnsupported
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = ("silu", "gelu", "relu")          # "gelu" is the tanh form
 MAX_HEAD, MAX_WIDTH = 128, 8192
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _need(ok, msg):
-    if not ok:
-        raise ValueError(msg)
-
-
-def _code(name, x, of=None):
-    if x.dtype not in _CODES:
-        raise HipUnsupported(f"{name}: {x.dtype}; float32, bfloat16 and float16 are implemented")
-    return _CODES[x.dtype]
+def _unsupported_type(name, x):
+    return HipUnsupported(f"{name}: {x.dtype}; float32, bfloat16 and float16 are implemented")
 
 
 def _on_gpu(**xs):
-    dev = None
+    """The index of the device that all tensors are on."""
+    dev = -1
     for n, x in xs.items():
         if x is None:
             continue
-        _need(isinstance(x, torch.Tensor), f"{n} has to be a tensor")
-        _need(x.is_cuda, f"{n} is on {x.device}: the policy operators run on the GPU")
-        _need(dev is None or x.device == dev, f"{n} is on {x.device}, the others on {dev}")
-        dev = x.device
+        if not isinstance(x, torch.Tensor):
+            raise ValueError(f"{n} has to be a tensor")
+        d = x.get_device()
+        if d < 0:
+            raise ValueError(f"{n} is on {x.device}: the policy operators run on the GPU")
+        if dev < 0:
+            dev = d
+        elif d != dev:
+            raise ValueError(f"{n} is on {x.device}, the others on cuda:{dev}")
     return dev
 
 
@@ -57,56 +57,68 @@ def _ptr(x):
 
 
 def _call(fn, dev, what, *args):
-    with torch.cuda.device(dev):
-        _lib.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+    """fn on the device's current stream."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
 # ------------------------------------------------------------------------------------------------ the memory
 def _delta_check(q, k, v, g, beta, state, reset, lead):
     dev = _on_gpu(q=q, k=k, v=v, g=g, beta=beta, state=state, reset=reset)
-    axes = {1: "[B, heads, size]", 2: "[B, T, heads, size]"}[lead]
-    _need(q.dim() == lead + 2 and q.shape == k.shape, f"q and k have to be {axes} of one shape: got {tuple(q.shape)} "
-                                                      f"and {tuple(k.shape)}")
-    _need(v.dim() == lead + 2 and v.shape[:lead] == q.shape[:lead],
-          f"v has to be {axes} over q's batch and steps: got {tuple(v.shape)} with q {tuple(q.shape)}")
-    Hk, K, H, V = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
-    _need(Hk > 0 and H > 0 and H % Hk == 0, f"{H} value heads do not share {Hk} query and key heads evenly")
-    _need(K > 0 and V > 0, "heads of size 0")
-    for n, x in (("g", g), ("beta", beta)):
-        _need(tuple(x.shape) == (*v.shape[:lead], H), f"{n} has to be {(*v.shape[:lead], H)}: got {tuple(x.shape)}")
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, f"q, k and v have to be of one type: got {q.dtype}, {k.dtype}, "
-                                                     f"{v.dtype}")
-    _need(g.dtype == beta.dtype, f"g and beta have to be of one type: got {g.dtype}, {beta.dtype}")
-    _code("q", q), _code("g", g)
+    qs, vs = q.shape, v.shape
+    if len(qs) != lead + 2 or qs != k.shape:
+        axes = {1: "[B, heads, size]", 2: "[B, T, heads, size]"}[lead]
+        raise ValueError(f"q and k have to be {axes} of one shape: got {tuple(qs)} and {tuple(k.shape)}")
+    if len(vs) != lead + 2 or vs[:lead] != qs[:lead]:
+        raise ValueError(f"v has to be laid out as q, over its batch and steps: got {tuple(vs)} with q {tuple(qs)}")
+    Hk, K, H, V = qs[-2], qs[-1], vs[-2], vs[-1]
+    if not (Hk > 0 and H > 0 and H % Hk == 0):
+        raise ValueError(f"{H} value heads do not share {Hk} query and key heads evenly")
+    if not (K > 0 and V > 0):
+        raise ValueError("heads of size 0")
+    if g.shape != vs[:-1] or beta.shape != vs[:-1]:
+        raise ValueError(f"g and beta have to be {tuple(vs[:-1])}: got {tuple(g.shape)} and {tuple(beta.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v have to be of one type: got {q.dtype}, {k.dtype}, {v.dtype}")
+    if g.dtype != beta.dtype:
+        raise ValueError(f"g and beta have to be of one type: got {g.dtype}, {beta.dtype}")
+    for n, x in (("q", q), ("g", g)):
+        if x.dtype not in _CODES:
+            raise _unsupported_type(n, x)
     if K > MAX_HEAD or V > MAX_HEAD:
         raise HipUnsupported(f"heads of {K} x {V}: key and value sizes up to {MAX_HEAD} are implemented")
-    if q.shape[0] * H * (-(-q.shape[1] // 32) if lead == 2 else 1) >= 1 << 24:
-        raise HipUnsupported(f"{q.shape[0]} robots x {H} heads x {q.shape[1] if lead == 2 else 1} steps: fewer than {1 << 24} robots x heads "
-                             "x chunks of 32 steps are implemented")
+    if qs[0] * H * (-(-qs[1] // 32) if lead == 2 else 1) >= 1 << 24:
+        raise HipUnsupported(f"{qs[0]} robots x {H} heads x {qs[1] if lead == 2 else 1} steps: fewer than {1 << 24} "
+                             "robots x heads x chunks of 32 steps are implemented")
     if state is not None:
-        _need(state.dtype == torch.float32, f"state is held in float32: got {state.dtype}")
-        _need(tuple(state.shape) == (q.shape[0], H, K, V), f"state has to be {(q.shape[0], H, K, V)}: got "
-                                                          f"{tuple(state.shape)}")
+        if state.dtype != torch.float32:
+            raise ValueError(f"state is held in float32: got {state.dtype}")
+        if state.shape != (qs[0], H, K, V):
+            raise ValueError(f"state has to be {(qs[0], H, K, V)}: got {tuple(state.shape)}")
     if reset is not None:
-        _need(reset.dtype in (torch.bool, torch.uint8), f"reset has to be bool or uint8: got {reset.dtype}")
-        _need(tuple(reset.shape) == tuple(q.shape[:lead]), f"reset has to be {tuple(q.shape[:lead])}: got "
-                                                           f"{tuple(reset.shape)}")
+        if reset.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"reset has to be bool or uint8: got {reset.dtype}")
+        if reset.shape != qs[:lead]:
+            raise ValueError(f"reset has to be {tuple(qs[:lead])}: got {tuple(reset.shape)}")
     return dev
 
 
-def _delta_args(q, k, v, g, beta, reset, scale, lead):
-    a = _lib.InetDelta()
-    a.B, a.T = q.shape[0], (q.shape[1] if lead == 2 else 1)
-    a.Hk, a.K, a.H, a.V = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
-    a.dtype, a.gate_dtype, a.scale = _CODES[q.dtype], _CODES[g.dtype], scale
-    for n, x in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta)):
-        s = x.stride()
-        setattr(a, n + "_s", (_lib.i64 * 3)(s[0], s[1] if lead == 2 else 0, s[lead]))
-        setattr(a, n, x.data_ptr())
-    if reset is not None:
-        a.reset_s = (_lib.i64 * 2)(reset.stride(0), reset.stride(1) if lead == 2 else 0)
-        a.reset = reset.data_ptr()
-    return a
+def _delta_args(q, k, v, g, beta, reset, scale, lead, chunk=0):
+    qs, vs = q.shape, v.shape
+    if lead == 2:
+        st = [x.stride()[:3] for x in (q, k, v, g, beta)]
+        rs = (0, 0) if reset is None else reset.stride()
+    else:
+        st = [(x.stride(0), 0, x.stride(1)) for x in (q, k, v, g, beta)]
+        rs = (0 if reset is None else reset.stride(0), 0)
+    return _lib.InetDelta(qs[0], qs[1] if lead == 2 else 1, qs[-2], vs[-2], qs[-1], vs[-1], _CODES[q.dtype],
+                          _CODES[g.dtype], scale, chunk, *st, rs, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+                          beta.data_ptr(), None if reset is None else reset.data_ptr())
 
 
 def _delta_work(lib, a, dev, backward):
@@ -116,30 +128,35 @@ def _delta_work(lib, a, dev, backward):
     return work
 
 
+def _delta_forward(q, k, v, g, beta, state, reset, scale, keep):
+    """(o, state, the inputs as read, what the backward pass takes)."""
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if state is not None:
+        state = state.contiguous()
+    lib = _lib.load_policy()
+    B, T, H, V = v.shape
+    K, dev = q.shape[-1], v.device
+    a = _delta_args(q, k, v, g, beta, reset, scale, 2)
+    a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
+    o = torch.empty((B, T, H, V), dtype=v.dtype, device=dev)
+    out = torch.empty((B, H, K, V), dtype=torch.float32, device=dev)
+    a.state, a.o, a.state_out = _ptr(state), o.data_ptr(), out.data_ptr()
+    chunk_state = err = None
+    work = _delta_work(lib, a, dev, 0)
+    if keep or work is not None:
+        err = torch.empty((B, T, H, V), dtype=torch.float32, device=dev)
+        if T > a.chunk:
+            chunk_state = torch.empty((B, H, (T - 1) // a.chunk, K, V), dtype=torch.float32, device=dev)
+        a.chunk_state, a.err = _ptr(chunk_state), err.data_ptr()
+    _call(lib.inet_policy_delta_forward, dev.index, "delta_rule", C.byref(a))
+    return o, out, (q, k, v, g, beta, state, reset, chunk_state, err)
+
+
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, reset, scale, keep):
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        if state is not None:
-            state = state.contiguous()
-        lib = _lib.load_policy()
-        B, T, H, V = v.shape
-        K = q.shape[-1]
-        a = _delta_args(q, k, v, g, beta, reset, scale, 2)
-        a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
-        o = torch.empty(B, T, H, V, dtype=v.dtype, device=v.device)
-        out = torch.empty(B, H, K, V, dtype=torch.float32, device=v.device)
-        a.state, a.o, a.state_out = _ptr(state), o.data_ptr(), out.data_ptr()
-        chunk_state = err = None
-        work = _delta_work(lib, a, v.device, 0)
-        if keep or work is not None:
-            err = torch.empty(B, T, H, V, dtype=torch.float32, device=v.device)
-            if T > a.chunk:
-                chunk_state = torch.empty(B, H, (T - 1) // a.chunk, K, V, dtype=torch.float32, device=v.device)
-            a.chunk_state, a.err = _ptr(chunk_state), err.data_ptr()
-        _call(lib.inet_policy_delta_forward, v.device, "delta_rule", C.byref(a))
-        if keep:
-            ctx.save_for_backward(q, k, v, g, beta, state, reset, chunk_state, err)
+    def forward(ctx, q, k, v, g, beta, state, reset, scale):
+        o, out, saved = _delta_forward(q, k, v, g, beta, state, reset, scale, True)
+        ctx.save_for_backward(*saved)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, out
@@ -149,27 +166,28 @@ class _DeltaRule(torch.autograd.Function):
     def backward(ctx, d_o, d_out):
         q, k, v, g, beta, state, reset, chunk_state, err = ctx.saved_tensors
         if d_o is None and d_out is None:
-            return (None,) * 9
+            return (None,) * 8
         lib = _lib.load_policy()
         B, T, H, V = v.shape
         Hk, K = q.shape[-2:]
+        dev = q.device
         a = _delta_args(q, k, v, g, beta, reset, ctx.scale, 2)
         a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
         a.state, a.chunk_state, a.err = _ptr(state), _ptr(chunk_state), err.data_ptr()
-        work = _delta_work(lib, a, q.device, 1)  # noqa: F841  (held until the call is enqueued)
-        new = lambda *s, dtype=q.dtype: torch.empty(*s, dtype=dtype, device=q.device)  # noqa: E731
+        work = _delta_work(lib, a, dev, 1)  # noqa: F841  (held until the call is enqueued)
         d_o = None if d_o is None else d_o.contiguous()
         d_out = None if d_out is None else d_out.contiguous()
-        dq, dk, dv = new(B, T, Hk, K), new(B, T, Hk, K), new(B, T, H, V)
-        dg, db = new(B, T, H, dtype=g.dtype), new(B, T, H, dtype=g.dtype)
-        ds = new(B, H, K, V, dtype=torch.float32) if ctx.needs_input_grad[5] else None
+        dq, dk = (torch.empty((B, T, Hk, K), dtype=q.dtype, device=dev) for _ in range(2))
+        dv = torch.empty((B, T, H, V), dtype=q.dtype, device=dev)
+        dg, db = (torch.empty((B, T, H), dtype=g.dtype, device=dev) for _ in range(2))
+        ds = torch.empty((B, H, K, V), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
         chunk_grad, err_grad = (None, None) if chunk_state is None else (torch.empty_like(chunk_state),
                                                                          torch.empty_like(err))
-        heads = new(2, B, T, H, K, dtype=torch.float32) if H != Hk else None
+        heads = torch.empty((2, B, T, H, K), dtype=torch.float32, device=dev) if H != Hk else None
         d = _lib.InetDeltaGrad(_ptr(d_o), _ptr(d_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
                                db.data_ptr(), _ptr(ds), _ptr(chunk_grad), _ptr(err_grad), _ptr(heads))
-        _call(lib.inet_policy_delta_backward, q.device, "delta_rule backward", C.byref(a), C.byref(d))
-        return dq, dk, dv, dg, db, ds, None, None, None
+        _call(lib.inet_policy_delta_backward, dev.index, "delta_rule backward", C.byref(a), C.byref(d))
+        return dq, dk, dv, dg, db, ds, None, None
 
 
 def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
@@ -187,23 +205,24 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
     Returns (o [B, T, H, V] of v's type, the memory after the window [B, H, K, V] float32)."""
     _delta_check(q, k, v, g, beta, state, reset, 2)
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    keep = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
-    return _DeltaRule.apply(q, k, v, g, beta, state, reset, scale, keep)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
+                                    beta.requires_grad or (state is not None and state.requires_grad)):
+        return _DeltaRule.apply(q, k, v, g, beta, state, reset, scale)
+    return _delta_forward(q, k, v, g, beta, state, reset, scale, False)[:2]
 
 
-@torch.no_grad()
 def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
     """One control step of the gated delta rule, the memory updated in place: q, k [B, Hk, K], v [B, H, V], g and beta
     [B, H], state [B, H, K, V] float32 contiguous, reset [B] (an emptied memory is empty whatever it held). Returns o
     [B, H, V] (in `out` if given, contiguous of v's type). No derivatives: windows are trained through delta_rule."""
     dev = _delta_check(q, k, v, g, beta, state, reset, 1)
-    _need(state is not None and state.is_contiguous(), "state has to be a contiguous tensor: it is updated in place")
+    if state is None or not state.is_contiguous():
+        raise ValueError("state has to be a contiguous tensor: it is updated in place")
     q, k, v = _rows(q), _rows(k), _rows(v)
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=dev)
-    else:
-        _need(out.shape == v.shape and out.dtype == v.dtype and out.device == dev and out.is_contiguous(),
-              f"out has to be a contiguous {tuple(v.shape)} tensor of {v.dtype} on {dev}")
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    elif out.shape != v.shape or out.dtype != v.dtype or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"out has to be a contiguous {tuple(v.shape)} tensor of {v.dtype} on {v.device}")
     a = _delta_args(q, k, v, g, beta, reset, float(q.shape[-1] ** -0.5 if scale is None else scale), 1)
     a.o, a.state_out = out.data_ptr(), state.data_ptr()
     _call(_lib.load_policy().inet_policy_delta_step, dev, "delta_rule_step", C.byref(a))
@@ -224,13 +243,10 @@ def _row_stride(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _ffn_args(x, w_gate, w_up, act):
-    a = _lib.InetFfn()
-    (a.N, a.D), a.F = x.shape, w_gate.shape[0]
-    a.dtype, a.act = _CODES[x.dtype], act
-    a.x_s, a.w_gate_s, a.w_up_s, a.y_s = _row_stride(x), _row_stride(w_gate), _row_stride(w_up), a.F
-    a.x, a.w_gate, a.w_up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
-    return a
+def _ffn_args(x, w_gate, w_up, act, y=None):
+    (N, D), F = x.shape, w_gate.shape[0]
+    return _lib.InetFfn(N, D, F, _CODES[x.dtype], act, _row_stride(x), _row_stride(w_gate), _row_stride(w_up), F,
+                        x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _ptr(y))
 
 
 def _ffn_work(lib, a, dev, backward):
@@ -240,17 +256,21 @@ def _ffn_work(lib, a, dev, backward):
     return work
 
 
+def _ffn_forward(x, w_gate, w_up, act):
+    x, w_gate, w_up = _aligned_rows(x), _aligned_rows(w_gate), _aligned_rows(w_up)
+    lib, dev = _lib.load_policy(), x.device
+    y = torch.empty((x.shape[0], w_gate.shape[0]), dtype=x.dtype, device=dev)
+    a = _ffn_args(x, w_gate, w_up, act, y)
+    work = _ffn_work(lib, a, dev, 0) if a.D % 8 else None  # noqa: F841  (held until the call is enqueued)
+    _call(lib.inet_policy_ffn_forward, dev.index, "gated_ffn", C.byref(a))
+    return y, (x, w_gate, w_up)
+
+
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act):
-        x, w_gate, w_up = _aligned_rows(x), _aligned_rows(w_gate), _aligned_rows(w_up)
-        lib = _lib.load_policy()
-        y = torch.empty(x.shape[0], w_gate.shape[0], dtype=x.dtype, device=x.device)
-        a = _ffn_args(x, w_gate, w_up, act)
-        a.y = y.data_ptr()
-        work = _ffn_work(lib, a, x.device, 0)  # noqa: F841  (held until the call is enqueued)
-        _call(lib.inet_policy_ffn_forward, x.device, "gated_ffn", C.byref(a))
-        ctx.save_for_backward(x, w_gate, w_up)
+        y, saved = _ffn_forward(x, w_gate, w_up, act)
+        ctx.save_for_backward(*saved)
         ctx.act = act
         return y
 
@@ -258,14 +278,14 @@ class _GatedFfn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, d_y):
         x, w_gate, w_up = ctx.saved_tensors
-        lib = _lib.load_policy()
+        lib, dev = _lib.load_policy(), x.device
         d_y = _rows(d_y)
         a = _ffn_args(x, w_gate, w_up, ctx.act)
-        new = lambda i, t: torch.empty(t.shape, dtype=t.dtype, device=t.device) if ctx.needs_input_grad[i] else None  # noqa: E731,E501
-        dx, dg, du = new(0, x), new(1, w_gate), new(2, w_up)
+        dx, dg, du = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+                      for t, need in zip((x, w_gate, w_up), ctx.needs_input_grad))
         d = _lib.InetFfnGrad(d_y.data_ptr(), _row_stride(d_y), _ptr(dx), _ptr(dg), _ptr(du))
-        work = _ffn_work(lib, a, x.device, 1)  # noqa: F841
-        _call(lib.inet_policy_ffn_backward, x.device, "gated_ffn backward", C.byref(a), C.byref(d))
+        work = _ffn_work(lib, a, dev, 1)  # noqa: F841
+        _call(lib.inet_policy_ffn_backward, dev.index, "gated_ffn backward", C.byref(a), C.byref(d))
         return dx, dg, du, None
 
 
@@ -274,50 +294,54 @@ def gated_ffn(x, w_gate, w_up, activation="silu"):
 
     x [..., D], w_gate and w_up [F, D] (torch.nn.Linear's layout), all bfloat16 or all float16; activation "silu",
     "gelu" (the tanh form) or "relu". Returns [..., F] of x's type. The backward pass computes the projections again."""
-    dev = _on_gpu(x=x, w_gate=w_gate, w_up=w_up)
-    _need(activation in ACTIVATIONS, f"activation {activation!r}: one of {ACTIVATIONS}")
-    _need(x.dim() >= 1 and w_gate.dim() == 2 and w_gate.shape == w_up.shape and x.shape[-1] == w_gate.shape[1],
-          f"x [..., D] with w_gate and w_up [F, D]: got {tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}")
-    _need(w_gate.shape[0] > 0 and w_gate.shape[1] > 0, "weights of size 0")
-    _need(x.dtype == w_gate.dtype == w_up.dtype, f"x, w_gate and w_up have to be of one type: got {x.dtype}, "
-                                                 f"{w_gate.dtype}, {w_up.dtype}")
+    _on_gpu(x=x, w_gate=w_gate, w_up=w_up)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r}: one of {ACTIVATIONS}")
+    xs, ws = x.shape, w_gate.shape
+    if len(xs) < 1 or len(ws) != 2 or w_up.shape != ws or xs[-1] != ws[1]:
+        raise ValueError(f"x [..., D] with w_gate and w_up [F, D]: got {tuple(xs)}, {tuple(ws)}, {tuple(w_up.shape)}")
+    if not (ws[0] > 0 and ws[1] > 0):
+        raise ValueError("weights of size 0")
+    if not (x.dtype == w_gate.dtype == w_up.dtype):
+        raise ValueError(f"x, w_gate and w_up have to be of one type: got {x.dtype}, {w_gate.dtype}, {w_up.dtype}")
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise HipUnsupported(f"gated_ffn of {x.dtype}: bfloat16 and float16 are implemented")
-    rows = x.reshape(-1, x.shape[-1])
+    rows = x if len(xs) == 2 else x.reshape(-1, xs[-1])
     if rows.shape[0] > 1 << 23:
         raise HipUnsupported(f"gated_ffn of {rows.shape[0]} rows: up to {1 << 23}")
-    y = _GatedFfn.apply(rows, w_gate, w_up, ACTIVATIONS.index(activation))
-    return y.view(*x.shape[:-1], w_gate.shape[0])
+    act = ACTIVATIONS.index(activation)
+    if torch.is_grad_enabled() and (rows.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        y = _GatedFfn.apply(rows, w_gate, w_up, act)
+    else:
+        y = _ffn_forward(rows, w_gate, w_up, act)[0]
+    return y if len(xs) == 2 else y.view(*xs[:-1], ws[0])
 
 
 # ------------------------------------------------------------------------------------------------ the norms
-def _norm_args(x, f, gate, scale, post, pre, eps):
-    a = _lib.InetNorm()
-    a.N, a.D = x.shape
-    a.dtype, a.eps = _CODES[x.dtype], eps
-    a.x, a.x_s = x.data_ptr(), _row_stride(x)
-    if f is not None:
-        a.f, a.f_s = f.data_ptr(), _row_stride(f)
-    if gate is not None:
-        a.gate_kind = 2 if gate.shape[1] == x.shape[1] and x.shape[1] > 1 else 1
-        a.gate, a.gate_s = gate.data_ptr(), _row_stride(gate)
-    a.scale, a.post_weight, a.pre_weight = _ptr(scale), _ptr(post), _ptr(pre)
-    return a
+def _norm_args(x, f, gate, scale, post, pre, eps, y=None, n=None):
+    N, D = x.shape
+    kind = 0 if gate is None else 2 if gate.shape[1] == D and D > 1 else 1
+    return _lib.InetNorm(N, D, _CODES[x.dtype], kind, eps, _row_stride(x), 0 if f is None else _row_stride(f),
+                         0 if gate is None else _row_stride(gate), x.data_ptr(), _ptr(f), _ptr(gate), _ptr(scale),
+                         _ptr(post), _ptr(pre), _ptr(y), _ptr(n))
+
+
+def _norm_forward(x, f, gate, scale, post, pre, eps):
+    x = _rows(x)
+    f, gate = None if f is None else _rows(f), None if gate is None else _rows(gate)
+    scale, post, pre = (None if t is None else t.contiguous() for t in (scale, post, pre))
+    y = None if f is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = None if pre is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a = _norm_args(x, f, gate, scale, post, pre, eps, y, n)
+    _call(_lib.load_policy().inet_policy_norm_forward, x.device.index, "block_norm", C.byref(a))
+    return y, n, (x, f, gate, scale, post, pre)
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, gate, scale, post, pre, eps):
-        x = _rows(x)
-        f, gate = (None if t is None else _rows(t) for t in (f, gate))
-        scale, post, pre = (None if t is None else t.contiguous() for t in (scale, post, pre))
-        lib = _lib.load_policy()
-        a = _norm_args(x, f, gate, scale, post, pre, eps)
-        new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)  # noqa: E731
-        y, n = (new() if f is not None else None), (new() if pre is not None else None)
-        a.y, a.n = _ptr(y), _ptr(n)
-        _call(lib.inet_policy_norm_forward, x.device, "block_norm", C.byref(a))
-        ctx.save_for_backward(x, f, gate, scale, post, pre)
+        y, n, saved = _norm_forward(x, f, gate, scale, post, pre, eps)
+        ctx.save_for_backward(*saved)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
         return y, n
@@ -328,19 +352,20 @@ class _BlockNorm(torch.autograd.Function):
         x, f, gate, scale, post, pre = ctx.saved_tensors
         if d_y is None and d_n is None:
             return (None,) * 7
-        lib = _lib.load_policy()
+        lib, dev = _lib.load_policy(), x.device
         a = _norm_args(x, f, gate, scale, post, pre, ctx.eps)
-        d_y, d_n = (None if t is None else t.contiguous() for t in (d_y, d_n))
-        new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        dx, df, dgate, dscale, dpost, dpre = map(new, (x, f, gate, scale, post, pre))
-        work = torch.empty(lib.inet_policy_norm_work(a.N, a.D), dtype=torch.uint8, device=x.device)
-        d = _lib.InetNormGrad(*map(_ptr, (d_y, d_n, dx, df, dgate, dscale, dpost, dpre, work)))
+        d_y, d_n = None if d_y is None else d_y.contiguous(), None if d_n is None else d_n.contiguous()
+        dx, df, dgate, dscale, dpost, dpre = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+                                              for t in (x, f, gate, scale, post, pre))
+        work = torch.empty(lib.inet_policy_norm_work(a.N, a.D), dtype=torch.uint8, device=dev)
+        d = _lib.InetNormGrad(_ptr(d_y), _ptr(d_n), dx.data_ptr(), _ptr(df), _ptr(dgate), _ptr(dscale), _ptr(dpost),
+                              _ptr(dpre), work.data_ptr())
         if pre is not None and d_n is None:      # (n took no part: its weight's gradient is zero)
             a.pre_weight = d.d_pre_weight = None
             dpre.zero_()
             if f is None:
                 return d_y, None, None, None, None, dpre, None
-        _call(lib.inet_policy_norm_backward, x.device, "block_norm backward", C.byref(a), C.byref(d))
+        _call(lib.inet_policy_norm_backward, dev.index, "block_norm backward", C.byref(a), C.byref(d))
         return dx, df, dgate, dscale, dpost, dpre, None
 
 
@@ -355,25 +380,36 @@ def block_norm(x, f=None, gate=None, scale=None, post_weight=None, pre_weight=No
     no norm before a next block. f None: no block before (y is x). Sums in 32 bits; n is the norm of y before y is
     rounded. Returns (y, n), n None without pre_weight."""
     dev = _on_gpu(x=x, f=f, gate=gate, scale=scale, post_weight=post_weight, pre_weight=pre_weight)
-    _need(x.dim() >= 1 and x.shape[-1] > 0, f"x has to be [..., D]: got {tuple(x.shape)}")
-    D = x.shape[-1]
-    _code("x", x)
+    xs = x.shape
+    if len(xs) < 1 or xs[-1] < 1:
+        raise ValueError(f"x has to be [..., D]: got {tuple(xs)}")
+    D = xs[-1]
+    if x.dtype not in _CODES:
+        raise _unsupported_type("x", x)
     if D > MAX_WIDTH:
         raise HipUnsupported(f"rows of {D} values: up to {MAX_WIDTH} are implemented")
-    for n, t, shapes in (("f", f, (x.shape,)), ("gate", gate, (x.shape, (*x.shape[:-1], 1)))):
-        if t is not None:
-            _need(tuple(t.shape) in [tuple(s) for s in shapes], f"{n} of {tuple(t.shape)} with x {tuple(x.shape)}")
-            _need(t.dtype == x.dtype, f"{n} has to be of x's type {x.dtype}: got {t.dtype}")
+    if f is not None and (f.shape != xs or f.dtype != x.dtype):
+        raise ValueError(f"f has to be as x, {tuple(xs)} of {x.dtype}: got {tuple(f.shape)} of {f.dtype}")
+    if gate is not None and (gate.dtype != x.dtype or (gate.shape != xs and gate.shape != (*xs[:-1], 1))):
+        raise ValueError(f"gate has to be {tuple(xs)} or {(*xs[:-1], 1)} of {x.dtype}: got {tuple(gate.shape)} of "
+                         f"{gate.dtype}")
     for n, t in (("scale", scale), ("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if t is not None:
-            _need(tuple(t.shape) == (D,) and t.dtype == torch.float32, f"{n} has to be [{D}] float32: got "
-                                                                       f"{tuple(t.shape)} {t.dtype}")
-    _need(f is not None or (gate is None and scale is None and post_weight is None),
-          "gate, scale and post_weight belong to a block's output f")
-    if f is None and pre_weight is None:
-        return x, None
-    rows = [None if t is None else t.reshape(-1, t.shape[-1]) for t in (x, f, gate)]
+        if t is not None and (t.shape != (D,) or t.dtype != torch.float32):
+            raise ValueError(f"{n} has to be [{D}] float32: got {tuple(t.shape)} of {t.dtype}")
+    if f is None:
+        if gate is not None or scale is not None or post_weight is not None:
+            raise ValueError("gate, scale and post_weight belong to a block's output f")
+        if pre_weight is None:
+            return x, None
+    flat = len(xs) == 2
+    rows = (x, f, gate) if flat else [None if t is None else t.reshape(-1, t.shape[-1]) for t in (x, f, gate)]
     if rows[0].shape[0] > 1 << 24:
-        raise HipUnsupported(f"block_norm of {rows[0].shape[0]} rows on {dev}: up to {1 << 24}")
-    y, n = _BlockNorm.apply(*rows, scale, post_weight, pre_weight, float(eps))
-    return (x if y is None else y.view(x.shape)), (None if n is None else n.view(x.shape))
+        raise HipUnsupported(f"block_norm of {rows[0].shape[0]} rows on cuda:{dev}: up to {1 << 24}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, f, gate, scale, post_weight, pre_weight)):
+        y, n = _BlockNorm.apply(*rows, scale, post_weight, pre_weight, float(eps))
+    else:
+        y, n, _ = _norm_forward(*rows, scale, post_weight, pre_weight, float(eps))
+    if flat:
+        return (x if y is None else y), n
+    return (x if y is None else y.view(xs)), (None if n is None else n.view(xs))

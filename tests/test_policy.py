@@ -81,7 +81,7 @@ def test_entry_points_need_the_gpu():
 class _OnGpu:
     """Lets the shape and type checks run on CPU tensors."""
     def __enter__(self):
-        self.saved, policy._on_gpu = policy._on_gpu, lambda **x: torch.device("cpu")
+        self.saved, policy._on_gpu = policy._on_gpu, lambda **x: 0
         self.call, policy._call = policy._call, lambda *a: pytest.fail("a refused call reached the library")
 
     def __exit__(self, *a):
