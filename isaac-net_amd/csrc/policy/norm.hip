@@ -18,33 +18,59 @@ namespace pol {
 constexpr int NORM_WG = 256;
 constexpr int NORM_BLOCKS = 1024;            // workgroups of the backward pass, at most
 
-// the sum over a row's LP lanes (LP <= 64), or over the workgroup (LP = 256; s: four words of LDS of its own)
+// the sum over a row's LP lanes (LP <= 64), or over the workgroup (LP = 256; s: four words of LDS of its own): along the
+// rows of 16 lanes by rotations, across them by swaps of rows and halves
+template <int CTRL> DEV float lane_turn(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
 template <int LP> DEV float row_sum(float x, float* s) {
-#pragma unroll
-    for (int o = 1; o < (LP < 64 ? LP : 64); o <<= 1) x += __shfl_xor(x, o);
+    x += lane_turn<0x128>(x);
+    x += lane_turn<0x124>(x);
+    x += lane_turn<0x122>(x);
+    x += lane_turn<0x121>(x);
+    if constexpr (LP >= 32) {
+        const unsigned u = __builtin_bit_cast(unsigned, x);
+        const auto v = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const unsigned even = v[0], odd = v[1];
+        x = __builtin_bit_cast(float, even) + __builtin_bit_cast(float, odd);
+    }
+    if constexpr (LP >= 64) {
+        const unsigned u = __builtin_bit_cast(unsigned, x);
+        const auto v = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const unsigned low = v[0], high = v[1];
+        x = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
+    }
     if constexpr (LP == 256) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
         __syncthreads();
-        x = s[0] + s[1] + s[2] + s[3];
+        x = (s[0] + s[1]) + (s[2] + s[3]);
     }
     return x;
 }
 
-// group j of a lane's values of a row: eight in sequence, or eight LP apart
-template <typename T, int LP, bool VEC> DEV void row_load(const T* __restrict__ p, int c, int j, int D, float (&x)[8]) {
-    if constexpr (VEC) {
-        const int at = (j * LP + c) * 8;
-        if (at < D) load8(p + at, 8, true, x);
-        else
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-    } else {
-        for (int e = 0; e < 8; ++e) {
-            const int at = (j * 8 + e) * LP + c;
-            x[e] = at < D ? (float)p[at] : 0.0f;
+// a row on its way from memory: the lane's NJ groups of eight, in sequence, or eight values LP apart
+template <typename T, int LP, int NJ, bool VEC> struct Row {
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    V8 v[NJ];
+    DEV void load(const T* __restrict__ p, int c, int D) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            v[j] = V8{};
+            if constexpr (VEC) {
+                const int at = (j * LP + c) * 8;
+                if (at < D) v[j] = *(const V8*)(p + at);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int at = (j * 8 + e) * LP + c;
+                    if (at < D) v[j][e] = p[at];
+                }
+            }
         }
     }
-}
+    DEV float at(int j, int e) const { return (float)v[j][e]; }
+};
 
 template <typename T, int LP, bool VEC> DEV void row_store(T* __restrict__ p, int c, int j, int D, const float (&x)[8]) {
     if constexpr (VEC) {
@@ -56,11 +82,13 @@ template <typename T, int LP, bool VEC> DEV void row_store(T* __restrict__ p, in
             } else {
                 typedef T V8 __attribute__((ext_vector_type(8)));
                 V8 v;
+#pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = (T)x[e];
                 *(V8*)(p + at) = v;
             }
         }
     } else {
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int at = (j * 8 + e) * LP + c;
             if (at < D) p[at] = (T)x[e];
@@ -69,11 +97,18 @@ template <typename T, int LP, bool VEC> DEV void row_store(T* __restrict__ p, in
 }
 
 // weights: 1 where there are none
-template <int LP, bool VEC> DEV void weight_load(const float* p, int c, int j, int D, float (&x)[8]) {
-    if (p) row_load<float, LP, VEC>(p, c, j, D, x);
-    else
-        for (int e = 0; e < 8; ++e) x[e] = 1.0f;
-}
+template <int LP, int NJ, bool VEC> struct Weights {
+    Row<float, LP, NJ, VEC> r;
+    DEV void load(const float* p, int c, int D) {
+        if (p) r.load(p, c, D);
+        else
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r.v[j][e] = 1.0f;
+    }
+    DEV float at(int j, int e) const { return r.v[j][e]; }
+};
 
 template <typename T, int LP, int NJ, bool VEC>
 __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
@@ -84,42 +119,51 @@ __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
     const bool live = row < a.N;
     const int D = live ? a.D : 0;
     const float inv = 1.0f / (float)a.D;
-    float y[NJ][8], f[NJ][8];
-    float sf = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        row_load<T, LP, VEC>((const T*)a.x + row * a.x_s, c, j, D, y[j]);
-        if (a.f) {
-            row_load<T, LP, VEC>((const T*)a.f + row * a.f_s, c, j, D, f[j]);
-            for (int e = 0; e < 8; ++e) sf += f[j][e] * f[j][e];
-        }
-    }
+    Row<T, LP, NJ, VEC> x, f, gt;
+    x.load((const T*)a.x + row * a.x_s, c, D);
+    float y[NJ][8];
     if (a.f) {
-        const float rf = a.post_weight ? rsqrtf(row_sum<LP>(sf, s_sum) * inv + a.eps) : 1.0f;
+        f.load((const T*)a.f + row * a.f_s, c, D);
+        if (a.gate_kind == 2) gt.load((const T*)a.gate + row * a.gate_s, c, D);
         const float row_gate = a.gate_kind == 1 && live ? (float)((const T*)a.gate)[row * a.gate_s] : 1.0f;
+        Weights<LP, NJ, VEC> w, s;
+        w.load(a.post_weight, c, a.D);
+        s.load(a.scale, c, a.D);
+        float rf = 1.0f;
+        if (a.post_weight) {
+            float sf = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sf += f.at(j, e) * f.at(j, e);
+            rf = rsqrtf(row_sum<LP>(sf, s_sum) * inv + a.eps);
+        }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            float w[8], s[8], gt[8];
-            weight_load<LP, VEC>(a.post_weight, c, j, D, w);
-            weight_load<LP, VEC>(a.scale, c, j, D, s);
-            if (a.gate_kind == 2) row_load<T, LP, VEC>((const T*)a.gate + row * a.gate_s, c, j, D, gt);
-            for (int e = 0; e < 8; ++e) {
-                const float h = f[j][e] * rf * w[e] * s[e];
-                y[j][e] += h * (a.gate_kind == 2 ? gt[e] : row_gate);
-            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[j][e] = x.at(j, e) + f.at(j, e) * rf * w.at(j, e) * s.at(j, e) * (a.gate_kind == 2 ? gt.at(j, e) : row_gate);
             row_store<T, LP, VEC>((T*)a.y + row * (int64_t)a.D, c, j, D, y[j]);
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[j][e] = x.at(j, e);
     }
     if (a.pre_weight) {
+        Weights<LP, NJ, VEC> w;
+        w.load(a.pre_weight, c, a.D);
         float sy = 0.0f;
+#pragma unroll
         for (int j = 0; j < NJ; ++j)
+#pragma unroll
             for (int e = 0; e < 8; ++e) sy += y[j][e] * y[j][e];
         const float ry = rsqrtf(row_sum<LP>(sy, s_sum) * inv + a.eps);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            float w[8];
-            weight_load<LP, VEC>(a.pre_weight, c, j, D, w);
-            for (int e = 0; e < 8; ++e) y[j][e] *= ry * w[e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[j][e] *= ry * w.at(j, e);
             row_store<T, LP, VEC>((T*)a.n + row * (int64_t)a.D, c, j, D, y[j]);
         }
     }
@@ -134,78 +178,90 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
     const float inv = 1.0f / (float)a.D;
     float ds[NJ][8] = {}, dpost[NJ][8] = {}, dpre[NJ][8] = {};
     const int64_t per = (a.N + (int64_t)gridDim.x * RW - 1) / ((int64_t)gridDim.x * RW);
+    const bool pre = a.pre_weight && d.d_n;
+    Row<T, LP, NJ, VEC> x, f, gt, dy, dn;
+    float row_gate = 1.0f;
+    auto fetch = [&](int64_t row) {                  // the next row's values, while the one before is computed with
+        const int D = row < a.N ? a.D : 0;
+        x.load((const T*)a.x + row * a.x_s, c, D);
+        dy.load((const T*)d.d_y + row * (int64_t)a.D, c, d.d_y ? D : 0);
+        if (a.f) {
+            f.load((const T*)a.f + row * a.f_s, c, D);
+            if (a.gate_kind == 2) gt.load((const T*)a.gate + row * a.gate_s, c, D);
+            else if (a.gate_kind == 1 && D) row_gate = (float)((const T*)a.gate)[row * a.gate_s];
+        }
+        if (pre) dn.load((const T*)d.d_n + row * (int64_t)a.D, c, D);
+    };
+    fetch((int64_t)blockIdx.x * RW + sub);
     for (int64_t it = 0; it < per; ++it) {
         const int64_t row = (it * gridDim.x + blockIdx.x) * RW + sub;
         const bool live = row < a.N;
         const int D = live ? a.D : 0;
-        float y[NJ][8], f[NJ][8] = {}, dy[NJ][8];
+        float y[NJ][8], h[NJ][8], g[NJ][8], dv[NJ][8], z[NJ][8];
         float sf = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            row_load<T, LP, VEC>((const T*)a.x + row * a.x_s, c, j, D, y[j]);
-            if (d.d_y) row_load<T, LP, VEC>((const T*)d.d_y + row * (int64_t)a.D, c, j, D, dy[j]);
-            else
-                for (int e = 0; e < 8; ++e) dy[j][e] = 0.0f;
-            if (a.f) {
-                row_load<T, LP, VEC>((const T*)a.f + row * a.f_s, c, j, D, f[j]);
-                for (int e = 0; e < 8; ++e) sf += f[j][e] * f[j][e];
-            }
-        }
-        const float rf = a.f && a.post_weight ? rsqrtf(row_sum<LP>(sf, s_sum) * inv + a.eps) : 1.0f;
-        const float row_gate = a.gate_kind == 1 && live ? (float)((const T*)a.gate)[row * a.gate_s] : 1.0f;
-        float gt[NJ][8];
-        if (a.f)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                float w[8], s[8];
-                weight_load<LP, VEC>(a.post_weight, c, j, D, w);
-                weight_load<LP, VEC>(a.scale, c, j, D, s);
-                if (a.gate_kind == 2) row_load<T, LP, VEC>((const T*)a.gate + row * a.gate_s, c, j, D, gt[j]);
-                else
-                    for (int e = 0; e < 8; ++e) gt[j][e] = row_gate;
-                for (int e = 0; e < 8; ++e) {
-                    f[j][e] *= rf;
-                    y[j][e] += gt[j][e] * s[e] * w[e] * f[j][e];
-                }
-            }
-        if (a.pre_weight && d.d_n) {
-            float sy = 0.0f, sz = 0.0f, dz[NJ][8];
-            for (int j = 0; j < NJ; ++j)
-                for (int e = 0; e < 8; ++e) sy += y[j][e] * y[j][e];
-            const float ry = rsqrtf(row_sum<LP>(sy, s_sum) * inv + a.eps);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                float w[8];
-                row_load<T, LP, VEC>((const T*)d.d_n + row * (int64_t)a.D, c, j, D, dz[j]);
-                weight_load<LP, VEC>(a.pre_weight, c, j, D, w);
-                for (int e = 0; e < 8; ++e) {
-                    y[j][e] *= ry;
-                    dpre[j][e] += dz[j][e] * y[j][e];
-                    dz[j][e] *= w[e];
-                    sz += dz[j][e] * y[j][e];
-                }
-            }
-            sz = row_sum<LP>(sz, s_sum) * inv;
-            for (int j = 0; j < NJ; ++j)
-                for (int e = 0; e < 8; ++e) dy[j][e] += ry * (dz[j][e] - y[j][e] * sz);
-        }
         for (int j = 0; j < NJ; ++j)
-            row_store<T, LP, VEC>((T*)d.d_x + row * (int64_t)a.D, c, j, D, dy[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[j][e] = x.at(j, e);
+                dv[j][e] = dy.at(j, e);
+                h[j][e] = a.f ? f.at(j, e) : 0.0f;
+                g[j][e] = a.gate_kind == 2 ? gt.at(j, e) : row_gate;
+                z[j][e] = pre ? dn.at(j, e) : 0.0f;
+                sf += h[j][e] * h[j][e];
+            }
+        if (it + 1 < per) fetch(row + (int64_t)gridDim.x * RW);
+        Weights<LP, NJ, VEC> w, s, wp;
+        float rf = 1.0f;
+        if (a.f) {
+            w.load(a.post_weight, c, a.D);
+            s.load(a.scale, c, a.D);
+            if (a.post_weight) rf = rsqrtf(row_sum<LP>(sf, s_sum) * inv + a.eps);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h[j][e] *= rf;                   // f^
+                    y[j][e] += g[j][e] * s.at(j, e) * w.at(j, e) * h[j][e];
+                }
+        }
+        if (pre) {
+            wp.load(a.pre_weight, c, a.D);
+            float sy = 0.0f, sz = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    sy += y[j][e] * y[j][e];
+                    sz += z[j][e] * wp.at(j, e) * y[j][e];
+                }
+            const float ry = rsqrtf(row_sum<LP>(sy, s_sum) * inv + a.eps);
+            sz = row_sum<LP>(sz, s_sum) * inv * ry;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    y[j][e] *= ry;                   // z of the formulas
+                    dpre[j][e] += z[j][e] * y[j][e];
+                    dv[j][e] += ry * (z[j][e] * wp.at(j, e) - y[j][e] * sz);
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) row_store<T, LP, VEC>((T*)d.d_x + row * (int64_t)a.D, c, j, D, dv[j]);
         if (a.f) {
             float sd = 0.0f, sg = 0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                float w[8], s[8], dg[8];
-                weight_load<LP, VEC>(a.post_weight, c, j, D, w);
-                weight_load<LP, VEC>(a.scale, c, j, D, s);
+                float dg[8];
+#pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float t = dy[j][e] * gt[j][e], h = f[j][e] * w[e];
-                    ds[j][e] += t * h;
-                    dpost[j][e] += t * s[e] * f[j][e];
-                    dg[e] = dy[j][e] * s[e] * h;
+                    const float t = dv[j][e] * g[j][e], sw = s.at(j, e) * w.at(j, e);
+                    ds[j][e] += t * h[j][e] * w.at(j, e);
+                    dpost[j][e] += t * s.at(j, e) * h[j][e];
+                    dg[e] = dv[j][e] * sw * h[j][e];
                     sg += dg[e];
-                    dy[j][e] = t * s[e] * w[e];
-                    sd += dy[j][e] * f[j][e];
+                    dv[j][e] = t * sw;
+                    sd += dv[j][e] * h[j][e];
                 }
                 if (a.gate_kind == 2) row_store<T, LP, VEC>((T*)d.d_gate + row * (int64_t)a.D, c, j, D, dg);
             }
@@ -216,8 +272,9 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
             sd = a.post_weight ? row_sum<LP>(sd, s_sum) * inv : 0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                for (int e = 0; e < 8; ++e) dy[j][e] = rf * (dy[j][e] - f[j][e] * sd);
-                row_store<T, LP, VEC>((T*)d.d_f + row * (int64_t)a.D, c, j, D, dy[j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dv[j][e] = rf * (dv[j][e] - h[j][e] * sd);
+                row_store<T, LP, VEC>((T*)d.d_f + row * (int64_t)a.D, c, j, D, dv[j]);
             }
         }
     }
@@ -228,13 +285,16 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
         for (int j = 0; j < NJ; ++j) {
             if constexpr (RW > 1) {
                 __syncthreads();
+#pragma unroll
                 for (int e = 0; e < 8; ++e) s_w[(sub * 8 + e) * LP + c] = x[j][e];
                 __syncthreads();
                 if (sub == 0)
                     for (int r = 1; r < RW; ++r)
+#pragma unroll
                         for (int e = 0; e < 8; ++e) x[j][e] += s_w[(r * 8 + e) * LP + c];
             }
             if (sub == 0)
+#pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int at = VEC ? (j * LP + c) * 8 + e : (j * 8 + e) * LP + c;
                     if (at < a.D) out[m * a.D + at] = x[j][e];
@@ -248,31 +308,39 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
     if (a.pre_weight) give(dpre, 2);
 }
 
-// the workgroups' partial rows added up, 64 columns a workgroup, its waves' shares in order
-__global__ __launch_bounds__(NORM_WG) void norm_weights_kernel(const float* __restrict__ work, int blocks, int D,
-                                                               float* ds, float* dpost, float* dpre) {
-    __shared__ float s[4][64];
+// the workgroups' partial rows added up, 64 columns a workgroup of 16 waves, the waves' shares in order
+__global__ __launch_bounds__(1024) void norm_weights_kernel(const float* __restrict__ work, int blocks, int D, float* ds,
+                                                            float* dpost, float* dpre) {
+    __shared__ float s[16][64];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, m = blockIdx.y;
     float* out = m == 0 ? ds : m == 1 ? dpost : dpre;
     const int col = blockIdx.x * 64 + lane;
     if (!out) return;
-    const int from = blocks * w / 4, to = blocks * (w + 1) / 4;
-    float x[4] = {};
+    const int from = blocks * w / 16, to = blocks * (w + 1) / 16;
+    float x[8] = {};
     if (col < D) {
         const float* p = work + (int64_t)m * D + col;
         int b = from;
-        for (; b + 4 <= to; b += 4)
-            for (int u = 0; u < 4; ++u) x[u] += p[(int64_t)(b + u) * 3 * D];
+        for (; b + 8 <= to; b += 8)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] += p[(int64_t)(b + u) * 3 * D];
         for (; b < to; ++b) x[0] += p[(int64_t)b * 3 * D];
     }
-    s[w][lane] = (x[0] + x[1]) + (x[2] + x[3]);
+    s[w][lane] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     __syncthreads();
-    if (w == 0 && col < D) out[col] = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
+    if (w == 0 && col < D) {
+        float y = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) y += s[u][lane];
+        out[col] = y;
+    }
 }
 
+// workgroups of the backward pass: one a compute unit, or enough that each takes eight groups of rows (the partial rows
+// are as long as the data's), as many as run at once at most
 static int blocks_for(int64_t N, int rows) {
-    const int64_t need = (N + rows - 1) / rows;
-    return (int)(need < NORM_BLOCKS ? need : NORM_BLOCKS);
+    const int64_t need = (N + rows - 1) / rows, want = need / 8 > 256 ? need / 8 : 256, n = need < want ? need : want;
+    return (int)(n < NORM_BLOCKS ? n : NORM_BLOCKS);
 }
 
 template <typename T, int LP, int NJ, bool VEC>
@@ -286,7 +354,7 @@ static int launch(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
     const int blocks = blocks_for(a.N, RW);
     hipLaunchKernelGGL((norm_backward_kernel<T, LP, NJ, VEC>), dim3(blocks), dim3(NORM_WG), 0, st, a, *d);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
-    hipLaunchKernelGGL(norm_weights_kernel, dim3((a.D + 63) / 64, 3), dim3(NORM_WG), 0, st, d->work, blocks, a.D,
+    hipLaunchKernelGGL(norm_weights_kernel, dim3((a.D + 63) / 64, 3), dim3(1024), 0, st, d->work, blocks, a.D,
                        a.f ? d->d_scale : nullptr, a.f ? d->d_post_weight : nullptr,
                        a.pre_weight ? d->d_pre_weight : nullptr);
     return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
@@ -356,7 +424,7 @@ int32_t inet_policy_norm_backward(const InetNorm* a, const InetNormGrad* d, void
     if ((d->d_scale && !a->scale) || (d->d_post_weight && !a->post_weight) || (d->d_pre_weight && !a->pre_weight))
         return INET_POLICY_EINVAL;
     if (a->N == 0) {                             // (no rows: the second kernel alone, over no partial rows, writes zeros)
-        hipLaunchKernelGGL(pol::norm_weights_kernel, dim3((a->D + 63) / 64, 3), dim3(pol::NORM_WG), 0,
+        hipLaunchKernelGGL(pol::norm_weights_kernel, dim3((a->D + 63) / 64, 3), dim3(1024), 0,
                            (hipStream_t)stream, d->work, 0, a->D, d->d_scale, d->d_post_weight, d->d_pre_weight);
         return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
     }
