@@ -203,20 +203,64 @@ template <typename T, int C, bool VEC> DEV void store_rows(const T* s, T* __rest
     }
 }
 
-// the state's tiles of 16 columns, from and to [K][V] at the first of the columns; off: row 4 g, column n
+// the state's tiles of 16 columns, from and to [K][V] at the first of the columns; off: row 4 g, column n, in bytes.
+// (p and what is added to it is the same in all lanes, so an access is a base, one offset for all, and no arithmetic)
+template <typename P> DEV P at_byte(P p, uint32_t off) { return (P)((uintptr_t)p + off); }
 template <int KT> DEV void state_load(f32x4 (&S)[KT], const float* __restrict__ p, uint32_t off, int V, int K, int g) {
+    if (K == KT * 16) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            S[kt][e] = kt * 16 + 4 * g + e < K ? p[off + (uint32_t)((kt * 16 + e) * V)] : 0.0f;
+            for (int e = 0; e < 4; ++e) S[kt][e] = *at_byte(p + (kt * 16 + e) * V, off);
+    } else {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[kt][e] = kt * 16 + 4 * g + e < K ? *at_byte(p + (kt * 16 + e) * V, off) : 0.0f;
+    }
 }
 template <int KT> DEV void state_store(const f32x4 (&S)[KT], float* __restrict__ p, uint32_t off, int V, int K, int g) {
+    if (K == KT * 16) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (kt * 16 + 4 * g + e < K) p[off + (uint32_t)((kt * 16 + e) * V)] = S[kt][e];
+            for (int e = 0; e < 4; ++e) *at_byte(p + (kt * 16 + e) * V, off) = S[kt][e];
+    } else {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (kt * 16 + 4 * g + e < K) *at_byte(p + (kt * 16 + e) * V, off) = S[kt][e];
+    }
+}
+// the same for 16 columns of a chunk's rows (row_s apart), `left` of them inside the window
+template <int RT> DEV void rows_load(f32x4 (&x)[RT], const float* __restrict__ p, uint32_t off, int64_t row_s, int left, int g) {
+    if (left >= RT * 16) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[rt][e] = *at_byte(p + (rt * 16 + e) * row_s, off);
+    } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[rt][e] = rt * 16 + 4 * g + e < left ? *at_byte(p + (rt * 16 + e) * row_s, off) : 0.0f;
+    }
+}
+template <int RT> DEV void rows_store(const f32x4 (&x)[RT], float* __restrict__ p, uint32_t off, int64_t row_s, int left, int g) {
+    if (left >= RT * 16) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *at_byte(p + (rt * 16 + e) * row_s, off) = x[rt][e];
+    } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (rt * 16 + 4 * g + e < left) *at_byte(p + (rt * 16 + e) * row_s, off) = x[rt][e];
+    }
 }
 
 // keeps what is computed from x inside the loop: addresses are cheaper to compute again than to hold in registers

@@ -123,7 +123,7 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
     };
     if (chunks) fetch((chunks - 1) * C);
 
-    uint32_t at = (uint32_t)(4 * g * d.V + w * 16 + n), at_err = (uint32_t)(4 * g * row_s + w * 16 + n);
+    uint32_t at = 4 * (uint32_t)(4 * g * d.V + w * 16 + n), at_err = 4 * (uint32_t)(4 * g * row_s + w * 16 + n);
     f32x4 S[KT] = {};                               // the gradient of the state, 16 columns
     if (mine && gr.d_state_out) state_load(S, gr.d_state_out + bh * d.K * d.V + c0, at, d.V, d.K, g);
 
@@ -141,12 +141,7 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
             f32x4 z[RT] = {}, u[RT];
             column_gradients<C, KP, NP>(S, true, z, u, s.gates, s.ln, Lds::LL, Kr, P, O, w * 16, n, g);
             if (mine) {
-                float* zs = gr.err_grad + rows0 + t0 * row_s;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (t0 + rt * 16 + 4 * g + e < d.T) zs[at_err + (uint32_t)((rt * 16 + e) * row_s)] = z[rt][e];
+                rows_store(z, gr.err_grad + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
                 if (ch + 1 < chunks)
                     state_store(S, gr.chunk_grad + (bh * (chunks - 1) + ch) * d.K * d.V + c0, at, d.V, d.K, g);
             }
@@ -157,20 +152,35 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
     if (mine && gr.d_state) state_store(S, gr.d_state + bh * d.K * d.V + c0, at, d.V, d.K, g);
 }
 
-// the rows' sums that the log-decays' gradients are made of: q . dQ, k . dK+, k . dK-, the state's share of k . dK- (each by
-// the key rows' part), E . Z, and <S, dS> by wave
-template <int C> struct Sums {
-    float q[4][C], kp[4][C], km[4][C], ks[4][C], ez[C], ss[4];
+// the rows' sums that the log-decays' gradients are made of, by the key rows' part: q . dQ, k . dK+, k . dK-, the state's
+// share of k . dK- (in the triangles' place when those are done with); and E . Z, and <S, dS> by wave
+template <int C> struct Parts {
+    float q[4][C], kp[4][C], km[4][C], ks[4][C];
+};
+template <int C> struct alignas(16) Sums {
+    float ez[C], ss[4];
 };
 
-// LDS of the chunk kernel in bytes: K and Q, X, Z and dO by rows (of vp + 8), gates and sums
-template <typename T, int C, int KP> constexpr size_t chunk_lds(int vp) {
-    constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1;
-    return sizeof(Gates<C>) + sizeof(Sums<C>) + sizeof(__bf16) * (2 * NP * C * (KP + 8) + (2 * NO + NP) * C * (vp + 8));
+// D and M of a chunk in LDS (as P: columns in the order perm()), in the place of X, Z and dO when those are done with
+template <typename T, int C> struct Inner {
+    static constexpr int NO = Elem<T>::ord + 1, LC = C + 8, SIZE = 2 * NO * C * LC;
+    Planes<NO> D, M;
+    DEV explicit Inner(__bf16* p) : D{p, LC, C * LC}, M{p + NO * C * LC, LC, C * LC} {}
+};
+
+// LDS of the chunk kernel in bytes: gates and sums, K and Q, and the rows X, Z and dO (of vp + 8) with the triangles in
+// their place at the end, Z and dO in the order in which the one-chunk kernel can have its own triangles in X's place
+template <typename T, int C> constexpr size_t rows_lds(int vp, size_t triangles) {
+    const size_t row = sizeof(__bf16) * C * (vp + 8), NP = Elem<T>::planes, NO = Elem<T>::ord + 1, x = NO * row,
+                 all = (NO + NP) * row + (x > triangles ? x : triangles), in = sizeof(__bf16) * Inner<T, C>::SIZE;
+    return all > in ? all : in;
+}
+template <typename T, int C, int KP> constexpr size_t chunk_lds(int vp, size_t triangles = 0) {
+    return sizeof(Gates<C>) + sizeof(Sums<C>) + sizeof(__bf16) * 2 * Elem<T>::planes * C * (KP + 8) +
+           rows_lds<T, C>(vp, triangles);
 }
 
-// X = beta E and dbeta's E . Z by rows; Z from memory (err_grad), and dV = beta Z to there, where z_in, else as it is in
-// LDS already
+// X = beta E, dbeta's E . Z and dV = beta Z by rows; Z from memory (err_grad) where z_in, else as it is in LDS already
 template <typename T, int C, bool VEC, int NO>
 DEV void stage_errors(const InetDelta& d, const float* z_in, T* dv, int64_t row0, int64_t row_s, int steps, int vp,
                       const Gates<C>& gates, const Planes<NO>& X, const Planes<NO>& Z, Sums<C>& sums) {
@@ -185,18 +195,18 @@ DEV void stage_errors(const InetDelta& d, const float* z_in, T* dv, int64_t row0
                 if (r < steps && c < d.V) load8(z_in + row0 + r * row_s + c, d.V - c, VEC, z);
                 Z.put4(r, c, z[0], z[1], z[2], z[3]);
                 Z.put4(r, c + 4, z[4], z[5], z[6], z[7]);
-                if (r < steps && c < d.V) {
-                    const float lo[4] = {beta * z[0], beta * z[1], beta * z[2], beta * z[3]},
-                                hi[4] = {beta * z[4], beta * z[5], beta * z[6], beta * z[7]};
-                    store4(dv + row0 + r * row_s + c, d.V - c, VEC, lo);
-                    store4(dv + row0 + r * row_s + c + 4, d.V - c - 4, VEC, hi);
-                }
             } else {
                 const Frag<NO> f = Z.frag(r, c);
 #pragma unroll
                 for (int m = 0; m < NO; ++m)
 #pragma unroll
                     for (int u = 0; u < 8; ++u) z[u] += (float)f.p[m][u];
+            }
+            if (r < steps && c < d.V) {
+                const float lo[4] = {beta * z[0], beta * z[1], beta * z[2], beta * z[3]},
+                            hi[4] = {beta * z[4], beta * z[5], beta * z[6], beta * z[7]};
+                store4(dv + row0 + r * row_s + c, d.V - c, VEC, lo);
+                store4(dv + row0 + r * row_s + c + 4, d.V - c - 4, VEC, hi);
             }
             X.put4(r, c, beta * e[0], beta * e[1], beta * e[2], beta * e[3]);
             X.put4(r, c + 4, beta * e[4], beta * e[5], beta * e[6], beta * e[7]);
@@ -216,140 +226,165 @@ DEV void row8(const float* __restrict__ p, bool in, int v, int V, bool vec, floa
 }
 
 // The gradients of q, k and the gates of one chunk, from K, Q, X, Z and dO in LDS and the state S before the chunk and its
-// gradient dS after it (NULL: zero). Wave w takes the steps of tile w % RT as its columns, and the key rows' tiles
-// w / RT, w / RT + 4 / RT, ...
+// gradient dS after it (NULL: zero). A wave takes key rows' tiles (and, where there are fewer than four of those, its share
+// of the steps' tiles), so that S and dS are read and split once; the triangles D and M wait in registers until X, Z and
+// dO, at `place`, are done with.
 template <typename T, int C, int KP, bool VEC, int NP, int NO>
 DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int h, int t0, const float* __restrict__ S,
                          const float* __restrict__ dS, const Gates<C>& gates, Sums<C>& sums, const Planes<NP>& Kr,
-                         const Planes<NP>& Qr, const Planes<NO>& X, const Planes<NO>& Z, const Planes<NP>& O, int vp) {
-    constexpr int ORD = Elem<T>::ord, RT = C / 16, KT = KP / 16, PARTS = 4 / RT;
+                         const Planes<NP>& Qr, const Planes<NO>& X, const Planes<NO>& Z, const Planes<NP>& O,
+                         __bf16* place, int vp) {
+    constexpr int ORD = Elem<T>::ord, RT = C / 16, KT = KP / 16, KW = KT < 4 ? KT : 4, TW = 4 / KW, TN = RT / TW;
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, hk = h / (d.H / d.Hk);
     const T* q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2];
     const T* k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2];
-    const int tt = w % RT, part = w / RT, i0 = tt * 16 + n;         // the wave's steps; this lane's
-    // the triangles' columns of this wave's steps, as operands: dt: D^T[j][i0]; dn: D[i][i0]; mt: M^T[i][i0] ([i < i0]:
-    // M[i0][i]); mn: M[i][i0]
-    f32x4 dt[RT] = {}, dn[RT] = {}, mt[RT] = {}, mn[RT] = {};
-    for (int v = 0; v < vp; v += 32) {
-        const Frag<NO> xi = X.frag(i0, v + 8 * g), zi = Z.frag(i0, v + 8 * g);
-        const Frag<NP> oi = O.frag(i0, v + 8 * g);
+    // row tile it of D (from dO) and of M (from Z): the lane's step i, steps j = 4 g + e of an earlier tile
+    constexpr int PASSES = C == 64 ? 2 : 1;
+    const int it = C == 64 ? w : w & 1;
+    f32x4 tri[PASSES][RT] = {};
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+        const int i = it * 16 + n;
+        const bool m = C == 64 ? pass : w >> 1;
+        for (int v = 0; v < vp; v += 32) {
+            if (m) {
+                const Frag<NO> z = Z.frag(i, v + 8 * g);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    if (r <= it) tri[pass][r] = mma<ORD>(X.frag(r * 16 + n, v + 8 * g), z, tri[pass][r]);
+            } else {
+                const Frag<NP> o = O.frag(i, v + 8 * g);
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    if (r <= it) tri[pass][r] = mma<ORD>(X.frag(r * 16 + n, v + 8 * g), o, tri[pass][r]);
+            }
+        }
+        const float f = m ? -gates.beta[i] : d.scale;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            if (r <= tt) {
-                const Frag<NO> x = X.frag(r * 16 + n, v + 8 * g);
-                dt[r] = mma<ORD>(x, oi, dt[r]);
-                mt[r] = mma<ORD>(x, zi, mt[r]);
-            }
-            if (r >= tt) {
-                dn[r] = mma<ORD>(O.frag(r * 16 + n, v + 8 * g), xi, dn[r]);
-                mn[r] = mma<ORD>(Z.frag(r * 16 + n, v + 8 * g), xi, mn[r]);
-            }
-        }
-    }
-    const float beta = gates.beta[i0];
+            const int j = r * 16 + 4 * g;
+            if (r <= it) {
+                const f32x4 dec = (r == it ? decay4<C, true>(gates, i, j) : decay4<C, false>(gates, i, j)) * f;
+                tri[pass][r] *= dec;
+                if (m && r == it)
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int i = r * 16 + 4 * g;
-        const f32x4 bt = *(const f32x4*)(gates.beta + i);
-        if (r <= tt) {
-            const f32x4 dec = r == tt ? decay4<C, true>(gates, i0, i) : decay4<C, false>(gates, i0, i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dt[r][e] *= d.scale * dec[e];
-                mt[r][e] = i + e < i0 ? -mt[r][e] * beta * dec[e] : 0.0f;
-            }
-        }
-        if (r >= tt) {
-            f32x4 dec;                             // Gam_{i + e, i0}
-            const float out = gates.out[r][i0];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                dec[e] = r > tt ? gates.in[i + e] * out
-                                : i + e >= i0 && gates.seg[i + e] == gates.seg[i0]
-                                      ? expf((float)(gates.G[i + e] - gates.G[i0])) : 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dn[r][e] *= d.scale * dec[e];
-                mn[r][e] = i + e > i0 ? -mn[r][e] * bt[e] * dec[e] : 0.0f;
+                    for (int e = 0; e < 4; ++e) tri[pass][r][e] = j + e < i ? tri[pass][r][e] : 0.0f;
             }
         }
     }
-    Frag<NO> dtf[RT / 2], dnf[RT / 2], mtf[RT / 2], mnf[RT / 2];
-    for (int p = 0; p < RT / 2; ++p) {
-        dtf[p] = split_tiles<NO>(dt[2 * p], dt[2 * p + 1]);
-        dnf[p] = split_tiles<NO>(dn[2 * p], dn[2 * p + 1]);
-        mtf[p] = split_tiles<NO>(mt[2 * p], mt[2 * p + 1]);
-        mnf[p] = split_tiles<NO>(mn[2 * p], mn[2 * p + 1]);
-    }
-    const float a = gates.a[i0], c = gates.c[i0], ya = -beta * a, oa = d.scale * a;
-    const int t = t0 + i0;
-    float sq = 0.0f, sp = 0.0f, sn = 0.0f, sc = 0.0f, ss = 0.0f;
-    for (int kt = part; kt < KT; kt += PARTS) {
+    // the state's shares; part: the wave's key rows, its steps' tiles: first, first + TW, ...
+    constexpr int KN = KT / KW;
+    const int part = w % KW, first = w / KW;
+    float sq[TN] = {}, sp[TN] = {}, sn[TN] = {}, sc[TN] = {}, ss = 0.0f;
+    f32x4 dq[KN][TN] = {}, dp[KN][TN] = {}, dm[KN][TN] = {};
+#pragma unroll
+    for (int kn = 0; kn < KN; ++kn) {
+        const int kt = kn * KW + part, row = kt * 16 + n;
         if (kt * 16 >= d.K) continue;
-        const int row = kt * 16 + n;
-        f32x4 dq = {}, dp = {}, dm = {};
         for (int v = 0; v < vp; v += 32) {
             float x[8], y[8];
             if (S) {
                 row8(S + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC, x);
                 const Frag<NO> sf = split8<NO>(x);
-                dq = mma<ORD>(sf, O.frag(i0, v + 8 * g), dq);
-                dp = mma<ORD>(sf, Z.frag(i0, v + 8 * g), dp);
+#pragma unroll
+                for (int u = 0; u < TN; ++u) {
+                    const int i = (first + u * TW) * 16 + n;
+                    dq[kn][u] = mma<ORD>(sf, O.frag(i, v + 8 * g), dq[kn][u]);
+                    dp[kn][u] = mma<ORD>(sf, Z.frag(i, v + 8 * g), dp[kn][u]);
+                }
             }
             if (dS) {
                 row8(dS + (int64_t)row * d.V, row < d.K, v + 8 * g, d.V, VEC, y);
-                dm = mma<ORD>(split8<NO>(y), X.frag(i0, v + 8 * g), dm);
-            }
-            if (S && dS && tt == 0)
+                const Frag<NO> df = split8<NO>(y);
 #pragma unroll
-                for (int u = 0; u < 8; ++u) ss += x[u] * y[u];
-        }
-        f32x4 dc;
+                for (int u = 0; u < TN; ++u)
+                    dm[kn][u] = mma<ORD>(df, X.frag((first + u * TW) * 16 + n, v + 8 * g), dm[kn][u]);
+                if (S && first == 0)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            dq[e] = a != 0.0f ? dq[e] * oa : 0.0f;
-            dp[e] = a != 0.0f ? dp[e] * ya : 0.0f;
-            dm[e] = c != 0.0f ? dm[e] * c : 0.0f;
-            dc[e] = dm[e];
-        }
-#pragma unroll
-        for (int p = 0; p < RT / 2; ++p) {
-            const Frag<NP> kf = Kr.tr_frag(kt, p, n, g), qf = Qr.tr_frag(kt, p, n, g);
-            dq = mma<ORD>(kf, dtf[p], dq);
-            dp = mma<ORD>(kf, mtf[p], dp);
-            dm = mma<ORD>(qf, dnf[p], dm);
-            dm = mma<ORD>(kf, mnf[p], dm);
-        }
-        const int kd = kt * 16 + 4 * g;
-        if (t < d.T && kd < d.K) {
-            float qv[4], kv[4], dk[4], dqv[4];
-            load4(q + t * d.q_s[1] + kd, d.K - kd, VEC, qv);
-            load4(k + t * d.k_s[1] + kd, d.K - kd, VEC, kv);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sq += dq[e] * qv[e];
-                sp += dp[e] * kv[e];
-                sn += dm[e] * kv[e];
-                sc += dc[e] * kv[e];
-                dk[e] = dp[e] + dm[e];
-                dqv[e] = dq[e];
-            }
-            const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.K + kd;
-            if (d.H == d.Hk) {
-                store4((T*)gr.d_q + at, d.K - kd, VEC, dqv);
-                store4((T*)gr.d_k + at, d.K - kd, VEC, dk);
-            } else {
-                store4(gr.head_grad + at, d.K - kd, VEC, dqv);
-                store4(gr.head_grad + (int64_t)d.B * d.T * d.H * d.K + at, d.K - kd, VEC, dk);
+                    for (int e = 0; e < 8; ++e) ss += x[e] * y[e];
             }
         }
     }
-    auto give = [&](float x, float (&to)[4][C]) {
-        x += __shfl_xor(x, 16);
-        x += __shfl_xor(x, 32);
-        if (g == 0) to[part][i0] = x;
-    };
-    give(sq, sums.q), give(sp, sums.kp), give(sn, sums.km), give(sc, sums.ks);
+    __syncthreads();                                    // X, Z and dO are done with
+    const Inner<T, C> in(place);
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+        const int i = it * 16 + n;
+        const bool m = C == 64 ? pass : w >> 1;
+        const Planes<NO> to{in.D.p + (m ? NO * C * in.D.ld : 0), in.D.ld, in.D.plane};     // (an offset: LDS to the compiler)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const f32x4 x = tri[pass][r];
+            if (r <= it || (r == it + 1 && (r & 1))) to.put4(i, perm(r * 16 + 4 * g), x[0], x[1], x[2], x[3]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kn = 0; kn < KN; ++kn) {
+        const int kt = kn * KW + part;
+        if (kt * 16 >= d.K) continue;
+#pragma unroll
+        for (int u = 0; u < TN; ++u) {
+            const int tt = first + u * TW, i = tt * 16 + n;
+            const float a = gates.a[i], c = gates.c[i], ya = -gates.beta[i] * a, oa = d.scale * a;
+            f32x4 q4 = dq[kn][u], p4 = dp[kn][u], m4 = dm[kn][u], dc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                q4[e] = a != 0.0f ? q4[e] * oa : 0.0f;
+                p4[e] = a != 0.0f ? p4[e] * ya : 0.0f;
+                m4[e] = c != 0.0f ? m4[e] * c : 0.0f;
+                dc[e] = m4[e];
+            }
+#pragma unroll
+            for (int p = 0; p < RT / 2; ++p) {
+                const Frag<NP> kf = Kr.tr_frag(kt, p, n, g);
+                if (2 * p <= tt) {                          // earlier steps
+                    q4 = mma<ORD>(kf, in.D.frag(i, p * 32 + 8 * g), q4);
+                    p4 = mma<ORD>(kf, in.M.frag(i, p * 32 + 8 * g), p4);
+                }
+                if (2 * p + 1 >= tt) {                      // later ones
+                    m4 = mma<ORD>(Qr.tr_frag(kt, p, n, g), in.D.tr_frag(tt, p, n, g), m4);
+                    m4 = mma<ORD>(kf, in.M.tr_frag(tt, p, n, g), m4);
+                }
+            }
+            const int kd = kt * 16 + 4 * g, t = t0 + i;
+            if (t < d.T && kd < d.K) {
+                float qv[4], kv[4], dk[4], dqv[4];
+                load4(q + t * d.q_s[1] + kd, d.K - kd, VEC, qv);
+                load4(k + t * d.k_s[1] + kd, d.K - kd, VEC, kv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sq[u] += q4[e] * qv[e];
+                    sp[u] += p4[e] * kv[e];
+                    sn[u] += m4[e] * kv[e];
+                    sc[u] += dc[e] * kv[e];
+                    dk[e] = p4[e] + m4[e];
+                    dqv[e] = q4[e];
+                }
+                const int64_t at = (((int64_t)b * d.T + t) * d.H + h) * d.K + kd;
+                if (d.H == d.Hk) {
+                    store4((T*)gr.d_q + at, d.K - kd, VEC, dqv);
+                    store4((T*)gr.d_k + at, d.K - kd, VEC, dk);
+                } else {
+                    store4(gr.head_grad + at, d.K - kd, VEC, dqv);
+                    store4(gr.head_grad + (int64_t)d.B * d.T * d.H * d.K + at, d.K - kd, VEC, dk);
+                }
+            }
+        }
+    }
+    static_assert(sizeof(Parts<C>) <= sizeof(__bf16) * Inner<T, C>::SIZE, "the triangles' place");
+    Parts<C>& parts = *(Parts<C>*)place;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < TN; ++u) {
+        const int i0 = (first + u * TW) * 16 + n;
+        auto give = [&](float x, float (&to)[4][C]) {
+            x += __shfl_xor(x, 16);
+            x += __shfl_xor(x, 32);
+            if (g == 0) to[part][i0] = x;
+        };
+        give(sq[u], parts.q), give(sp[u], parts.kp), give(sn[u], parts.km), give(sc[u], parts.ks);
+    }
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
     if (lane == 0) sums.ss[w] = ss;
     __syncthreads();
@@ -360,9 +395,9 @@ DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int
         if (lane < C) {
             seg = gates.seg[lane];
 #pragma unroll
-            for (int m = 0; m < PARTS; ++m) {
-                x += sums.q[m][lane] + sums.kp[m][lane] - sums.km[m][lane];
-                e += sums.ks[m][lane];
+            for (int m = 0; m < KW; ++m) {
+                x += parts.q[m][lane] + parts.kp[m][lane] - parts.km[m][lane];
+                e += parts.ks[m][lane];
             }
         }
         // the state's share, at the last step
@@ -428,18 +463,12 @@ void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
     const int64_t kv = (int64_t)d.K * d.V, at = bh * (chunks - 1) + ch;
     const float* S = ch ? d.chunk_state + (at - 1) * kv : d.state ? d.state + bh * kv : nullptr;
     const float* dS = ch + 1 < chunks ? gr.chunk_grad + at * kv : gr.d_state_out ? gr.d_state_out + bh * kv : nullptr;
-    chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, t0, S, dS, gates, sums, Kr, Qr, X, Z, O, vp);
+    chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, t0, S, dS, gates, sums, Kr, Qr, X, Z, O, rows, vp);
 }
 
-// LDS of the one-chunk kernel: the chunk kernel's, with X where the triangles and 64 columns of dV on their way out were
-// until the errors' gradients were known
-template <typename T, int C> constexpr size_t triangles_lds() {
-    return sizeof(__bf16) * 3 * C * (C + 8) + sizeof(float) * C * (C + 4) + sizeof(T) * C * LV;
-}
-template <typename T, int C, int KP> constexpr size_t window_lds(int vp) {
-    const size_t x = sizeof(__bf16) * (Elem<T>::ord + 1) * C * (vp + 8), t = triangles_lds<T, C>();
-    return chunk_lds<T, C, KP>(vp) + (t > x ? t - x : 0);
-}
+// the one-chunk kernel's triangles P and L, in X's place until that is staged
+template <int C> constexpr size_t triangles_lds() { return sizeof(__bf16) * 3 * C * (C + 8) + sizeof(float) * C * (C + 4); }
+template <typename T, int C, int KP> constexpr size_t window_lds(int vp) { return chunk_lds<T, C, KP>(vp, triangles_lds<C>()); }
 
 // The whole backward pass of a window of at most C steps, one workgroup a robot and head.
 template <typename T, int C, int KP, bool VEC>
@@ -456,9 +485,8 @@ void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
     __bf16* rows = pool + 2 * NP * C * LK;
     const Planes<NO> Z{rows, lv, C * lv}, X{rows + (NO + NP) * C * lv, lv, C * lv};
     const Planes<NP> O{rows + NO * C * lv, lv, C * lv};
-    const Planes<3> P{X.p, LC, C * LC};             // (X's place, until it is staged)
+    const Planes<3> P{X.p, LC, C * LC};             // (X's place and after, until it is staged)
     float* ln = (float*)(P.p + 3 * C * LC);
-    T* out = (T*)(ln + C * LL);
     const int64_t bh = blockIdx.x, row_s = (int64_t)d.H * d.V, kv = (int64_t)d.K * d.V;
     const int b = blockIdx.x / d.H, h = blockIdx.x % d.H, hk = h / (d.H / d.Hk);
     const int64_t row0 = (int64_t)b * d.T * row_s + h * d.V;
@@ -481,31 +509,27 @@ void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
     for (int c0 = 0; c0 < d.V; c0 += 64) {
         const int width = d.V - c0 < 64 ? d.V - c0 : 64;
         const bool mine = w * 16 + n < width;
-        const uint32_t at = (uint32_t)(4 * g * d.V + w * 16 + n);
+        const uint32_t at = 4 * (uint32_t)(4 * g * d.V + w * 16 + n);
         if (c0 + w * 16 < vp) {                     // (columns from V up to vp: zeros)
             f32x4 z[RT] = {}, u[RT], S[KT] = {};
             if (mine && gr.d_state_out) state_load(S, gr.d_state_out + bh * kv + c0, at, d.V, d.K, g);
             column_gradients<C, KP, NP>(S, gr.d_state_out != nullptr, z, u, gates, ln, LL, Kr, P, O, c0 + w * 16, n, g);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                tile_put(out + rt * 16 * LV + w * 16, LV, n, g, z[rt] * *(const f32x4*)(gates.beta + rt * 16 + 4 * g));
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) Z.put1(rt * 16 + 4 * g + e, c0 + w * 16 + n, z[rt][e]);
-            }
             if (gr.d_state) {
                 state_gradient<C, KP, NP>(S, z, u, gates, d.scale, Kr, Qr, n, g);
                 if (mine) state_store(S, gr.d_state + bh * kv + c0, at, d.V, d.K, g);
             }
         }
-        __syncthreads();
-        store_rows<T, C, VEC>(out, (T*)gr.d_v + row0 + c0, row_s, d.T, width);
-        __syncthreads();
     }
-    stage_errors<T, C, VEC, NO>(d, nullptr, (T*)nullptr, row0, row_s, d.T, vp, gates, X, Z, sums);
+    __syncthreads();
+    stage_errors<T, C, VEC, NO>(d, nullptr, (T*)gr.d_v, row0, row_s, d.T, vp, gates, X, Z, sums);
     __syncthreads();
     chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, 0, d.state ? d.state + bh * kv : nullptr,
                                            gr.d_state_out ? gr.d_state_out + bh * kv : nullptr, gates, sums, Kr, Qr, X,
-                                           Z, O, vp);
+                                           Z, O, rows, vp);
 }
 
 // gradients of shared query and key heads: the value heads' own, summed in head order

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_f
     };
     if (chunks) fetch(0);
 
-    uint32_t at = (uint32_t)(4 * g * d.V + w * 16 + n), at_err = (uint32_t)(4 * g * row_s + w * 16 + n);
+    uint32_t at = 4 * (uint32_t)(4 * g * d.V + w * 16 + n), at_err = 4 * (uint32_t)(4 * g * row_s + w * 16 + n);
     f32x4 S[KT] = {};
     if (mine && d.state) state_load(S, d.state + bh * d.K * d.V + c0, at, d.V, d.K, g);
 
@@ -81,14 +81,7 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_f
                 }
             }
             solve_down<C>(x, s.ln, Lds::LL, n, g);
-            if (d.err && mine) {
-                float* err = d.err + rows0 + t0 * row_s;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (t0 + rt * 16 + 4 * g + e < d.T) err[at_err + (uint32_t)((rt * 16 + e) * row_s)] = x[rt][e];
-            }
+            if (d.err && mine) rows_store(x, d.err + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
 #pragma unroll

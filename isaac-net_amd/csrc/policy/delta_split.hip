@@ -109,21 +109,15 @@ __global__ __launch_bounds__(DELTA_WG, 2) void delta_before_kernel(InetDelta d, 
                 for (int kt = 0; kt < KT; ++kt) G[kt] = mma<2>(Qr.tr_frag(kt, kp, n, g), of, G[kt]);
             }
             if (w * 16 + n < width)
-                state_store(G, work.G + unit * d.K * d.V + c0, (uint32_t)(4 * g * d.V + w * 16 + n), d.V, d.K, g);
+                state_store(G, work.G + unit * d.K * d.V + c0, 4 * (uint32_t)(4 * g * d.V + w * 16 + n), d.V, d.K, g);
         } else {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) x[rt] = plane_tile(R, rt * 16, w * 16, n, g);
         }
         solve(x);
         if (w * 16 + n < width) {
-            float* to = U + ((int64_t)b * d.T + t0) * row_s + h * d.V + c0 + w * 16 + n;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = rt * 16 + 4 * g + e;
-                    if (t0 + i < d.T) to[i * row_s] = x[rt][e];
-                }
+            rows_store(x, U + ((int64_t)b * d.T + t0) * row_s + h * d.V + c0, 4 * (uint32_t)(4 * g * row_s + w * 16 + n), row_s,
+                       d.T - t0, g);
         }
     }
     if (blockIdx.y) return;
@@ -178,15 +172,15 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int c0 = blockIdx.y * 64, width = d.V - c0 < 64 ? d.V - c0 : 64;
     const bool mine = w * 16 + n < width;
-    const uint32_t at = (uint32_t)(4 * g * d.V + w * 16 + n);
+    uint32_t at = 4 * (uint32_t)(4 * g * d.V + w * 16 + n), at_row = 4 * (uint32_t)(4 * g * row_s + w * 16 + n);
     const T* k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2];
-    float* rows = U + b * (int64_t)d.T * row_s + h * d.V + c0 + w * 16 + n;
+    float* rows = U + b * (int64_t)d.T * row_s + h * d.V + c0;
     const int64_t kv = (int64_t)d.K * d.V;
 
     Rows<T, C, KP, VEC> kr;
     bf16x8 wr[NW];
     float fr = 0.0f;
-    f32x4 un[RT], gn[KT];
+    f32x4 un[RT] = {}, gn[KT] = {};
     auto fetch = [&](int ch) {
         const int64_t unit = bh * chunks + ch;
 #pragma unroll
@@ -199,16 +193,8 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
         if (threadIdx.x < 2 * C + 4) fr = work.f[unit * (2 * C + 4) + threadIdx.x];
     };
     auto fetch_own = [&](int ch) {                  // the wave's own columns
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = ch * C + rt * 16 + 4 * g + e;
-                un[rt][e] = mine && t < d.T ? rows[t * row_s] : 0.0f;
-            }
+        if (mine) rows_load(un, rows + ch * C * row_s, at_row, row_s, d.T - ch * C, g);
         if (BACK) {
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt) gn[kt] = f32x4{};
             if (mine) state_load(gn, work.G + (bh * chunks + ch) * kv + c0, at, d.V, d.K, g);
         }
     };
@@ -231,6 +217,7 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
     for (int i = 0; i < chunks; ++i) {
         const int ch = chunk_at(i);
         const Buf& s = buf[i & 1];
+        keep(at), keep(at_row);
         f32x4 x[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) x[rt] = un[rt];
@@ -262,10 +249,9 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[rt][e] += m[e] != 0.0f ? y[rt][e] : 0.0f;
-                    const int t = ch * C + rt * 16 + 4 * g + e;
-                    if (mine && t < d.T) rows[t * row_s] = x[rt][e];
                 }
             }
+            if (mine) rows_store(x, rows + ch * C * row_s, at_row, row_s, d.T - ch * C, g);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -312,16 +298,10 @@ __global__ __launch_bounds__(DELTA_WG, 2) void delta_after_kernel(InetDelta d) {
     Gate gate;
     kr.load((const T*)d.k + b * d.k_s[0] + hk * d.k_s[2], d.k_s[1], t0, d.T, d.K);
     qr.load((const T*)d.q + b * d.q_s[0] + hk * d.q_s[2], d.q_s[1], t0, d.T, d.K);
-    f32x4 S[KT] = {}, x[RT];
+    f32x4 S[KT] = {}, x[RT] = {};
     const float* from = ch ? d.chunk_state + (bh * (chunks - 1) + ch - 1) * kv : d.state ? d.state + bh * kv : nullptr;
-    if (mine && from) state_load(S, from + c0, (uint32_t)(4 * g * d.V + w * 16 + n), d.V, d.K, g);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = rt * 16 + 4 * g + e;
-            x[rt][e] = mine && t0 + i < d.T ? d.err[row0 + i * row_s + w * 16 + n] : 0.0f;
-        }
+    if (mine && from) state_load(S, from + c0, 4 * (uint32_t)(4 * g * d.V + w * 16 + n), d.V, d.K, g);
+    if (mine) rows_load(x, d.err + row0, 4 * (uint32_t)(4 * g * row_s + w * 16 + n), row_s, d.T - t0, g);
     if (w == 0) {
         gate.load<C>(d, b, h, t0);
         put_gates<C>(s.gates, gate);
