@@ -68,19 +68,40 @@ template <typename T> DEV void load4(const T* __restrict__ p, int n, bool vec, f
 
 template <int N> struct Frag { bf16x8 p[N]; };
 
-template <int N> DEV Frag<N> split8(const float (&x)[8]) {
-    Frag<N> f;
-    float r[8];
+// two values to bfloat16 in one instruction, and what they leave over
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+DEV uint32_t round2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+DEV float low_of(uint32_t u) { return __builtin_bit_cast(float, u << 16); }
+DEV float high_of(uint32_t u) { return __builtin_bit_cast(float, u & 0xffff0000u); }
+
+// values to planes, two at a time: plane i of values 2 j, 2 j + 1 in out[i][j]
+template <int N, int PAIRS> DEV void split_pairs(const float (&x)[2 * PAIRS], uint32_t (&out)[N][PAIRS]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = x[e];
+    for (int j = 0; j < PAIRS; ++j) {
+        float a = x[2 * j], b = x[2 * j + 1];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const __bf16 h = (__bf16)r[e];
-            f.p[i][e] = h;
-            if (i + 1 < N) r[e] -= (float)h;
+        for (int i = 0; i < N; ++i) {
+            const uint32_t h = round2(a, b);
+            out[i][j] = h;
+            if (i + 1 < N) {
+                a -= low_of(h);
+                b -= high_of(h);
+            }
         }
+    }
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <int N> DEV Frag<N> split8(const float (&x)[8]) {
+    uint32_t u[N][4];
+    split_pairs<N, 4>(x, u);
+    Frag<N> f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) f.p[i] = __builtin_bit_cast(bf16x8, (u32x4{u[i][0], u[i][1], u[i][2], u[i][3]}));
     return f;
 }
 
@@ -162,14 +183,11 @@ template <int N> struct Planes {
         }
     }
     DEV void put4(int row, int place, float a, float b, float c, float d) const {
-        float x[4] = {a, b, c, d};
+        const float x[4] = {a, b, c, d};
+        uint32_t u[N][2];
+        split_pairs<N, 2>(x, u);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            bf16x4 h;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { h[e] = (__bf16)x[e]; x[e] -= (float)h[e]; }
-            *(bf16x4*)(p + i * plane + row * ld + place) = h;
-        }
+        for (int i = 0; i < N; ++i) *(u32x2*)(p + i * plane + row * ld + place) = u32x2{u[i][0], u[i][1]};
     }
 };
 
