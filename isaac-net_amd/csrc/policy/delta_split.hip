@@ -219,12 +219,20 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
         const Buf& s = buf[i & 1];
         keep(at), keep(at_row);
         f32x4 x[RT];
+        // (what was fetched for this chunk is waited for here, not with what is fetched next)
+        auto arrived = [](f32x4& v) { asm volatile("" : "+v"(v)); };
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) x[rt] = un[rt];
+        for (int rt = 0; rt < RT; ++rt) {
+            x[rt] = un[rt];
+            arrived(x[rt]);
+        }
         f32x4 G[KT];
         if (BACK)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) G[kt] = gn[kt];
+            for (int kt = 0; kt < KT; ++kt) {
+                G[kt] = gn[kt];
+                arrived(G[kt]);
+            }
         if (i + 1 < chunks) {
             fetch(chunk_at(i + 1));
             fetch_own(chunk_at(i + 1));
@@ -239,8 +247,10 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
 #pragma unroll
             for (int kp = 0; kp < KT / 2; ++kp) {
                 const Frag<3> sf = split_tiles<3>(S[2 * kp], S[2 * kp + 1]);
+                Frag<3> wf[RT];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) y[rt] = mma<2>(W.frag(rt * 16 + n, kp * 32 + 8 * g), sf, y[rt]);
+                for (int rt = 0; rt < RT; ++rt) wf[rt] = W.frag(rt * 16 + n, kp * 32 + 8 * g);
+                mma_rows<2>(wf, sf, y);
             }
             const float a_end = s.f[2 * C];
 #pragma unroll
@@ -261,8 +271,10 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
             for (int kp = 0; kp < RT / 2; ++kp) {
                 const f32x4 f0 = *(const f32x4*)(s.f + kp * 32 + 4 * g), f1 = *(const f32x4*)(s.f + kp * 32 + 16 + 4 * g);
                 const Frag<3> xf = split_tiles<3>(x[2 * kp] * f0, x[2 * kp + 1] * f1);
+                Frag<NP> kf[KT];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), xf, S[kt]);
+                for (int kt = 0; kt < KT; ++kt) kf[kt] = Kr.tr_frag(kt, kp, n, g);
+                mma_rows<2>(kf, xf, S);
             }
         }
         if (i + 1 < chunks) put(buf[(i + 1) & 1]);

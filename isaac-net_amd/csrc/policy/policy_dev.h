@@ -121,6 +121,18 @@ template <int ORD, int NA, int NB> DEV f32x4 mma(const Frag<NA>& a, const Frag<N
     return c;
 }
 
+// the same for several A against one B, plane product by plane product, so that no instruction waits for the one before it
+template <int ORD, int NA, int NB, int R> DEV void mma_rows(const Frag<NA> (&a)[R], const Frag<NB>& b, f32x4 (&c)[R]) {
+#pragma unroll
+    for (int s = ORD; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (s - i >= 0 && s - i < NB)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    c[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[r].p[i], b.p[s - i], c[r], 0, 0, 0);
+}
+
 // c + A B over a 16-long contraction in 32 bits: a = A's row n at columns 4 g .. 4 g + 3, b a 16 x 16 result
 DEV f32x4 mma32(f32x4 a, f32x4 b, f32x4 c) {
 #pragma unroll
