@@ -111,10 +111,11 @@ template <typename T, int C, int KP, bool VEC> struct Rows {
     static constexpr int GR = C * (KP / 8), NL = (GR + DELTA_WG - 1) / DELTA_WG;
     typedef T V8 __attribute__((ext_vector_type(8)));
     V8 v[NL];
+    int tid = threadIdx.x;                               // (of the DELTA_WG that load together)
     DEV void load(const T* __restrict__ x, int64_t st, int t0, int t_end, int K) {
 #pragma unroll
         for (int m = 0; m < NL; ++m) {
-            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            const int i = tid + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
             v[m] = V8{};
             if (i < GR && t0 + r < t_end && c < K) {
                 const T* p = x + (t0 + r) * st + c;
@@ -129,14 +130,14 @@ template <typename T, int C, int KP, bool VEC> struct Rows {
     DEV void put(T* s, int ld) const {                            // as they are
 #pragma unroll
         for (int m = 0; m < NL; ++m) {
-            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            const int i = tid + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
             if (GR % DELTA_WG == 0 || i < GR) *(V8*)(s + r * ld + c) = v[m];
         }
     }
     template <int N> DEV void put_natural(const Planes<N>& s) const {       // columns in their own order
 #pragma unroll
         for (int m = 0; m < NL; ++m) {
-            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            const int i = tid + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
             if (GR % DELTA_WG == 0 || i < GR) {
                 s.put4(r, c, (float)v[m][0], (float)v[m][1], (float)v[m][2], (float)v[m][3]);
                 s.put4(r, c + 4, (float)v[m][4], (float)v[m][5], (float)v[m][6], (float)v[m][7]);
@@ -146,7 +147,7 @@ template <typename T, int C, int KP, bool VEC> struct Rows {
     template <int N> DEV void put(const Planes<N>& s) const {
 #pragma unroll
         for (int m = 0; m < NL; ++m) {
-            const int i = threadIdx.x + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
+            const int i = tid + m * DELTA_WG, r = i / (KP / 8), c = i % (KP / 8) * 8;
             if (GR % DELTA_WG == 0 || i < GR) {
                 s.put4(r, perm(c), (float)v[m][0], (float)v[m][1], (float)v[m][2], (float)v[m][3]);
                 s.put4(r, perm(c + 4), (float)v[m][4], (float)v[m][5], (float)v[m][6], (float)v[m][7]);

@@ -156,9 +156,11 @@ template <typename T, int C, int KP> struct ScanBuf {
     alignas(16) float f[2 * C + 4];
 };
 
-// One workgroup a robot, head and 64 columns; wave w owns 16 columns of the state. X overwrites U.
+// One workgroup of eight waves a robot, head and 64 columns: waves 0 .. 3 own 16 columns of the state each, waves 4 .. 7 bring
+// the next chunk's operands to LDS (the one wave a SIMD that computes is a single chain; what it need not do shortens it).
+// X overwrites U.
 template <typename T, int C, int KP, bool BACK, bool VEC>
-__global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, const float* __restrict__ first,
+__global__ __launch_bounds__(2 * DELTA_WG, 2) void delta_serial_kernel(InetDelta d, const float* __restrict__ first,
                                                                    float* __restrict__ last, float* __restrict__ between,
                                                                    float* __restrict__ U, SplitWork work) {
     constexpr int NP = Elem<T>::planes, RT = C / 16, KT = KP / 16, LK = KP + 8, WG8 = 3 * C * (KP / 8),
@@ -177,41 +179,53 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
     float* rows = U + b * (int64_t)d.T * row_s + h * d.V + c0;
     const int64_t kv = (int64_t)d.K * d.V;
 
+    auto chunk_at = [&](int i) { return BACK ? chunks - 1 - i : i; };
+    const int tid = threadIdx.x & (DELTA_WG - 1);
     Rows<T, C, KP, VEC> kr;
+    kr.tid = tid;
     bf16x8 wr[NW];
     float fr = 0.0f;
-    f32x4 un[RT] = {}, gn[KT] = {};
     auto fetch = [&](int ch) {
         const int64_t unit = bh * chunks + ch;
 #pragma unroll
         for (int m = 0; m < NW; ++m) {
-            const int i = threadIdx.x + m * DELTA_WG;
+            const int i = tid + m * DELTA_WG;
             if (WG8 % DELTA_WG == 0 || i < WG8)
                 wr[m] = *(const bf16x8*)(work.w + (unit * 3 * C + i / (KP / 8)) * KP + i % (KP / 8) * 8);
         }
         kr.load(k, d.k_s[1], ch * C, d.T, d.K);
-        if (threadIdx.x < 2 * C + 4) fr = work.f[unit * (2 * C + 4) + threadIdx.x];
+        if (tid < 2 * C + 4) fr = work.f[unit * (2 * C + 4) + tid];
     };
+    auto put = [&](Buf& s) {
+#pragma unroll
+        for (int m = 0; m < NW; ++m) {
+            const int i = tid + m * DELTA_WG;
+            if (WG8 % DELTA_WG == 0 || i < WG8) *(bf16x8*)(s.w + i / (KP / 8) * LK + i % (KP / 8) * 8) = wr[m];
+        }
+        kr.put(Planes<NP>{s.k, LK, C * LK});
+        if (tid < 2 * C + 4) s.f[tid] = fr;
+    };
+    if (w >= 4) {
+        fetch(chunk_at(0));
+        put(buf[0]);
+        if (chunks > 1) fetch(chunk_at(1));
+        __syncthreads();
+        for (int i = 0; i < chunks; ++i) {
+            if (i + 1 < chunks) put(buf[(i + 1) & 1]);
+            if (i + 2 < chunks) fetch(chunk_at(i + 2));
+            __syncthreads();
+        }
+        return;
+    }
+    f32x4 un[RT] = {}, gn[KT] = {};
     auto fetch_own = [&](int ch) {                  // the wave's own columns
         if (mine) rows_load(un, rows + ch * C * row_s, at_row, row_s, d.T - ch * C, g);
         if (BACK) {
             if (mine) state_load(gn, work.G + (bh * chunks + ch) * kv + c0, at, d.V, d.K, g);
         }
     };
-    auto put = [&](Buf& s) {
-#pragma unroll
-        for (int m = 0; m < NW; ++m) {
-            const int i = threadIdx.x + m * DELTA_WG;
-            if (WG8 % DELTA_WG == 0 || i < WG8) *(bf16x8*)(s.w + i / (KP / 8) * LK + i % (KP / 8) * 8) = wr[m];
-        }
-        kr.put(Planes<NP>{s.k, LK, C * LK});
-        if (threadIdx.x < 2 * C + 4) s.f[threadIdx.x] = fr;
-    };
     f32x4 S[KT] = {};
     if (mine && first) state_load(S, first + bh * kv + c0, at, d.V, d.K, g);
-    auto chunk_at = [&](int i) { return BACK ? chunks - 1 - i : i; };
-    fetch(chunk_at(0));
-    put(buf[0]);
     fetch_own(chunk_at(0));
     __syncthreads();
     for (int i = 0; i < chunks; ++i) {
@@ -233,10 +247,7 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
                 G[kt] = gn[kt];
                 arrived(G[kt]);
             }
-        if (i + 1 < chunks) {
-            fetch(chunk_at(i + 1));
-            fetch_own(chunk_at(i + 1));
-        }
+        if (i + 1 < chunks) fetch_own(chunk_at(i + 1));
         if (w * 16 < width) {
             const Planes<3> W{(__bf16*)s.w, LK, C * LK};
             const Planes<NP> Kr{(__bf16*)s.k, LK, C * LK};
@@ -277,7 +288,6 @@ __global__ __launch_bounds__(DELTA_WG, 1) void delta_serial_kernel(InetDelta d, 
                 mma_rows<2>(kf, xf, S);
             }
         }
-        if (i + 1 < chunks) put(buf[(i + 1) & 1]);
         __syncthreads();
     }
     if (mine && last) state_store(S, last + bh * kv + c0, at, d.V, d.K, g);
@@ -368,7 +378,7 @@ static int launch(const InetDelta& d, const InetDeltaGrad* g, hipStream_t st) {
     hipLaunchKernelGGL(before, dim3(d.B * d.H * chunks, cols), dim3(DELTA_WG), bl, st, d, rhs, rs[0], rs[1], rs[2], U,
                        work);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
-    hipLaunchKernelGGL(serial, dim3(d.B * d.H, cols), dim3(DELTA_WG), sl, st, d, BACK ? g->d_state_out : d.state,
+    hipLaunchKernelGGL(serial, dim3(d.B * d.H, cols), dim3(2 * DELTA_WG), sl, st, d, BACK ? g->d_state_out : d.state,
                        BACK ? g->d_state : d.state_out, BACK ? g->chunk_grad : d.chunk_state, U, work);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     if (!BACK) {
