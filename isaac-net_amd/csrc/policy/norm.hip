@@ -6,8 +6,8 @@
 //     dz = dn w_pre,  dy' = dy + (dz - z mean(dz z)) / rms(y),  dx = dy',  dgate = dy' s h,  ds += dy' gate h
 //     df^ = dy' gate s w_post,  dw_post += dy' gate s f^,  df = (df^ - f^ mean(df^ f^)) / rms(f),  dw_pre += dn z
 // Memory bounds it: each row is read once into registers (the backward pass computes y again from x and f rather than
-// read it, so y stays unrounded) and every sum over a row goes across its lanes in 32 bits. LP lanes take a row,
-// NJ groups of 8 values each; with rows that do not start on 16 bytes a lane takes single values LP apart instead.
+// read it, so y stays unrounded) and every sum over a row goes across its lanes in 32 bits. LP lanes take a row, NJ groups
+// of 8 values each, 16 bytes at a time wherever rows start.
 // The sums over rows for the weights stay in each workgroup's registers through all its rows, then go to the workspace
 // as one partial row a workgroup; a second kernel adds those in a fixed order, so results do not vary from run to run.
 #include "policy_dev.h"
@@ -23,7 +23,7 @@ constexpr int NORM_BLOCKS = 1024;            // workgroups of the backward pass,
 template <int CTRL> DEV float lane_turn(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-template <int LP> DEV float row_sum(float x, float* s) {
+template <int LP> DEV float lane_sum(float x) {
     x += lane_turn<0x128>(x);
     x += lane_turn<0x124>(x);
     x += lane_turn<0x122>(x);
@@ -40,59 +40,73 @@ template <int LP> DEV float row_sum(float x, float* s) {
         const unsigned low = v[0], high = v[1];
         x = __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
     }
-    if constexpr (LP == 256) {
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
-        __syncthreads();
-        x = (s[0] + s[1]) + (s[2] + s[3]);
-    }
     return x;
 }
+// two sums at once; over a workgroup's four waves through one of two places in LDS in turn, so that one barrier a call
+// is enough (a place is written again only after the other's barrier, by when all have read it)
+template <int LP> struct RowSums {
+    float (*s)[8];
+    int turn = 0;
+    DEV void sum(float& a, float& b) {
+        a = lane_sum<LP>(a);
+        b = lane_sum<LP>(b);
+        if constexpr (LP == 256) {
+            float* t = s[turn];
+            turn ^= 1;
+            const int w = threadIdx.x >> 6;
+            if ((threadIdx.x & 63) == 0) {
+                t[w] = a;
+                t[4 + w] = b;
+            }
+            __syncthreads();
+            a = (t[0] + t[1]) + (t[2] + t[3]);
+            b = (t[4] + t[5]) + (t[6] + t[7]);
+        }
+    }
+    DEV float sum(float a) {
+        float b = 0.0f;
+        sum(a, b);
+        return a;
+    }
+};
 
-// a row on its way from memory: the lane's NJ groups of eight, in sequence, or eight values LP apart
+// eight values wherever they start (WHOLE: on 16 bytes): one 16-byte access (two for float32) either way
+template <typename T, bool WHOLE> struct Eight {
+    typedef T Value __attribute__((ext_vector_type(8)));
+    typedef T Place __attribute__((ext_vector_type(8), aligned(WHOLE ? 16 : sizeof(T))));
+};
+
+// a row on its way from memory: the lane's NJ groups of eight, LP groups apart. VEC: rows start on 16 bytes and hold whole
+// groups; else a row's last group may be a part.
 template <typename T, int LP, int NJ, bool VEC> struct Row {
-    typedef T V8 __attribute__((ext_vector_type(8)));
+    typedef typename Eight<T, VEC>::Value V8;
     V8 v[NJ];
     DEV void load(const T* __restrict__ p, int c, int D) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
+            const int at = (j * LP + c) * 8;
             v[j] = V8{};
-            if constexpr (VEC) {
-                const int at = (j * LP + c) * 8;
-                if (at < D) v[j] = *(const V8*)(p + at);
-            } else {
+            if (VEC ? at < D : at + 8 <= D) v[j] = *(const typename Eight<T, VEC>::Place*)(p + at);
+            else if (!VEC && at < D)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int at = (j * 8 + e) * LP + c;
-                    if (at < D) v[j][e] = p[at];
-                }
-            }
+                for (int e = 0; e < 7; ++e)
+                    if (at + e < D) v[j][e] = p[at + e];
         }
     }
     DEV float at(int j, int e) const { return (float)v[j][e]; }
 };
 
 template <typename T, int LP, bool VEC> DEV void row_store(T* __restrict__ p, int c, int j, int D, const float (&x)[8]) {
-    if constexpr (VEC) {
-        const int at = (j * LP + c) * 8;
-        if (at < D) {
-            if constexpr (sizeof(T) == 4) {
-                *(f32x4*)(p + at) = f32x4{x[0], x[1], x[2], x[3]};
-                *(f32x4*)(p + at + 4) = f32x4{x[4], x[5], x[6], x[7]};
-            } else {
-                typedef T V8 __attribute__((ext_vector_type(8)));
-                V8 v;
+    const int at = (j * LP + c) * 8;
+    if (VEC ? at < D : at + 8 <= D) {
+        typename Eight<T, VEC>::Value v;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = (T)x[e];
-                *(V8*)(p + at) = v;
-            }
-        }
-    } else {
+        for (int e = 0; e < 8; ++e) v[e] = (T)x[e];
+        *(typename Eight<T, VEC>::Place*)(p + at) = v;
+    } else if (!VEC && at < D) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int at = (j * 8 + e) * LP + c;
-            if (at < D) p[at] = (T)x[e];
-        }
+        for (int e = 0; e < 7; ++e)
+            if (at + e < D) p[at + e] = (T)x[e];
     }
 }
 
@@ -113,7 +127,8 @@ template <int LP, int NJ, bool VEC> struct Weights {
 template <typename T, int LP, int NJ, bool VEC>
 __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
     constexpr int RW = NORM_WG / LP;
-    __shared__ float s_sum[4];
+    __shared__ float s_sum[2][8];
+    RowSums<LP> sums{s_sum};
     const int c = threadIdx.x % LP;
     const int64_t row = (int64_t)blockIdx.x * RW + threadIdx.x / LP;
     const bool live = row < a.N;
@@ -136,7 +151,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sf += f.at(j, e) * f.at(j, e);
-            rf = rsqrtf(row_sum<LP>(sf, s_sum) * inv + a.eps);
+            rf = rsqrtf(sums.sum(sf) * inv + a.eps);
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -159,7 +174,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sy += y[j][e] * y[j][e];
-        const float ry = rsqrtf(row_sum<LP>(sy, s_sum) * inv + a.eps);
+        const float ry = rsqrtf(sums.sum(sy) * inv + a.eps);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -172,7 +187,8 @@ __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
 template <typename T, int LP, int NJ, bool VEC>
 __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, InetNormGrad d) {
     constexpr int RW = NORM_WG / LP;
-    __shared__ float s_sum[4];
+    __shared__ float s_sum[2][8];
+    RowSums<LP> sums{s_sum};
     __shared__ float s_w[RW > 1 ? RW * LP * 8 : 1];
     const int c = threadIdx.x % LP, sub = threadIdx.x / LP;
     const float inv = 1.0f / (float)a.D;
@@ -216,7 +232,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
         if (a.f) {
             w.load(a.post_weight, c, a.D);
             s.load(a.scale, c, a.D);
-            if (a.post_weight) rf = rsqrtf(row_sum<LP>(sf, s_sum) * inv + a.eps);
+            if (a.post_weight) rf = rsqrtf(sums.sum(sf) * inv + a.eps);
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -235,8 +251,9 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
                     sy += y[j][e] * y[j][e];
                     sz += z[j][e] * wp.at(j, e) * y[j][e];
                 }
-            const float ry = rsqrtf(row_sum<LP>(sy, s_sum) * inv + a.eps);
-            sz = row_sum<LP>(sz, s_sum) * inv * ry;
+            sums.sum(sy, sz);
+            const float ry = rsqrtf(sy * inv + a.eps);
+            sz *= inv * ry;
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -265,11 +282,9 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
                 }
                 if (a.gate_kind == 2) row_store<T, LP, VEC>((T*)d.d_gate + row * (int64_t)a.D, c, j, D, dg);
             }
-            if (a.gate_kind == 1) {
-                sg = row_sum<LP>(sg, s_sum);
-                if (live && c == 0) ((T*)d.d_gate)[row] = (T)sg;
-            }
-            sd = a.post_weight ? row_sum<LP>(sd, s_sum) * inv : 0.0f;
+            sums.sum(sg, sd);
+            if (a.gate_kind == 1 && live && c == 0) ((T*)d.d_gate)[row] = (T)sg;
+            sd = a.post_weight ? sd * inv : 0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -296,7 +311,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
             if (sub == 0)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int at = VEC ? (j * LP + c) * 8 + e : (j * 8 + e) * LP + c;
+                    const int at = (j * LP + c) * 8 + e;
                     if (at < a.D) out[m * a.D + at] = x[j][e];
                 }
         }

@@ -52,6 +52,11 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
+def _like(x):
+    """A contiguous tensor for x's gradient."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _ptr(x):
     return None if x is None else x.data_ptr()
 
@@ -169,21 +174,18 @@ class _DeltaRule(torch.autograd.Function):
             return (None,) * 8
         lib = _lib.load_policy()
         B, T, H, V = v.shape
-        Hk, K = q.shape[-2:]
-        dev = q.device
+        K, dev = q.shape[-1], q.device
         a = _delta_args(q, k, v, g, beta, reset, ctx.scale, 2)
         a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
         a.state, a.chunk_state, a.err = _ptr(state), _ptr(chunk_state), err.data_ptr()
         work = _delta_work(lib, a, dev, 1)  # noqa: F841  (held until the call is enqueued)
         d_o = None if d_o is None else d_o.contiguous()
         d_out = None if d_out is None else d_out.contiguous()
-        dq, dk = (torch.empty((B, T, Hk, K), dtype=q.dtype, device=dev) for _ in range(2))
-        dv = torch.empty((B, T, H, V), dtype=q.dtype, device=dev)
-        dg, db = (torch.empty((B, T, H), dtype=g.dtype, device=dev) for _ in range(2))
+        dq, dk, dv, dg, db = map(_like, (q, k, v, g, beta))
         ds = torch.empty((B, H, K, V), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
         chunk_grad, err_grad = (None, None) if chunk_state is None else (torch.empty_like(chunk_state),
                                                                          torch.empty_like(err))
-        heads = torch.empty((2, B, T, H, K), dtype=torch.float32, device=dev) if H != Hk else None
+        heads = torch.empty((2, B, T, H, K), dtype=torch.float32, device=dev) if H != q.shape[-2] else None
         d = _lib.InetDeltaGrad(_ptr(d_o), _ptr(d_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
                                db.data_ptr(), _ptr(ds), _ptr(chunk_grad), _ptr(err_grad), _ptr(heads))
         _call(lib.inet_policy_delta_backward, dev.index, "delta_rule backward", C.byref(a), C.byref(d))
@@ -281,8 +283,7 @@ class _GatedFfn(torch.autograd.Function):
         lib, dev = _lib.load_policy(), x.device
         d_y = _rows(d_y)
         a = _ffn_args(x, w_gate, w_up, ctx.act)
-        dx, dg, du = (torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
-                      for t, need in zip((x, w_gate, w_up), ctx.needs_input_grad))
+        dx, dg, du = (_like(t) if need else None for t, need in zip((x, w_gate, w_up), ctx.needs_input_grad))
         d = _lib.InetFfnGrad(d_y.data_ptr(), _row_stride(d_y), _ptr(dx), _ptr(dg), _ptr(du))
         work = _ffn_work(lib, a, dev, 1)  # noqa: F841
         _call(lib.inet_policy_ffn_backward, dev.index, "gated_ffn backward", C.byref(a), C.byref(d))
@@ -355,8 +356,7 @@ class _BlockNorm(torch.autograd.Function):
         lib, dev = _lib.load_policy(), x.device
         a = _norm_args(x, f, gate, scale, post, pre, ctx.eps)
         d_y, d_n = None if d_y is None else d_y.contiguous(), None if d_n is None else d_n.contiguous()
-        dx, df, dgate, dscale, dpost, dpre = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
-                                              for t in (x, f, gate, scale, post, pre))
+        dx, df, dgate, dscale, dpost, dpre = (None if t is None else _like(t) for t in (x, f, gate, scale, post, pre))
         work = torch.empty(lib.inet_policy_norm_work(a.N, a.D), dtype=torch.uint8, device=dev)
         d = _lib.InetNormGrad(_ptr(d_y), _ptr(d_n), dx.data_ptr(), _ptr(df), _ptr(dgate), _ptr(dscale), _ptr(dpost),
                               _ptr(dpre), work.data_ptr())
