@@ -76,37 +76,54 @@ template <typename T, bool WHOLE> struct Eight {
     typedef T Place __attribute__((ext_vector_type(8), aligned(WHOLE ? 16 : sizeof(T))));
 };
 
-// a row on its way from memory: the lane's NJ groups of eight, LP groups apart. VEC: rows start on 16 bytes and hold whole
-// groups; else a row's last group may be a part.
+// Group j of a lane: values `base` .. base + 7 of the row, those from `skip` on its own. VEC: rows start on 16 bytes and hold
+// whole groups; else the last group of a row ends with the row and shares its first values with the group before, so that it
+// is one access too (a row of fewer than eight values is read one by one).
+template <int LP, bool VEC> struct Group {
+    int base, skip;
+    bool in;
+    DEV Group(int c, int j, int D) {
+        const int at = (j * LP + c) * 8;
+        in = at < D;
+        base = VEC || at + 8 <= D || D < 8 ? at : D - 8;
+        skip = VEC ? 0 : at - base;
+    }
+};
+
+// a row on its way from memory: the lane's NJ groups of eight, LP groups apart
 template <typename T, int LP, int NJ, bool VEC> struct Row {
     typedef typename Eight<T, VEC>::Value V8;
     V8 v[NJ];
     DEV void load(const T* __restrict__ p, int c, int D) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int at = (j * LP + c) * 8;
+            const Group<LP, VEC> q(c, j, D);
             v[j] = V8{};
-            if (VEC ? at < D : at + 8 <= D) v[j] = *(const typename Eight<T, VEC>::Place*)(p + at);
-            else if (!VEC && at < D)
+            if (VEC || D >= 8) {
+                if (q.in) v[j] = *(const typename Eight<T, VEC>::Place*)(p + q.base);
+            } else if (q.in) {
 #pragma unroll
                 for (int e = 0; e < 7; ++e)
-                    if (at + e < D) v[j][e] = p[at + e];
+                    if (e < D) v[j][e] = p[e];
+            }
         }
     }
     DEV float at(int j, int e) const { return (float)v[j][e]; }
+    DEV float own(const Group<LP, VEC>& q, int j, int e) const { return VEC || e >= q.skip ? (float)v[j][e] : 0.0f; }
 };
 
 template <typename T, int LP, bool VEC> DEV void row_store(T* __restrict__ p, int c, int j, int D, const float (&x)[8]) {
-    const int at = (j * LP + c) * 8;
-    if (VEC ? at < D : at + 8 <= D) {
+    const Group<LP, VEC> q(c, j, D);
+    if (!q.in) return;
+    if (VEC || (q.skip == 0 && D >= 8)) {
         typename Eight<T, VEC>::Value v;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (T)x[e];
-        *(typename Eight<T, VEC>::Place*)(p + at) = v;
-    } else if (!VEC && at < D) {
+        *(typename Eight<T, VEC>::Place*)(p + q.base) = v;
+    } else {
 #pragma unroll
-        for (int e = 0; e < 7; ++e)
-            if (at + e < D) p[at + e] = (T)x[e];
+        for (int e = 0; e < 8; ++e)
+            if (e >= q.skip && q.base + e < D) p[q.base + e] = (T)x[e];
     }
 }
 
@@ -150,21 +167,24 @@ __global__ __launch_bounds__(NORM_WG) void norm_forward_kernel(InetNorm a) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sf += f.at(j, e) * f.at(j, e);
+                for (int e = 0; e < 8; ++e) {
+                    const float v = f.own(Group<LP, VEC>(c, j, D), j, e);
+                    sf += v * v;
+                }
             rf = rsqrtf(sums.sum(sf) * inv + a.eps);
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                y[j][e] = x.at(j, e) + f.at(j, e) * rf * w.at(j, e) * s.at(j, e) * (a.gate_kind == 2 ? gt.at(j, e) : row_gate);
+                y[j][e] = x.own(Group<LP, VEC>(c, j, D), j, e) + f.own(Group<LP, VEC>(c, j, D), j, e) * rf * w.at(j, e) * s.at(j, e) * (a.gate_kind == 2 ? gt.at(j, e) : row_gate);
             row_store<T, LP, VEC>((T*)a.y + row * (int64_t)a.D, c, j, D, y[j]);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[j][e] = x.at(j, e);
+            for (int e = 0; e < 8; ++e) y[j][e] = x.own(Group<LP, VEC>(c, j, D), j, e);
     }
     if (a.pre_weight) {
         Weights<LP, NJ, VEC> w;
@@ -219,11 +239,12 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                y[j][e] = x.at(j, e);
-                dv[j][e] = dy.at(j, e);
-                h[j][e] = a.f ? f.at(j, e) : 0.0f;
+                const Group<LP, VEC> q(c, j, a.D);
+                y[j][e] = x.own(q, j, e);
+                dv[j][e] = dy.own(q, j, e);
+                h[j][e] = a.f ? f.own(q, j, e) : 0.0f;
                 g[j][e] = a.gate_kind == 2 ? gt.at(j, e) : row_gate;
-                z[j][e] = pre ? dn.at(j, e) : 0.0f;
+                z[j][e] = pre ? dn.own(q, j, e) : 0.0f;
                 sf += h[j][e] * h[j][e];
             }
         if (it + 1 < per) fetch(row + (int64_t)gridDim.x * RW);
@@ -311,8 +332,8 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
             if (sub == 0)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int at = (j * LP + c) * 8 + e;
-                    if (at < a.D) out[m * a.D + at] = x[j][e];
+                    const Group<LP, VEC> q(c, j, a.D);
+                    if (q.in && e >= q.skip && q.base + e < a.D) out[m * a.D + q.base + e] = x[j][e];
                 }
         }
     };
