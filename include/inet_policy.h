@@ -77,8 +77,8 @@ typedef struct InetDeltaGrad {
 int32_t inet_policy_abi_version(void);
 const char *inet_policy_build_info(void);
 
-/* steps a chunk for these sizes (0: unsupported) */
-int32_t inet_policy_delta_chunk(int32_t T, int32_t K, int32_t V, int32_t dtype);
+/* steps a chunk for a window's sizes and types, which are read from a (0: invalid or unsupported) */
+int32_t inet_policy_delta_chunk(const InetDelta *a);
 /* workspace of a window's forward or backward pass in bytes (sizes, type and chunk are read from a; -1: invalid) */
 int64_t inet_policy_delta_work(const InetDelta *a, int32_t backward);
 int32_t inet_policy_delta_forward(const InetDelta *a, void *stream);

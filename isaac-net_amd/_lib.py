@@ -250,7 +250,7 @@ def load_policy(path=POLICY_LIB_PATH):
     lib.inet_policy_build_info.restype = C.c_char_p
     if lib.inet_policy_abi_version() != POLICY_ABI_VERSION:
         raise RuntimeError("libinet_policy.so ABI version mismatch; rebuild it")
-    lib.inet_policy_delta_chunk.argtypes = [i32, i32, i32, i32]
+    lib.inet_policy_delta_chunk.argtypes = [C.POINTER(InetDelta)]
     lib.inet_policy_delta_work.argtypes = [C.POINTER(InetDelta), i32]
     lib.inet_policy_delta_work.restype = i64
     lib.inet_policy_ffn_work.argtypes = [i64, i32, i32, i32]

@@ -551,27 +551,32 @@ __global__ __launch_bounds__(256) void delta_heads_kernel(const float* __restric
 template <typename T, int C, int KP, bool VEC>
 static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
     const int chunks = (d.T + C - 1) / C, vp = (d.V + 31) & ~31;
-    constexpr int V_MOST = std::is_same<T, _Float16>::value && C == 64 ? 64 : INET_POLICY_MAX_HEAD;
-    static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && window_lds<T, C, KP>(V_MOST) <= LDS_MAX, "LDS");
-    if (chunks == 1) {
-        auto window = delta_window_kernel<T, C, KP, VEC>;
-        const size_t lds = window_lds<T, C, KP>(vp);
-        if (allow_lds((const void*)window, lds)) return INET_POLICY_ELAUNCH;
-        hipLaunchKernelGGL(window, dim3(d.B * d.H), dim3(DELTA_WG), lds, st, d, g);
+    static_assert(chunk_lds<T, C, KP>(INET_POLICY_MAX_HEAD) <= LDS_MAX, "LDS");
+    if (d.work) {
+        if (int rc = delta_split(d, &g, VEC, st)) return rc;
+    } else if constexpr (C == 32) {               // (chunks of 64 are for delta_split alone)
+        static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && window_lds<T, C, KP>(INET_POLICY_MAX_HEAD) <= LDS_MAX, "LDS");
+        if (chunks == 1) {
+            auto window = delta_window_kernel<T, C, KP, VEC>;
+            const size_t lds = window_lds<T, C, KP>(vp);
+            if (allow_lds((const void*)window, lds)) return INET_POLICY_ELAUNCH;
+            hipLaunchKernelGGL(window, dim3(d.B * d.H), dim3(DELTA_WG), lds, st, d, g);
+        } else {
+            auto scan = delta_scan_kernel<T, C, KP, VEC>;
+            const size_t lds = sizeof(ScanLds<T, C, KP>);
+            if (allow_lds((const void*)scan, lds)) return INET_POLICY_ELAUNCH;
+            hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
+        }
         if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     } else {
-        const size_t lds = sizeof(ScanLds<T, C, KP>), cl = chunk_lds<T, C, KP>(vp);
-        auto scan = delta_scan_kernel<T, C, KP, VEC>;
+        return INET_POLICY_EINVAL;
+    }
+    if (!chunks) return INET_POLICY_OK;
+    if (chunks > 1) {
         auto chunk = delta_chunk_kernel<T, C, KP, VEC>;
-        if (allow_lds((const void*)scan, lds) || allow_lds((const void*)chunk, cl)) return INET_POLICY_ELAUNCH;
-        if (d.work) {
-            if (int rc = delta_split(d, &g, VEC, st)) return rc;
-        } else {
-            hipLaunchKernelGGL(scan, dim3(d.B * d.H, (d.V + 63) / 64), dim3(DELTA_WG), lds, st, d, g);
-            if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
-        }
-        if (!chunks) return INET_POLICY_OK;
-        hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), cl, st, d, g);
+        const size_t lds = chunk_lds<T, C, KP>(vp);
+        if (allow_lds((const void*)chunk, lds)) return INET_POLICY_ELAUNCH;
+        hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), lds, st, d, g);
         if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     }
     if (d.H != d.Hk) {

@@ -127,7 +127,8 @@ int delta_forward(const InetDelta& d, bool vec, hipStream_t st) {
     return delta_dispatch(d, [&](auto t, auto c, auto kp) {
         typedef typename decltype(t)::type T;
         constexpr int C = decltype(c)::value, KP = decltype(kp)::value;
-        return vec ? launch<T, C, KP, true>(d, st) : launch<T, C, KP, false>(d, st);
+        if constexpr (C == 32) return vec ? launch<T, C, KP, true>(d, st) : launch<T, C, KP, false>(d, st);
+        return INET_POLICY_EINVAL;                // (chunks of 64 are for delta_split alone)
     });
 }
 

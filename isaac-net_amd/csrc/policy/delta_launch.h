@@ -19,26 +19,22 @@ inline bool allow_lds(const void* kernel, size_t bytes) {
 template <typename V> struct Type { typedef V type; };
 template <int V> using Int = std::integral_constant<int, V>;
 
-// (more planes fill the LDS with fewer steps: 32-bit values and large float16 heads go by chunks of 32 alone)
-template <typename F, typename T> int delta_dispatch_t(const InetDelta& d, T t, F&& f) {
-    constexpr bool F32 = std::is_same<typename T::type, float>::value;
-    constexpr bool B16 = std::is_same<typename T::type, __bf16>::value;
-    if (d.chunk == 32)
-        return d.K <= 32 ? f(t, Int<32>{}, Int<32>{}) : d.K <= 64 ? f(t, Int<32>{}, Int<64>{})
-                                                                  : f(t, Int<32>{}, Int<128>{});
-    if constexpr (!F32) {
-        if (d.K <= 32) return f(t, Int<64>{}, Int<32>{});
-        if (d.K <= 64) return f(t, Int<64>{}, Int<64>{});
-    }
-    if constexpr (B16) return f(t, Int<64>{}, Int<128>{});
-    return INET_POLICY_EINVAL;
+template <typename T, typename F> int delta_dispatch_keys(const InetDelta& d, F&& f) {
+    constexpr Type<T> t{};
+    if constexpr (std::is_same<T, __bf16>::value)
+        if (d.chunk == 64)
+            return d.K <= 32 ? f(t, Int<64>{}, Int<32>{}) : d.K <= 64 ? f(t, Int<64>{}, Int<64>{})
+                                                                      : f(t, Int<64>{}, Int<128>{});
+    if (d.chunk != 32) return INET_POLICY_EINVAL;
+    return d.K <= 32 ? f(t, Int<32>{}, Int<32>{}) : d.K <= 64 ? f(t, Int<32>{}, Int<64>{})
+                                                              : f(t, Int<32>{}, Int<128>{});
 }
 
 // f(type, chunk, padded key size) for a window's sizes
 template <typename F> int delta_dispatch(const InetDelta& d, F&& f) {
-    if (d.dtype == INET_POLICY_F32) return delta_dispatch_t(d, Type<float>{}, f);
-    if (d.dtype == INET_POLICY_BF16) return delta_dispatch_t(d, Type<__bf16>{}, f);
-    return delta_dispatch_t(d, Type<_Float16>{}, f);
+    if (d.dtype == INET_POLICY_F32) return delta_dispatch_keys<float>(d, f);
+    if (d.dtype == INET_POLICY_BF16) return delta_dispatch_keys<__bf16>(d, f);
+    return delta_dispatch_keys<_Float16>(d, f);
 }
 
 // vec: all rows start on 16 bytes and hold whole groups of eight

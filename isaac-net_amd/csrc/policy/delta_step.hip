@@ -121,19 +121,36 @@ static int check(const InetDelta* a) {
     return INET_POLICY_OK;
 }
 
+// The way through a window. The matrices of a chunk and what they make grow with C, and with them the LDS a workgroup holds:
+// by chunks of 32 three share a compute unit, by 64 two. 2048 robots of 4 heads of 64 x 64, bfloat16, training, us at 32 and
+// 64 steps a chunk: 24 steps 275 and 875, 64 steps 740 and 1045, 200 steps 2534 and 3258.
+// A window of a few robots is delta_split.hip's, which takes all its chunks at once but for the state's own chain (`groups`
+// workgroups). One pass and split, us, 64 x 64, bfloat16, training:
+//     T         16 groups      64 groups      96 groups      128 groups
+//     100        64,  63        71,  72        73,  77         72,  79
+//     150        72,  65        80,  79        85,  81         84,  87
+//     400       152, 110       165, 136       179, 156        185, 179
+//     1000      344, 195       378, 265       411, 373        449, 458
+// so from five chunks on, up to 96 groups. There the chain's length counts, and chunks of 64 halve it: 168, 271 and 344 us for
+// the last line's first three, 475 for 2 x 4096 of 8 heads that take 618 by 32; at T = 400 they gain nothing (112, 141, 184).
+// Bfloat16 alone takes 64: float16's second plane makes them no faster (64 groups, T = 1000: 299 by 32, 331 by 64), and
+// float32's third does not fit the LDS.
+static int64_t groups_of(const InetDelta* a) { return (int64_t)a->B * a->H * ((a->V + 63) / 64); }
+static bool split(const InetDelta* a) {
+    const int64_t chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;
+    return chunks >= 5 && groups_of(a) <= 96;
+}
+static int chunk_of(const InetDelta* a) {
+    return a->dtype == INET_POLICY_BF16 && a->T > 512 && groups_of(a) <= 96 ? 64 : 32;
+}
+
 static int check_window(const InetDelta* a) {
     if (int rc = check(a)) return rc;
-    if (a->chunk != inet_policy_delta_chunk(a->T, a->K, a->V, a->dtype)) return INET_POLICY_EINVAL;
+    if (a->chunk != chunk_of(a)) return INET_POLICY_EINVAL;
     if ((int64_t)a->H * a->V > 1 << 22) return INET_POLICY_EUNSUPPORTED;      // (a chunk's offsets are 32-bit)
     const int64_t chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;
     if ((int64_t)a->B * a->H * chunks > GRID_MAX) return INET_POLICY_EUNSUPPORTED;
     return INET_POLICY_OK;
-}
-
-// whether a window goes by delta_split.hip: several chunks, and too few robots and heads for the chip's compute units
-static bool split(const InetDelta* a) {
-    const int64_t groups = (int64_t)a->B * a->H * ((a->V + 63) / 64), chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;
-    return chunks >= 4 && groups < 256;
 }
 
 // whether the inputs' rows start on 16 bytes and hold whole groups of eight
@@ -149,12 +166,7 @@ static bool aligned(const InetDelta* a) {
 
 extern "C" {
 
-int32_t inet_policy_delta_chunk(int32_t T, int32_t K, int32_t V, int32_t dtype) {
-    if (T < 0 || K < 1 || V < 1 || K > INET_POLICY_MAX_HEAD || V > INET_POLICY_MAX_HEAD || dtype < 0 || dtype > 2)
-        return 0;
-    if (dtype == INET_POLICY_F32 || (dtype == INET_POLICY_F16 && (K > 64 || V > 64))) return 32;   // (LDS: delta_launch.h)
-    return T <= 32 ? 32 : 64;
-}
+int32_t inet_policy_delta_chunk(const InetDelta* a) { return pol::check(a) ? 0 : pol::chunk_of(a); }
 
 int64_t inet_policy_delta_work(const InetDelta* a, int32_t backward) {
     if (pol::check_window(a)) return -1;

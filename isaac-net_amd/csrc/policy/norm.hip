@@ -16,7 +16,6 @@
 namespace pol {
 
 constexpr int NORM_WG = 256;
-constexpr int NORM_BLOCKS = 1024;            // workgroups of the backward pass, at most
 
 // the sum over a row's LP lanes (LP <= 64), or over the workgroup (LP = 256; s: four words of LDS of its own): along the
 // rows of 16 lanes by rotations, across them by swaps of rows and halves
@@ -372,11 +371,12 @@ __global__ __launch_bounds__(1024) void norm_weights_kernel(const float* __restr
     }
 }
 
-// workgroups of the backward pass: one a compute unit, or enough that each takes eight groups of rows (the partial rows
-// are as long as the data's), as many as run at once at most
+// workgroups of the backward pass: two a compute unit where each then has eight groups of rows or more, else one (a
+// workgroup's partial rows are as long as the data's). us at 256, 512 and 1024 workgroups: 131072 x 512 bfloat16 322, 249
+// and 258; 20000 x 512 42, 33 and 36; 4000 x 4000 74, 84 and 99; 5001 x 999 float32 45, 52 and 65
 static int blocks_for(int64_t N, int rows) {
-    const int64_t need = (N + rows - 1) / rows, want = need / 8 > 256 ? need / 8 : 256, n = need < want ? need : want;
-    return (int)(n < NORM_BLOCKS ? n : NORM_BLOCKS);
+    const int64_t need = (N + rows - 1) / rows, want = need >= 8 * 512 ? 512 : 256;
+    return (int)(need < want ? need : want);
 }
 
 template <typename T, int LP, int NJ, bool VEC>
@@ -396,8 +396,11 @@ static int launch(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
 }
 
-// lanes a row and groups a lane: as few lanes as hold the row with one group each, then more groups, and the whole
-// workgroup from 2048 values on
+// lanes a row and groups a lane: as few lanes as hold the row with one group each (N D = 2^25, bfloat16, full gate, training,
+// us: D = 128 by 16 lanes 202, 32 lanes 292, 64 lanes 473; D = 256 by 32 lanes 195, 16 x 2 groups 203, 64 lanes 290), then two
+// groups of a wave (D = 1024: 200, a workgroup a row 285), then a workgroup a row, whose waves hold few registers: a wave with
+// three or four groups takes 365 against 353 at D = 1071, 214 against 235 at 1536, 199 against 214 at 2048, but in float32
+// (N D = 2^24) 211 against 192 at 1536 and 292 against 192 at 2048
 template <typename T, bool VEC> static int sizes(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
     if (a.D <= 128) return launch<T, 16, 1, VEC>(a, d, st);
     if (a.D <= 256) return launch<T, 32, 1, VEC>(a, d, st);

@@ -142,7 +142,7 @@ def _delta_forward(q, k, v, g, beta, state, reset, scale, keep):
     B, T, H, V = v.shape
     K, dev = q.shape[-1], v.device
     a = _delta_args(q, k, v, g, beta, reset, scale, 2)
-    a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
+    a.chunk = lib.inet_policy_delta_chunk(C.byref(a))
     o = torch.empty((B, T, H, V), dtype=v.dtype, device=dev)
     out = torch.empty((B, H, K, V), dtype=torch.float32, device=dev)
     a.state, a.o, a.state_out = _ptr(state), o.data_ptr(), out.data_ptr()
@@ -176,7 +176,7 @@ class _DeltaRule(torch.autograd.Function):
         B, T, H, V = v.shape
         K, dev = q.shape[-1], q.device
         a = _delta_args(q, k, v, g, beta, reset, ctx.scale, 2)
-        a.chunk = lib.inet_policy_delta_chunk(T, K, V, a.dtype)
+        a.chunk = lib.inet_policy_delta_chunk(C.byref(a))
         a.state, a.chunk_state, a.err = _ptr(state), _ptr(chunk_state), err.data_ptr()
         work = _delta_work(lib, a, dev, 1)  # noqa: F841  (held until the call is enqueued)
         d_o = None if d_o is None else d_o.contiguous()

@@ -96,6 +96,14 @@ def test_window(dt, B, T, Hk, H, K, V):
     check_delta(*delta_inputs(B, T, Hk, H, K, V, DT[dt]))
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,T,Hk,H,K,V", [
+    (1, 161, 1, 2, 32, 24), (2, 530, 1, 1, 48, 64), (1, 577, 1, 2, 128, 96), (1, 1025, 1, 1, 24, 72),  # a few robots
+    (40, 70, 1, 3, 32, 40), (33, 130, 3, 3, 64, 64), (20, 100, 5, 5, 100, 128)])                       # many
+def test_window_of_several_chunks(dt, B, T, Hk, H, K, V):
+    check_delta(*delta_inputs(B, T, Hk, H, K, V, DT[dt], seed=16, end=0.02))
+
+
 @pytest.mark.parametrize("dt,gate", [("bf16", "f32"), ("f32", "bf16"), ("f16", "f32")])
 def test_window_gates_of_another_type(dt, gate):
     check_delta(*delta_inputs(2, 75, 1, 2, 48, 32, DT[dt], gate_dt=DT[gate]))
@@ -129,9 +137,10 @@ def test_window_values(dt, case):
     check_delta(ins, reset, d_o, d_s)
 
 
-def test_window_emptied_memory_is_empty():
+@pytest.mark.parametrize("dt,B,T", [("f32", 3, 70), ("f32", 3, 20), ("bf16", 3, 200), ("bf16", 3, 600), ("f16", 50, 200)])
+def test_window_emptied_memory_is_empty(dt, B, T):
     """Whatever the state held, an episode that starts at the window's first step sees none of it, in either direction."""
-    ins, reset, d_o, d_s = delta_inputs(3, 70, 1, 2, 32, 32, torch.float32, seed=4)
+    ins, reset, d_o, d_s = delta_inputs(B, T, 1, 2, 32, 32, DT[dt], seed=4)
     reset[0, 0] = True
     ins[5][0] = math.nan
     a, b = delta_both([*ins[:5], torch.nan_to_num(ins[5], nan=0.0)], reset, d_o, d_s)
@@ -140,7 +149,7 @@ def test_window_emptied_memory_is_empty():
         assert torch.equal(x, y), n
 
 
-@pytest.mark.parametrize("T", [20, 90])
+@pytest.mark.parametrize("T", [20, 90, 200])
 @pytest.mark.parametrize("used", ["o", "state"])
 def test_window_one_output_used(T, used):
     ins, reset, d_o, d_s = delta_inputs(2, T, 1, 2, 32, 48, torch.float32, seed=14, end=0.02)

@@ -146,9 +146,10 @@ def test_c_entry_points_refuse_before_any_launch(lib):
     assert lib.inet_policy_delta_forward(B(d), none) == -1                          # no heads
     d.B, d.T, d.Hk, d.H, d.K, d.V = 2, 40, 1, 2, 16, 16
     assert lib.inet_policy_delta_forward(B(d), none) == -1                          # chunk not set
-    d.chunk = lib.inet_policy_delta_chunk(40, 16, 16, 0)
-    assert d.chunk == 32 and lib.inet_policy_delta_chunk(40, 16, 16, 1) == 64
-    assert lib.inet_policy_delta_chunk(40, 129, 16, 1) == 0 == lib.inet_policy_delta_chunk(40, 16, 16, 3)
+    for key, value, chunk in (("T", 4000, 32), ("dtype", 1, 64), ("B", 96, 32), ("K", 129, 0), ("dtype", 3, 0)):
+        setattr(d, key, value)
+        assert lib.inet_policy_delta_chunk(B(d)) == chunk, key
+    d.B, d.T, d.K, d.dtype, d.chunk = 2, 40, 16, 0, 32
     assert lib.inet_policy_delta_forward(B(d), none) == -1                          # no tensors
     assert lib.inet_policy_delta_backward(B(d), B(dg), none) == -1
     assert lib.inet_policy_delta_step(B(d), none) == -1                             # T is not 1
