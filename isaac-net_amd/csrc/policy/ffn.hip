@@ -255,7 +255,9 @@ struct FfnShape {
 };
 
 // y, or (BACK) da and du side by side in da [N][2 F8]. A workgroup takes tile after tile: the next one's first step is on
-// its way, and dy has come during the last step, while the results are stored.
+// its way, and dy has come during the last step, while the results are stored. The matrix instructions bound it, then what
+// the activation and the stores leave of their time: 131072 x 512 x 2048, bfloat16, silu: y 640 us, 859 TFLOP/s (the library's
+// product of these sizes alone 716, 8192^3 1302); da and du 1025 us with 1.6 GB of dy, da and du beside the same products.
 template <typename T, typename P, int ACT, bool BACK>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __restrict__ y, const T* __restrict__ dy,
@@ -342,7 +344,9 @@ void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __r
     }
 }
 
-// C [rows][cols] = a b (+ a2 b2 where there are such), or shares of the sum each to a C of its own
+// C [rows][cols] = a b (+ a2 b2 where there are such), or shares of the sum each to a C of its own. At the sizes above: dx
+// 650 us, 846 TFLOP/s (the library's product 925); both dW 590 us, 932 TFLOP/s (559). An operand across the sum goes through
+// registers and is transposed by LDS reads, which is what keeps it from the rate of 8192^3.
 template <typename T, typename P, bool RA, bool CA, typename O>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, Operand<T, CA> b2, int64_t K,
@@ -376,7 +380,7 @@ void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, O
     else finish(std::false_type{});
 }
 
-// rows padded to a multiple of eight with zeros
+// rows padded to a multiple of eight with zeros (a copy; odd widths alone)
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_pad_kernel(const T* __restrict__ in, int64_t in_s, int64_t rows, int D,
                                                       T* __restrict__ out, int D8) {
@@ -387,7 +391,8 @@ __global__ __launch_bounds__(256) void ffn_pad_kernel(const T* __restrict__ in, 
     out[i] = c < D ? in[r * in_s + c] : (T)0.0f;
 }
 
-// the shares of a product over N added up in order: out [rows][D] of parts [count][.][cols]
+// the shares of a product over N added up in order: out [rows][D] of parts [count][.][cols]. Memory bounds it: 17 us for both
+// weights at 131072 x 512 x 2048 (8 shares, 72 MB, from the L2s in part)
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_add_kernel(const float* __restrict__ parts, int count, int64_t stride,
                                                       int64_t rows, int D, int cols, T* __restrict__ out) {
@@ -404,7 +409,9 @@ static int64_t tiles(int64_t x, int t) { return (x + t - 1) / t; }
 static unsigned blocks256(int64_t n) { return (unsigned)((n + 255) / 256); }
 
 // The tile of a product by how many of the largest it has: 256 x 256 (eight waves, a compute unit's LDS to itself) where
-// they fill the chip's 256 compute units, else 128 x 128, else 64 x 64.
+// they fill the chip's 256 compute units, else 128 x 128, else 64 x 64. Forward, us by tiles of 64, 128 and 256: 512 x 256 x 1024
+// 5, 7, 12; 1500 x 512 x 2048 16, 15, 20; 2048 x 512 x 2048 19, 16, 20; 4096 x 512 x 2048 34, 27, 23; 8192 x 256 x 1024 21, 19,
+// 16; 65536 x 512 x 2048 549, 460, 332.
 static int size_for(int64_t rows, int64_t cols) {
     return tiles(rows, 256) * tiles(cols, 256) >= 256 ? 2 : tiles(rows, 128) * tiles(cols, 128) >= 256 ? 1 : 0;
 }
@@ -417,7 +424,10 @@ using Sized = typename std::conditional<SIZE == 2, Product<T, 256, 256, 2, 4, RA
               typename std::conditional<SIZE == 1, Product<T, 128, 128, 2, 2, RA, CA, HALVES>,
                                         Product<T, 64, 64, 2, 2, RA, CA, HALVES>>::type>::type;
 
-// the weights' gradients: the tile, and shares of the sum over N, at least 512 rows each, until the chip is full twice over
+// the weights' gradients: the tile, and shares of the sum over N, at least 512 rows each, until the chip is full, of the smaller
+// tile twice over. us of dx and dW with the adding up, by tiles of 128 and 256: 65536 x 512 x 2048 735, 629; 65536 x 512 x 1024
+// 383, 360; 65536 x 256 x 1024 213, 207; 4096 x 256 x 1024 50, 61; 4096 x 512 x 1024 59, 64. By 256 and 512 workgroups: 65536 x
+// 512 x 2048 of 128 1031, 735, of 256 629, 637. By 256, 512 and 1024 rows a share at least: 4096 x 512 x 1024 60, 59, 90.
 static int dw_size(int64_t D8, int64_t F8) { return tiles(2 * F8, 256) * tiles(D8, 256) >= 16 ? 2 : 1; }
 static int shares(int64_t N, int64_t D8, int64_t F8) {
     const int size = dw_size(D8, F8), b = size == 2 ? 256 : 128;
