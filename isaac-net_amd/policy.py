@@ -68,6 +68,8 @@ def _call(fn, dev, what, *args):
     else:
         with torch.cuda.device(dev):
             rc = fn(*args, _raw_stream(dev))
+    if rc == -2:                                 # INET_POLICY_EUNSUPPORTED
+        raise HipUnsupported(f"{what}: more rows, heads or steps than a launch takes")
     if rc:
         _lib.check(rc, what)
 

@@ -411,6 +411,17 @@ def test_norm_gradient_against_differences():
             assert abs(diff - want) <= 0.01 * want, i
 
 
+def test_too_many_rows_are_refused():
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device=DEV).expand((1 << 24) + 1, 8)
+    with pytest.raises(P.HipUnsupported, match="block_norm"):
+        P.block_norm(x, pre_weight=torch.ones(8, device=DEV))
+    with pytest.raises(P.HipUnsupported, match="gated_ffn"):
+        P.gated_ffn(x, x[:8], x[:8])
+    q = torch.zeros(1, 1, 1, 1, device=DEV).expand(1 << 24, 1, 1, 1)
+    with pytest.raises(P.HipUnsupported, match="delta_rule"):
+        P.delta_rule(q, q, q, q[..., 0], q[..., 0])
+
+
 # ------------------------------------------------------------------------------------------------ as a user runs them
 def test_twice_the_same_and_another_stream():
     """Results do not vary from run to run, nor on a stream of the caller's."""
