@@ -418,7 +418,7 @@ def test_too_many_rows_are_refused():
     with pytest.raises(P.HipUnsupported, match="gated_ffn"):
         P.gated_ffn(x, x[:8], x[:8])
     q = torch.zeros(1, 1, 1, 1, device=DEV).expand(1 << 24, 1, 1, 1)
-    with pytest.raises(P.HipUnsupported, match="delta_rule"):
+    with pytest.raises(P.HipUnsupported, match="robots x heads x chunks"):
         P.delta_rule(q, q, q, q[..., 0], q[..., 0])
 
 
