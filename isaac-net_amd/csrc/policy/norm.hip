@@ -381,14 +381,17 @@ static int blocks_for(int64_t N, int rows) {
     return (int)(need < want ? need : want);
 }
 
+template <typename T, int LP, int NJ, bool VEC> static int launch_forward(const InetNorm& a, hipStream_t st) {
+    constexpr int RW = NORM_WG / LP;
+    hipLaunchKernelGGL((norm_forward_kernel<T, LP, NJ, VEC>), dim3((unsigned)((a.N + RW - 1) / RW)), dim3(NORM_WG), 0,
+                       st, a);
+    return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
+}
+
 template <typename T, int LP, int NJ, bool VEC>
 static int launch(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
     constexpr int RW = NORM_WG / LP;
-    if (!d) {
-        hipLaunchKernelGGL((norm_forward_kernel<T, LP, NJ, VEC>), dim3((unsigned)((a.N + RW - 1) / RW)), dim3(NORM_WG),
-                           0, st, a);
-        return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
-    }
+    if (!d) return launch_forward<T, LP, NJ, VEC>(a, st);
     const int blocks = blocks_for(a.N, RW);
     hipLaunchKernelGGL((norm_backward_kernel<T, LP, NJ, VEC>), dim3(blocks), dim3(NORM_WG), 0, st, a, *d);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
@@ -400,14 +403,19 @@ static int launch(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
 
 // lanes a row and groups a lane: as few lanes as hold the row with one group each (N D = 2^25, bfloat16, full gate, training,
 // us: D = 128 by 16 lanes 202, 32 lanes 292, 64 lanes 473; D = 256 by 32 lanes 195, 16 x 2 groups 203, 64 lanes 290), then two
-// groups of a wave (D = 1024: 200, a workgroup a row 285), then a workgroup a row, whose waves hold few registers: a wave with
-// three or four groups takes 365 against 353 at D = 1071, 214 against 235 at 1536, 199 against 214 at 2048, but in float32
-// (N D = 2^24) 211 against 192 at 1536 and 292 against 192 at 2048
+// groups of a wave (D = 1024: 200, a workgroup a row 285), then, where rows are whole 16-bit groups on 16 bytes, three groups
+// (1032: 254, a workgroup a row 296; 1304: 250, 262; 1536: 214, 237) and forward four (forward alone at 1600 61, 67, 1904 60, 69,
+// 2048 59, 64; backward 182, 161, 188, 149, 134, 138), else a workgroup a row, whose waves hold few registers (odd rows at D = 1071
+// 353, three groups 365; float32, N D = 2^24: 1536 192, 211; 2048 192, 292)
 template <typename T, bool VEC> static int sizes(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
     if (a.D <= 128) return launch<T, 16, 1, VEC>(a, d, st);
     if (a.D <= 256) return launch<T, 32, 1, VEC>(a, d, st);
     if (a.D <= 512) return launch<T, 64, 1, VEC>(a, d, st);
     if (a.D <= 1024) return launch<T, 64, 2, VEC>(a, d, st);
+    if constexpr (VEC && sizeof(T) == 2) {
+        if (a.D <= 1536) return launch<T, 64, 3, VEC>(a, d, st);
+        if (a.D <= 2048 && !d) return launch_forward<T, 64, 4, VEC>(a, st);
+    }
     if (a.D <= 2048) return launch<T, 256, 1, VEC>(a, d, st);
     if (a.D <= 4096) return launch<T, 256, 2, VEC>(a, d, st);
     return launch<T, 256, 4, VEC>(a, d, st);

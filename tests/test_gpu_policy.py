@@ -364,7 +364,7 @@ def check_norm(N, D, *args, **kw):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("N,D", [(1, 1), (3, 8), (17, 127), (33, 128), (5, 200), (9, 256), (70, 500), (6, 512), (5, 999),
-                                 (4, 1024), (7, 1111), (3, 2048), (3, 4000), (2, 8192), (2100, 64)])
+                                 (4, 1024), (7, 1111), (600, 1032), (9, 1536), (6, 1704), (3, 2048), (3, 4000), (2, 8192), (2100, 64)])
 def test_norm(dt, N, D):
     check_norm(N, D, DT[dt])
 
