@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+import torch.autograd.graph
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -23,6 +24,7 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = ("silu", "gelu", "relu")          # "gelu" is the tanh form
 MAX_HEAD, MAX_WIDTH = 128, 8192
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_overwritten = torch.autograd.graph.increment_version    # what the kernels write, autograd does not see
 
 
 def _unsupported_type(name, x):
@@ -230,6 +232,7 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
     a = _delta_args(q, k, v, g, beta, reset, float(q.shape[-1] ** -0.5 if scale is None else scale), 1)
     a.o, a.state_out = out.data_ptr(), state.data_ptr()
     _call(_lib.load_policy().inet_policy_delta_step, dev, "delta_rule_step", C.byref(a))
+    _overwritten((state, out))                   # (a window's backward pass may have been given either to keep)
     return out
 
 
