@@ -220,10 +220,14 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
 def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
     """One control step of the gated delta rule, the memory updated in place: q, k [B, Hk, K], v [B, H, V], g and beta
     [B, H], state [B, H, K, V] float32 contiguous, reset [B] (an emptied memory is empty whatever it held). Returns o
-    [B, H, V] (in `out` if given, contiguous of v's type). No derivatives: windows are trained through delta_rule."""
+    [B, H, V] (in `out` if given, contiguous of v's type). No derivatives (in grad mode an input that requires grad is refused):
+    windows are trained through delta_rule."""
     dev = _delta_check(q, k, v, g, beta, state, reset, 1)
     if state is None or not state.is_contiguous():
         raise ValueError("state has to be a contiguous tensor: it is updated in place")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
+                                    beta.requires_grad or state.requires_grad or (out is not None and out.requires_grad)):
+        raise HipUnsupported("delta_rule_step has no derivatives: call it under torch.no_grad(), or delta_rule")
     q, k, v = _rows(q), _rows(k), _rows(v)
     if out is None:
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device)

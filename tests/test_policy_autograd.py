@@ -5,6 +5,7 @@ import torch
 
 import isaac_net_amd as P
 from test_gpu_policy import delta_inputs
+from test_policy import _OnGpu
 
 DEV = "cuda:0"
 
@@ -35,3 +36,27 @@ def test_values_overwritten_before_the_backward_pass_are_noticed():
         P.delta_rule_step(*(t[:, 0].clone() for t in x[:5]), x[5].clone(), out=x[2][:, 0])
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.sum().backward()
+
+
+def test_a_step_that_would_drop_derivatives_is_refused():
+    """delta_rule_step has none: in grad mode it takes no tensor that asks for them, and leaves the state as it was."""
+    x = [torch.zeros(2, 1, 8), torch.zeros(2, 1, 8), torch.zeros(2, 2, 4), torch.zeros(2, 2), torch.zeros(2, 2)]
+    state, out = torch.zeros(2, 2, 8, 4), torch.zeros(2, 2, 4)
+    with _OnGpu():
+        for t in (*x, state, out):
+            t.requires_grad_(True)
+            with pytest.raises(P.HipUnsupported, match="derivatives"):
+                P.delta_rule_step(*x, state, out=out)
+            t.requires_grad_(False)
+
+
+@pytest.mark.gpu
+def test_a_step_without_grad_mode_takes_any_tensor():
+    ins, _, _, _ = delta_inputs(2, 1, 1, 2, 32, 32, torch.float32, seed=22)
+    x = [t.to(DEV) for t in ins]
+    y = [t[:, 0].clone() for t in x[:5]]
+    state = x[5].clone()
+    want = P.delta_rule_step(*y, state)
+    with torch.no_grad():
+        got = P.delta_rule_step(*(t.requires_grad_(True) for t in y), x[5])
+    assert torch.equal(got, want) and torch.equal(x[5], state) and not got.requires_grad
