@@ -4,8 +4,8 @@ norms, as hand-written HIP kernels behind the C ABI of include/inet_policy.h (li
 A robot is one row of the batch: an engine's E envs x R robots flattened. Between two control steps a policy calls
 delta_rule_step (every robot's memory takes one step, in place); to train, it calls delta_rule over a window of steps
 from the state that the rollout held, with the envs' episode ends as `reset`. delta_rule, gated_ffn and block_norm take
-part in torch's autograd (first derivatives). Every call goes on torch's current stream and returns without waiting;
-workspaces come from torch's allocator.
+part in torch's autograd (first derivatives, reverse mode). Every call goes on torch's current stream and returns without
+waiting; workspaces come from torch's allocator.
 
 Wrong shapes, types and devices raise ValueError, sizes and types that the kernels do not implement HipUnsupported.
 """
@@ -15,6 +15,7 @@ import ctypes as C
 
 import torch
 import torch.autograd.graph
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -31,9 +32,17 @@ def _unsupported_type(name, x):
     return HipUnsupported(f"{name}: {x.dtype}; float32, bfloat16 and float16 are implemented")
 
 
+def _no_tangents(xs):
+    for n, x in xs.items():
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise HipUnsupported(f"{n} has a tangent: the policy operators have no forward-mode derivatives")
+
+
 def _on_gpu(**xs):
     """The index of the device that all tensors are on."""
     dev = -1
+    if forward_ad._current_level >= 0:           # (inside a dual_level)
+        _no_tangents(xs)
     for n, x in xs.items():
         if x is None:
             continue
@@ -228,6 +237,8 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or state.requires_grad or (out is not None and out.requires_grad)):
         raise HipUnsupported("delta_rule_step has no derivatives: call it under torch.no_grad(), or delta_rule")
+    if out is not None and forward_ad._current_level >= 0:
+        _no_tangents({"out": out})
     q, k, v = _rows(q), _rows(k), _rows(v)
     if out is None:
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device)

@@ -1,7 +1,10 @@
 """The policy operators beside torch's autograd: what a call overwrites is known to it, and derivatives that an operator
 does not have are refused, not dropped."""
+import contextlib
+
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import isaac_net_amd as P
 from test_gpu_policy import delta_inputs
@@ -60,3 +63,24 @@ def test_a_step_without_grad_mode_takes_any_tensor():
     with torch.no_grad():
         got = P.delta_rule_step(*(t.requires_grad_(True) for t in y), x[5])
     assert torch.equal(got, want) and torch.equal(x[5], state) and not got.requires_grad
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent goes through no operator: with one on any input they refuse, in grad mode or not."""
+    q, k, v, g, beta = (torch.zeros(2, 3, 1, 8), torch.zeros(2, 3, 1, 8), torch.zeros(2, 3, 2, 4), torch.zeros(2, 3, 2),
+                        torch.zeros(2, 3, 2))
+    x, w = torch.zeros(3, 8).half(), torch.zeros(5, 8).half()
+    y, one = torch.zeros(3, 8), torch.ones(8)
+    calls = [(P.delta_rule, dict(q=q, k=k, v=v, g=g, beta=beta, state=torch.zeros(2, 2, 8, 4))),
+             (P.delta_rule_step, dict(q=q[:, 0], k=k[:, 0], v=v[:, 0], g=g[:, 0], beta=beta[:, 0],
+                                      state=torch.zeros(2, 2, 8, 4), out=torch.zeros(2, 2, 4))),
+             (P.gated_ffn, dict(x=x, w_gate=w, w_up=w.clone())),
+             (P.block_norm, dict(x=y, f=y.clone(), gate=y.clone(), scale=one, post_weight=one.clone(),
+                                 pre_weight=one.clone()))]
+    for f, kw in calls:
+        for n, t in kw.items():
+            for grad in (True, False):
+                with _OnGpu() if n == "out" else contextlib.nullcontext(), forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    dual = forward_ad.make_dual(t, torch.ones_like(t))
+                    with pytest.raises(P.HipUnsupported, match=f"{n}.*forward-mode"):
+                        f(**{**kw, n: dual})
