@@ -72,6 +72,12 @@ def _ptr(x):
     return None if x is None else x.data_ptr()
 
 
+def _span(x):
+    """x's first byte and the one past its last."""
+    at = x.data_ptr()
+    return at, at + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size() if x.numel() else at
+
+
 def _call(fn, dev, what, *args):
     """fn on the device's current stream."""
     if torch.cuda.current_device() == dev:
@@ -229,7 +235,7 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
 def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
     """One control step of the gated delta rule, the memory updated in place: q, k [B, Hk, K], v [B, H, V], g and beta
     [B, H], state [B, H, K, V] float32 contiguous, reset [B] (an emptied memory is empty whatever it held). Returns o
-    [B, H, V] (in `out` if given, contiguous of v's type). No derivatives (in grad mode an input that requires grad is refused):
+    [B, H, V] (in `out` if given, contiguous of v's type: v itself, or over none of the inputs). No derivatives (in grad mode an input that requires grad is refused):
     windows are trained through delta_rule."""
     dev = _delta_check(q, k, v, g, beta, state, reset, 1)
     if state is None or not state.is_contiguous():
@@ -244,6 +250,15 @@ def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     elif out.shape != v.shape or out.dtype != v.dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out has to be a contiguous {tuple(v.shape)} tensor of {v.dtype} on {v.device}")
+    else:
+        first, end = _span(out)
+        for n, x in (("q", q), ("k", k), ("v", v), ("g", g), ("beta", beta), ("state", state), ("reset", reset)):
+            # (a wave has read its own values of v before it writes them: v itself may be out)
+            if x is None or (n == "v" and x.data_ptr() == first and x.is_contiguous()):
+                continue
+            at, to = _span(x)
+            if at < end and first < to:
+                raise ValueError(f"out overlaps {n}: the kernel reads one head's while it writes another's")
     a = _delta_args(q, k, v, g, beta, reset, float(q.shape[-1] ** -0.5 if scale is None else scale), 1)
     a.o, a.state_out = out.data_ptr(), state.data_ptr()
     _call(_lib.load_policy().inet_policy_delta_step, dev, "delta_rule_step", C.byref(a))

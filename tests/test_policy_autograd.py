@@ -7,6 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 import isaac_net_amd as P
+from isaac_net_amd import policy
 from test_gpu_policy import delta_inputs
 from test_policy import _OnGpu
 
@@ -84,3 +85,34 @@ def test_forward_mode_derivatives_are_refused():
                     dual = forward_ad.make_dual(t, torch.ones_like(t))
                     with pytest.raises(P.HipUnsupported, match=f"{n}.*forward-mode"):
                         f(**{**kw, n: dual})
+
+
+def test_an_output_over_an_input_is_refused():
+    """A step's heads are written while others are read: `out` may lie over none of the tensors that the call reads
+    (but be v)."""
+    buf = torch.zeros(2 * 2 * 8 * 4 + 64)
+    x = [torch.zeros(2, 2, 4) for _ in range(3)] + [torch.zeros(2, 2) for _ in range(2)]
+    state = buf[:2 * 2 * 4 * 4].view(2, 2, 4, 4)
+    with _OnGpu():
+        policy._on_gpu = lambda **x: -1               # (what a CPU tensor says of itself)
+        for i in range(5):
+            y = [t.clone() for t in x]
+            y[i] = buf[100:].as_strided(x[i].shape, x[i].stride())
+            with pytest.raises(ValueError, match="overlaps"):
+                P.delta_rule_step(*y, torch.zeros(2, 2, 4, 4), out=buf[101:117].view(2, 2, 4))
+        with pytest.raises(ValueError, match="overlaps"):
+            P.delta_rule_step(*x, state, out=buf[60:76].view(2, 2, 4))
+        reset = torch.zeros(64, dtype=torch.uint8)
+        with pytest.raises(ValueError, match="overlaps"):
+            P.delta_rule_step(*x, state, reset=reset[10:12], out=reset.view(torch.float32).view(2, 2, 4))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,V", [(2, 32), (3, 128), (1, 5)])
+def test_a_step_may_write_its_heads_over_v(H, V):
+    ins, _, _, _ = delta_inputs(70, 1, 1, H, 32, V, torch.bfloat16, seed=23)
+    x = [t.to(DEV) for t in ins]
+    y, states = [t[:, 0].clone() for t in x[:5]], [x[5].clone(), x[5].clone()]
+    want = P.delta_rule_step(*y, states[0])
+    assert P.delta_rule_step(*y, states[1], out=y[2]) is y[2]
+    assert torch.equal(y[2], want) and torch.equal(*states)
