@@ -254,7 +254,11 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
         if (a.f) {
             w.load(a.post_weight, c, a.D);
             s.load(a.scale, c, a.D);
-            if (a.post_weight) rf = rsqrtf(sums.sum(sf) * inv + a.eps);
+            // (a row past the last is zeros: with eps 0 its reciprocal would be infinite, and NaN in the weights' sums)
+            if (a.post_weight) {
+                const float sum = sums.sum(sf);
+                rf = live ? rsqrtf(sum * inv + a.eps) : 0.0f;
+            }
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(NORM_WG) void norm_backward_kernel(InetNorm a, Inet
                     sz += z[j][e] * wp.at(j, e) * y[j][e];
                 }
             sums.sum(sy, sz);
-            const float ry = rsqrtf(sy * inv + a.eps);
+            const float ry = live ? rsqrtf(sy * inv + a.eps) : 0.0f;
             sz *= inv * ry;
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
