@@ -116,7 +116,7 @@ int32_t inet_policy_ffn_backward(const InetFfn *a, const InetFfnGrad *d, void *s
 typedef struct InetNorm {
     int64_t N;
     int32_t D, dtype, gate_kind;                /* gate_kind 0: none, 1: one value a row, 2: one a value */
-    float eps;
+    float eps;                                  /* 0 or more */
     int64_t x_s, f_s, gate_s;
     const void *x, *f, *gate;                   /* f NULL: y = x (no block before) */
     const float *scale, *post_weight, *pre_weight;   /* [D] float32; scale NULL: 1; post_weight NULL: h = f;

@@ -444,7 +444,8 @@ static int run(const InetNorm& a, const InetNormGrad* d, hipStream_t st) {
 }
 
 static int check(const InetNorm* a) {
-    if (!a || a->N < 0 || a->D < 1 || a->dtype < 0 || a->dtype > 2 || a->gate_kind < 0 || a->gate_kind > 2)
+    if (!a || a->N < 0 || a->D < 1 || a->dtype < 0 || a->dtype > 2 || a->gate_kind < 0 || a->gate_kind > 2 ||
+        !(a->eps >= 0.0f))
         return INET_POLICY_EINVAL;
     if (a->D > INET_POLICY_MAX_WIDTH || a->N > (int64_t)1 << 24) return INET_POLICY_EUNSUPPORTED;
     if (a->N == 0) return INET_POLICY_OK;

@@ -431,6 +431,8 @@ def block_norm(x, f=None, gate=None, scale=None, post_weight=None, pre_weight=No
     for n, t in (("scale", scale), ("post_weight", post_weight), ("pre_weight", pre_weight)):
         if t is not None and (t.shape != (D,) or t.dtype != torch.float32):
             raise ValueError(f"{n} has to be [{D}] float32: got {tuple(t.shape)} of {t.dtype}")
+    if not eps >= 0:
+        raise ValueError(f"eps has to be 0 or more: got {eps}")
     if f is None:
         if gate is not None or scale is not None or post_weight is not None:
             raise ValueError("gate, scale and post_weight belong to a block's output f")
