@@ -243,7 +243,7 @@ template <int ACT> DEV void activation(float a, float& h, float& dh) {
         h = a * s;
         dh = s + h * (1.0f - s) * (1.5957691216057308f + 0.21406440f * a2);
     } else {
-        h = a > 0.0f ? a : 0.0f;
+        h = a <= 0.0f ? 0.0f : a;              // (NaN stays)
         dh = a > 0.0f ? 1.0f : 0.0f;
     }
 }

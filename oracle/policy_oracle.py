@@ -37,7 +37,7 @@ def gated_ffn(x, w_gate, w_up, activation="silu"):
     elif activation == "gelu":
         h = 0.5 * a * (1 + torch.tanh(math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)))
     else:
-        h = torch.where(a > 0, a, torch.zeros_like(a))
+        h = torch.where(a <= 0, torch.zeros_like(a), a)          # (NaN stays)
     return h * (x @ w_up.T)
 
 

@@ -1,5 +1,7 @@
 """The policy operators where values are not finite, or where a step between finite ones would not be: a robot whose memory
 or inputs went wrong, a norm without an epsilon, gradients larger than their 16-bit type."""
+import math
+
 import pytest
 import torch
 
@@ -25,3 +27,18 @@ def test_norm_without_an_epsilon(dt, N, D):
         got.append([*outs, *torch.autograd.grad(outs, leaves, [e.to(o) for o, e in zip(outs, d)])])
     for n, a, b in zip(("y", "n", "d_x", "d_f", "d_gate", "d_scale", "d_post_weight", "d_pre_weight"), *got):
         close(n, a, b, D + (N if a.dim() == 1 else 0))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_ffn_passes_nan_on(dt, act):
+    """A robot's NaN, or one in a gate projection alone, comes out as one and nowhere else."""
+    gen = torch.Generator().manual_seed(31)
+    x, wg, wu = rand(gen, 40, 64).to(DT[dt]), rand(gen, 48, 64).to(DT[dt]), rand(gen, 48, 64).to(DT[dt])
+    x[3, 5] = math.nan
+    wg[7, 9] = math.nan
+    with torch.no_grad():
+        y = P.gated_ffn(x.to(DEV), wg.to(DEV), wu.to(DEV), activation=act).cpu()
+    want = torch.zeros(40, 48, dtype=torch.bool)
+    want[3, :] = want[:, 7] = True
+    assert torch.equal(torch.isnan(y), want)
