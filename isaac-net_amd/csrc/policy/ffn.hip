@@ -239,7 +239,8 @@ template <int ACT> DEV void activation(float a, float& h, float& dh) {
         h = a * s;
         dh = s + h * (1.0f - s);
     } else if constexpr (ACT == INET_POLICY_GELU) {
-        const float a2 = a * a, s = logistic(1.5957691216057308f * a * (1.0f + 0.044715f * a2));
+        // (a2 bounded: from |a| of 10^4 on s is 0 or 1 to the last bit, and past 2^64 a * a would be infinite, dh NaN)
+        const float a2 = fminf(a * a, 1e8f), s = logistic(1.5957691216057308f * a * (1.0f + 0.044715f * a2));
         h = a * s;
         dh = s + h * (1.0f - s) * (1.5957691216057308f + 0.21406440f * a2);
     } else {

@@ -42,3 +42,17 @@ def test_ffn_passes_nan_on(dt, act):
     want = torch.zeros(40, 48, dtype=torch.bool)
     want[3, :] = want[:, 7] = True
     assert torch.equal(torch.isnan(y), want)
+
+
+def test_gelu_far_out():
+    """Gate projections of 2^65 and more, whose square is past 32 bits: the activation is the identity there, or zero."""
+    x = torch.tensor([[2.0 ** 40, 1.0]], dtype=torch.bfloat16)
+    wg = torch.tensor([[2.0 ** 30, 0.0], [-2.0 ** 30, 0.0], [0.0, 0.5]], dtype=torch.bfloat16)
+    wu = torch.tensor([[0.0, 2.0 ** -30]] * 3, dtype=torch.bfloat16)
+    got = []
+    for f, dev in ((P.gated_ffn, DEV), (O.gated_ffn, "cpu")):
+        leaves = [t.to(dev).requires_grad_(True) for t in (x, wg, wu)]
+        y = f(*leaves, activation="gelu")
+        got.append([y, *torch.autograd.grad([y], leaves, [torch.ones_like(y)])])
+    for n, a, b, roundings in zip(("y", "dx", "dw_gate", "dw_up"), *got, (1, 3, 3, 3)):
+        close(n, a, b, 5, roundings=roundings)
