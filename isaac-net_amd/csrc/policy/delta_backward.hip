@@ -544,16 +544,17 @@ void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
 template <typename T>
 __global__ __launch_bounds__(256) void delta_heads_kernel(const float* __restrict__ x, T* __restrict__ q,
                                                           T* __restrict__ k, int64_t rows, int K, int rep) {
-    const int64_t total = rows * K, i = (int64_t)blockIdx.x * 256 + threadIdx.x;    // rows: B T Hk
-    if (i >= total) return;
-    const int64_t row = i / K, c = i % K;
-    float sq = 0.0f, sk = 0.0f;
-    for (int r = 0; r < rep; ++r) {
-        sq += x[(row * rep + r) * K + c];
-        sk += x[total * rep + (row * rep + r) * K + c];
+    const int64_t total = rows * K;                     // rows: B T Hk
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / K, c = i % K;
+        float sq = 0.0f, sk = 0.0f;
+        for (int r = 0; r < rep; ++r) {
+            sq += x[(row * rep + r) * K + c];
+            sk += x[total * rep + (row * rep + r) * K + c];
+        }
+        q[i] = (T)sq;
+        k[i] = (T)sk;
     }
-    q[i] = (T)sq;
-    k[i] = (T)sk;
 }
 
 template <typename T, int C, int KP, bool VEC>
@@ -589,8 +590,8 @@ static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
     }
     if (d.H != d.Hk) {
         const int64_t rows = (int64_t)d.B * d.T * d.Hk;
-        hipLaunchKernelGGL(delta_heads_kernel<T>, dim3((unsigned)((rows * d.K + 255) / 256)), dim3(256), 0, st,
-                           g.head_grad, (T*)g.d_q, (T*)g.d_k, rows, d.K, d.H / d.Hk);
+        hipLaunchKernelGGL(delta_heads_kernel<T>, dim3(blocks256(rows * d.K)), dim3(256), 0, st, g.head_grad, (T*)g.d_q,
+                           (T*)g.d_k, rows, d.K, d.H / d.Hk);
     }
     return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
 }

@@ -77,9 +77,10 @@ __global__ __launch_bounds__(256) void delta_step_kernel(InetDelta d, int blocks
 
 template <typename T, int LP, int VW, int RL> static int launch(const InetDelta& d, hipStream_t st) {
     const int blocks = (d.V + LP * VW - 1) / (LP * VW);
-    const int64_t units = (int64_t)d.B * d.H * blocks;
+    const int64_t grid = ((int64_t)d.B * d.H * blocks + 3) / 4;
+    if (grid > GRID_MAX) return INET_POLICY_EUNSUPPORTED;
     auto k = delta_step_kernel<T, LP, VW, RL>;
-    hipLaunchKernelGGL(k, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, d, blocks);
+    hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), 0, st, d, blocks);
     return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
 }
 
@@ -112,8 +113,6 @@ int delta_step(const InetDelta& d, hipStream_t st) {
 }
 
 // ------------------------------------------------------------------------------------------------ C ABI
-constexpr int64_t GRID_MAX = (1 << 24) - 1;       // workgroups of 256 lanes a launch
-
 static int elem_size(int dtype) { return dtype == INET_POLICY_F32 ? 4 : 2; }
 
 static int check(const InetDelta* a) {

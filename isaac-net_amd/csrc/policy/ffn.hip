@@ -385,11 +385,11 @@ void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, O
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_pad_kernel(const T* __restrict__ in, int64_t in_s, int64_t rows, int D,
                                                       T* __restrict__ out, int D8) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * D8) return;
-    const int64_t r = i / D8;
-    const int c = (int)(i % D8);
-    out[i] = c < D ? in[r * in_s + c] : (T)0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * D8; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / D8;
+        const int c = (int)(i % D8);
+        out[i] = c < D ? in[r * in_s + c] : (T)0.0f;
+    }
 }
 
 // the shares of a product over N added up in order: out [rows][D] of parts [count][.][cols]. Memory bounds it: 17 us for both
@@ -397,17 +397,16 @@ __global__ __launch_bounds__(256) void ffn_pad_kernel(const T* __restrict__ in, 
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_add_kernel(const float* __restrict__ parts, int count, int64_t stride,
                                                       int64_t rows, int D, int cols, T* __restrict__ out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * D) return;
-    const float* p = parts + i / D * cols + i % D;
-    float x = 0.0f;
-    for (int s = 0; s < count; ++s) x += p[s * stride];
-    out[i] = (T)x;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * D; i += (int64_t)gridDim.x * 256) {
+        const float* p = parts + i / D * cols + i % D;
+        float x = 0.0f;
+        for (int s = 0; s < count; ++s) x += p[s * stride];
+        out[i] = (T)x;
+    }
 }
 
 static int64_t up8(int64_t x) { return (x + 7) & ~(int64_t)7; }
 static int64_t tiles(int64_t x, int t) { return (x + t - 1) / t; }
-static unsigned blocks256(int64_t n) { return (unsigned)((n + 255) / 256); }
 
 // The tile of a product by how many of the largest it has: 256 x 256 (eight waves, a compute unit's LDS to itself) where
 // they fill the chip's 256 compute units, else 128 x 128, else 64 x 64. Forward, us by tiles of 64, 128 and 256: 512 x 256 x 1024
@@ -549,15 +548,20 @@ template <typename T> static int run(const InetFfn& a, const InetFfnGrad* d, hip
     return INET_POLICY_OK;
 }
 
-static int check(const InetFfn* a) {
+static int check(const InetFfn* a, bool back) {
     if (!a || a->N < 0 || a->D < 1 || a->F < 1 || a->act < 0 || a->act > 2 || a->dtype < 0 || a->dtype > 2)
         return INET_POLICY_EINVAL;
     if (a->dtype == INET_POLICY_F32 || a->D > 1 << 20 || a->F > 1 << 20) return INET_POLICY_EUNSUPPORTED;
     for (int64_t s : {a->x_s, a->w_gate_s, a->w_up_s})       // (a tile's offsets are 32-bit)
         if (s < 0 || s > (int64_t)1 << 22) return INET_POLICY_EUNSUPPORTED;
     if (a->N > (int64_t)1 << 23) return INET_POLICY_EUNSUPPORTED;
-    if (tiles(a->N, 64) * tiles(a->F, 32) > (1 << 24) - 1 || tiles(a->N, 64) * tiles(a->D, 64) > (1 << 24) - 1)
+    if (tiles(a->N, 64) * tiles(a->F, 32) > GRID_MAX || tiles(a->N, 64) * tiles(a->D, 64) > GRID_MAX)
         return INET_POLICY_EUNSUPPORTED;     // (workgroups a launch)
+    if (back) {                              // (and of the weights' gradients, of 512 lanes for tiles of 256)
+        const int64_t D8 = up8(a->D), F8 = up8(a->F), big = dw_size(D8, F8) == 2 ? 2 : 1;
+        if (tiles(2 * F8, 128 * big) * tiles(D8, 128 * big) * shares(a->N, D8, F8) > GRID_MAX / big)
+            return INET_POLICY_EUNSUPPORTED;
+    }
     if (a->N == 0) return INET_POLICY_OK;
     if (!a->x || !a->w_gate || !a->w_up) return INET_POLICY_EINVAL;
     if (a->D % 8 == 0) {                      // rows are read 16 bytes at a time; other widths are padded first
@@ -591,7 +595,7 @@ int64_t inet_policy_ffn_work(int64_t N, int32_t D, int32_t F, int32_t backward) 
 }
 
 int32_t inet_policy_ffn_forward(const InetFfn* a, void* stream) {
-    if (int rc = pol::check(a)) return rc;
+    if (int rc = pol::check(a, false)) return rc;
     if (a->N == 0) return INET_POLICY_OK;
     if (!a->y) return INET_POLICY_EINVAL;
     return a->dtype == INET_POLICY_BF16 ? pol::run<__bf16>(*a, nullptr, (hipStream_t)stream)
@@ -599,7 +603,7 @@ int32_t inet_policy_ffn_forward(const InetFfn* a, void* stream) {
 }
 
 int32_t inet_policy_ffn_backward(const InetFfn* a, const InetFfnGrad* d, void* stream) {
-    if (int rc = pol::check(a)) return rc;
+    if (int rc = pol::check(a, true)) return rc;
     if (!d) return INET_POLICY_EINVAL;
     if (a->N == 0)                            // (no rows: the weights' gradients are zero)
         return a->dtype == INET_POLICY_BF16 ? pol::zero_weights<__bf16>(*a, *d, (hipStream_t)stream)

@@ -387,8 +387,9 @@ static int blocks_for(int64_t N, int rows) {
 
 template <typename T, int LP, int NJ, bool VEC> static int launch_forward(const InetNorm& a, hipStream_t st) {
     constexpr int RW = NORM_WG / LP;
-    hipLaunchKernelGGL((norm_forward_kernel<T, LP, NJ, VEC>), dim3((unsigned)((a.N + RW - 1) / RW)), dim3(NORM_WG), 0,
-                       st, a);
+    const int64_t grid = (a.N + RW - 1) / RW;
+    if (grid > GRID_MAX) return INET_POLICY_EUNSUPPORTED;
+    hipLaunchKernelGGL((norm_forward_kernel<T, LP, NJ, VEC>), dim3((unsigned)grid), dim3(NORM_WG), 0, st, a);
     return hipGetLastError() == hipSuccess ? INET_POLICY_OK : INET_POLICY_ELAUNCH;
 }
 

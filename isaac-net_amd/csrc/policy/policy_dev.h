@@ -22,6 +22,14 @@
 
 namespace pol {
 
+// workgroups of 256 lanes a launch: a grid has fewer than 2^32 lanes
+constexpr int64_t GRID_MAX = (1 << 24) - 1;
+// for `items` elements, a lane each; a kernel so launched strides over what is past the grid
+inline unsigned blocks256(int64_t items) {
+    const int64_t n = (items + 255) / 256;
+    return (unsigned)(n < GRID_MAX ? n : GRID_MAX);
+}
+
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
