@@ -23,6 +23,10 @@
 // the blocks below enter by 32-bit matrix instructions.
 //
 // The log-decays' sums are held in 64 bits: their differences stay exact to 32 bits whatever the chunk has decayed by.
+//
+// A chunk's products take every step with every other, those that may not see each other by a factor of zero, which an
+// infinity or NaN passes (0 x NaN). So where a chunk's rows X or Z are not finite, its 16 columns go by single steps
+// (steps_forward, steps_backward): what is wrong stays with its episode, and with the steps that follow it.
 #pragma once
 #include "policy_dev.h"
 #include "../../../include/inet_policy.h"
@@ -266,6 +270,8 @@ template <int RT> DEV void rows_store(const f32x4 (&x)[RT], float* __restrict__ 
 
 // keeps what is computed from x inside the loop: addresses are cheaper to compute again than to hold in registers
 DEV void keep(uint32_t& x) { asm volatile("" : "+v"(x)); }
+// the same for what is equal in all lanes
+template <typename X> DEV void keep_same(X& x) { asm volatile("" : "+s"(x)); }
 
 // tile row it of the triangles: -L (in Ln, f32, rows of ld) from K K^T, or P from Q K^T. The products are taken
 // transposed (K's rows as A), so that a lane holds four steps j of one step i. ROWS_BETA: L_ij takes beta_i, else beta_j.
@@ -374,6 +380,111 @@ template <int C> DEV void solve_up(f32x4 (&z)[C / 16], const float* ln, int ld, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] = ln[(rt * 16 + 4 * g + e) * ld + rt * 16 + n];
         z[rt] = mma32(a, acc, f32x4{});
+    }
+}
+
+// whether a chunk's rows times their factors (the write strengths: the last step's is in no other step's equation) are all
+// finite, for the whole wave
+template <int RT> DEV bool all_finite(const f32x4 (&x)[RT], const float* factor, int g) {
+    float s = 0.0f;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const f32x4 f = *(const f32x4*)(factor + rt * 16 + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += x[rt][e] * f[e] * 0.0f;              // 0, or NaN
+    }
+    return __builtin_amdgcn_ballot_w64(s != s) == 0;
+}
+
+// one step's gates: what the memory is kept by (0: emptied) and the write strength
+struct StepGate {
+    float keep, beta;
+    DEV StepGate(const InetDelta& d, int b, int h, int t) {
+        const float g = gate_load(d.g, b * d.g_s[0] + t * d.g_s[1] + h * d.g_s[2], d.gate_dtype);
+        beta = gate_load(d.beta, b * d.beta_s[0] + t * d.beta_s[1] + h * d.beta_s[2], d.gate_dtype);
+        keep = (d.reset && d.reset[b * d.reset_s[0] + t * d.reset_s[1]]) || (double)g < DECAY_MIN ? 0.0f : expf(g);
+    }
+};
+
+// a step's key or query at the lane's rows of the state. (Single steps compute their places anew each time: what they hold
+// in registers the chunks' products have to do without.)
+template <typename T, int KT> DEV void step_row(const T* p, int K, int g, f32x4 (&x)[KT]) {
+    uint32_t row = 4 * g;
+    keep(row);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t r = row + kt * 16 + e;
+            const float v = (float)p[r < (uint32_t)K ? r : 0u];
+            x[kt][e] = r < (uint32_t)K ? v : 0.0f;
+        }
+}
+// a column's sum over its rows, in four lanes
+template <int KT> DEV float column_sum(const f32x4 (&a)[KT], const f32x4 (&b)[KT]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += a[kt][e] * b[kt][e];
+    s += __shfl_xor(s, 16);
+    return s + __shfl_xor(s, 32);
+}
+
+// a chunk of up to C steps from t0 on, one by one, for a wave's 16 columns: the state after it; give(step, error, output) in a
+// lane a column (OUT: outputs wanted). k, q, v: the head's rows; col: the lane's column of v (in: there is one).
+template <int C, bool OUT, typename T, int KT, typename F>
+DEV void steps_forward(const InetDelta& d, int b, int h, int t0, const T* k, const T* q, const T* v, int64_t v_s, int col,
+                       bool in, f32x4 (&S)[KT], int g, F&& give) {
+#pragma nounroll
+    for (int t = 0; t < C && t0 + t < d.T; ++t) {
+        keep_same(b), keep_same(h), keep_same(k), keep_same(q), keep_same(v);
+        uint32_t c = in ? col : 0;
+        keep(c);
+        const StepGate gate(d, b, h, t0 + t);
+        f32x4 r[KT];
+        step_row(k + (t0 + t) * d.k_s[1], d.K, g, r);
+        const float value = in ? (float)v[(t0 + t) * v_s + c] : 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[kt][e] = gate.keep != 0.0f ? gate.keep * S[kt][e] : 0.0f;
+        const float err = value - column_sum(r, S), w = gate.beta * err;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) S[kt] += r[kt] * w;
+        float out = 0.0f;
+        if (OUT) {
+            step_row(q + (t0 + t) * d.q_s[1], d.K, g, r);
+            out = d.scale * column_sum(r, S);
+        }
+        if (g == 0) give(t, err, out);
+    }
+}
+// the same backwards: S from the gradient of the state after the chunk to that before it, give(step, Z). u: the head's rows of dO
+template <int C, typename T, int KT, typename F>
+DEV void steps_backward(const InetDelta& d, int b, int h, int t0, const T* k, const T* q, const T* u, int64_t u_s, int col,
+                        bool in, f32x4 (&S)[KT], int g, F&& give) {
+#pragma nounroll
+    for (int t = (d.T - t0 < C ? d.T - t0 : C) - 1; t >= 0; --t) {
+        keep_same(b), keep_same(h), keep_same(k), keep_same(q), keep_same(u);
+        uint32_t c = in ? col : 0;
+        keep(c);
+        const StepGate gate(d, b, h, t0 + t);
+        f32x4 r[KT];
+        const float out = in ? d.scale * (float)u[(t0 + t) * u_s + c] : 0.0f;
+        step_row(q + (t0 + t) * d.q_s[1], d.K, g, r);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) S[kt] += r[kt] * out;
+        step_row(k + (t0 + t) * d.k_s[1], d.K, g, r);
+        const float z = column_sum(r, S), w = -gate.beta * z;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float s = S[kt][e] + r[kt][e] * w;
+                S[kt][e] = gate.keep != 0.0f ? gate.keep * s : 0.0f;
+            }
+        if (g == 0) give(t, z);
     }
 }
 

@@ -15,11 +15,13 @@ template <typename T, int C, int KP> struct ForwardLds {
 // One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns. Per chunk: K, Q and the gates to LDS,
 // the triangles and the diagonal blocks' inverses by the waves in parts, then each wave's own columns through products whose
 // results are the next one's operands in its registers. Chunks are short chains, so what bounds it is how many workgroups
-// share a compute unit and wait in turn: three, within 168 registers (four, within 128, spill: 608 us for the 472 below).
+// share a compute unit and wait in turn: three, within 168 registers (four, within 128, spill: 608 us for the 480 below), but
+// two where float32's planes of 64 keys fill the LDS.
 // 16384 robots x 24 steps x 2 heads of 64 x 64, bfloat16, state in and out: 480 us for the 1.48 GB it has to move (3.1 TB/s,
 // where a copy makes 4.8) and 0.2 GB of errors kept; 300 x 77 x 6 heads of 40 x 56, float32: 109 us.
 template <typename T, int C, int KP, bool VEC>
-__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_forward_kernel(InetDelta d) {
+__global__ __launch_bounds__(DELTA_WG, 3 * sizeof(ForwardLds<T, C, KP>) <= LDS_MAX && KP <= 64 ? 3 : 2)
+void delta_forward_kernel(InetDelta d) {
     constexpr int NP = Elem<T>::planes, ORD = Elem<T>::ord, NO = ORD + 1, RT = C / 16, KT = KP / 16;
     extern __shared__ char lds_raw[];
     typedef ForwardLds<T, C, KP> Lds;
@@ -86,30 +88,38 @@ __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2) void delta_f
                 }
             }
             solve_down<C>(x, s.ln, Lds::LL, n, g);
-            if (d.err && mine) rows_store(x, d.err + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
+            if (all_finite(x, s.gates.beta, g)) {
+                if (d.err && mine) rows_store(x, d.err + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
+                for (int rt = 0; rt < RT; ++rt) x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
 #pragma unroll
-            for (int kp = 0; kp < RT / 2; ++kp) {
-                const Frag<NO> xf = split_tiles<NO>(x[2 * kp], x[2 * kp + 1]);
+                for (int kp = 0; kp < RT / 2; ++kp) {
+                    const Frag<NO> xf = split_tiles<NO>(x[2 * kp], x[2 * kp + 1]);
 #pragma unroll
-                for (int rt = 2 * kp; rt < RT; ++rt)
-                    o[rt] = mma<ORD>(P.frag(rt * 16 + n, kp * 32 + 8 * g), xf, o[rt]);
-            }
+                    for (int rt = 2 * kp; rt < RT; ++rt)
+                        o[rt] = mma<ORD>(P.frag(rt * 16 + n, kp * 32 + 8 * g), xf, o[rt]);
+                }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) tile_put(s.o + rt * 16 * LV + w * 16, LV, n, g, o[rt]);
-            const float a_end = s.gates.a_end;
+                for (int rt = 0; rt < RT; ++rt) tile_put(s.o + rt * 16 * LV + w * 16, LV, n, g, o[rt]);
+                const float a_end = s.gates.a_end;
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
+                    for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
 #pragma unroll
-            for (int kp = 0; kp < RT / 2; ++kp) {
-                const f32x4 c0 = *(const f32x4*)(s.gates.c + kp * 32 + 4 * g),
-                            c1 = *(const f32x4*)(s.gates.c + kp * 32 + 16 + 4 * g);
-                const Frag<3> xf = split_tiles<3>(x[2 * kp] * c0, x[2 * kp + 1] * c1);
+                for (int kp = 0; kp < RT / 2; ++kp) {
+                    const f32x4 c0 = *(const f32x4*)(s.gates.c + kp * 32 + 4 * g),
+                                c1 = *(const f32x4*)(s.gates.c + kp * 32 + 16 + 4 * g);
+                    const Frag<3> xf = split_tiles<3>(x[2 * kp] * c0, x[2 * kp + 1] * c1);
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), xf, S[kt]);
+                    for (int kt = 0; kt < KT; ++kt) S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), xf, S[kt]);
+                }
+            } else {
+                const int col = w * 16 + n;
+                steps_forward<C, true>(d, b, h, t0, k, q, v, d.v_s[1], col, mine, S, g, [&](int t, float err, float out) {
+                    s.o[t * LV + col] = (T)out;
+                    if (d.err && mine) d.err[rows0 + (t0 + t) * row_s + col] = err;
+                });
             }
         }
         __syncthreads();

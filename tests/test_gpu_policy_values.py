@@ -7,7 +7,7 @@ import torch
 
 import isaac_net_amd as P
 from oracle import policy_oracle as O
-from test_gpu_policy import DEV, DT, close, rand
+from test_gpu_policy import DEV, DT, NAMES, close, delta_inputs, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,80 @@ def test_gelu_far_out():
         got.append([y, *torch.autograd.grad([y], leaves, [torch.ones_like(y)])])
     for n, a, b, roundings in zip(("y", "dx", "dw_gate", "dw_up"), *got, (1, 3, 3, 3)):
         close(n, a, b, 5, roundings=roundings)
+
+
+def close_where_finite(what, x, ref, terms, **kw):
+    """As close() where the definition is finite; where it is not, x is not either."""
+    ok = torch.isfinite(ref.detach())
+    x = x.detach().cpu()
+    wrong = (torch.isfinite(x) != ok).sum().item()
+    assert not wrong, f"{what}: {wrong} of {ok.numel()} values finite where the definition is not, or the reverse"
+    close(what, torch.where(ok, x, torch.zeros_like(x)), torch.where(ok, ref, torch.zeros_like(ref)), terms, **kw)
+
+
+# the ways through a window: one chunk; several in one pass; few robots by chunks of 32 and, in bfloat16 alone, of 64; rows of
+# whole groups of eight on 16 bytes or not; one or several blocks of 64 columns
+WAYS = [("f32", 3, 24, 32, 32), ("bf16", 3, 24, 64, 64), ("f16", 3, 31, 40, 72), ("f32", 2, 70, 64, 40),
+        ("bf16", 50, 200, 32, 32), ("f16", 2, 70, 100, 17), ("f32", 2, 200, 48, 64), ("bf16", 2, 300, 128, 128),
+        ("bf16", 1, 600, 64, 64), ("bf16", 1, 530, 33, 65)]
+
+
+def outputs_where_finite(ins, reset):
+    got = P.delta_rule(*(t.to(DEV) for t in ins), reset=reset.to(DEV))
+    want = O.delta_rule(*ins, reset=reset)
+    for n, x, y in zip(NAMES, got, want):
+        close_where_finite(n, x, y, ins[0].shape[1] + ins[0].shape[3] + ins[2].shape[3])
+
+
+@pytest.mark.parametrize("what", ["state", "state_inf", "q", "k", "v", "v_inf", "g", "beta", "v_column"])
+@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
+def test_an_episode_sees_nothing_of_the_one_before(dt, B, T, K, V, what):
+    """A robot whose memory or inputs are not finite, its episode ending inside a chunk: from there on, and in the memory
+    after the window, all is as the recurrence has it, and so are the steps before the first wrong one."""
+    ins, reset, _, _ = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=34, end=0.02)
+    end = T - 7 if "state" not in what else 5
+    at = end - 6
+    reset[0] = False
+    reset[0, end] = True
+    q, k, v, g, beta, state = ins
+    if what == "state":
+        state[0, 1] = math.nan
+    elif what == "state_inf":
+        state[0, 0, 0, 0] = math.inf
+    elif what in ("q", "k", "v"):
+        {"q": q, "k": k, "v": v}[what][0, at, 0, 3] = math.nan
+    elif what == "v_inf":
+        v[0, at, 1] = math.inf
+    elif what == "g":
+        g[0, at, 1] = math.nan
+    elif what == "beta":
+        beta[0, end - 1, 1] = math.nan                 # the episode's last step: in no later one's equation
+    elif what == "v_column":
+        v[0, at, :, V - 1] = math.nan
+    outputs_where_finite(ins, reset)
+
+
+@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
+def test_steps_see_nothing_of_later_ones(dt, B, T, K, V):
+    """A window whose last steps hold no values (a robot's history that ends early): those before are as without them."""
+    ins, reset, _, _ = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=35, end=0.02)
+    for x in ins[:5]:
+        x[0, T - 5:] = math.nan
+    reset[0, T - 5:] = False
+    outputs_where_finite(ins, reset)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [24, 70, 200, 600])
+def test_a_memory_gone_wrong_is_empty_after_its_reset(dt, T):
+    """Against the same window from a sound memory: equal outputs from the reset on, up to the order of sums."""
+    ins, reset, _, _ = delta_inputs(3, T, 1, 2, 32, 32, DT[dt], seed=37, end=0.02)
+    reset[0, :6], reset[0, 5] = False, True
+    x = [t.to(DEV) for t in ins]
+    o, s = P.delta_rule(*x, reset=reset.to(DEV))
+    x[5][0] = math.nan
+    o2, s2 = P.delta_rule(*x, reset=reset.to(DEV))
+    assert torch.isnan(o2[0, :5]).all() and torch.isfinite(o2[0, 5:]).all() and torch.isfinite(s2).all()
+    assert torch.equal(o[1:], o2[1:]) and torch.equal(s[1:], s2[1:])
+    close("o", o2[0, 5:], o[0, 5:], T + 64, roundings=2)
+    close("state", s2[0], s[0], T + 64)
