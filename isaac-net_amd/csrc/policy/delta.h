@@ -396,10 +396,18 @@ template <int RT> DEV bool all_finite(const f32x4 (&x)[RT], const float* factor,
     return __builtin_amdgcn_ballot_w64(s != s) == 0;
 }
 
+// the kernel's first argument read again where it lies, so that the single steps' share of it takes no registers before
+typedef const __attribute__((address_space(4))) InetDelta SameDelta;
+DEV SameDelta& same_delta() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    keep_same(p);
+    return *(SameDelta*)p;
+}
+
 // one step's gates: what the memory is kept by (0: emptied) and the write strength
 struct StepGate {
     float keep, beta;
-    DEV StepGate(const InetDelta& d, int b, int h, int t) {
+    DEV StepGate(SameDelta& d, int b, int h, int t) {
         const float g = gate_load(d.g, b * d.g_s[0] + t * d.g_s[1] + h * d.g_s[2], d.gate_dtype);
         beta = gate_load(d.beta, b * d.beta_s[0] + t * d.beta_s[1] + h * d.beta_s[2], d.gate_dtype);
         keep = (d.reset && d.reset[b * d.reset_s[0] + t * d.reset_s[1]]) || (double)g < DECAY_MIN ? 0.0f : expf(g);
@@ -434,7 +442,7 @@ template <int KT> DEV float column_sum(const f32x4 (&a)[KT], const f32x4 (&b)[KT
 // a chunk of up to C steps from t0 on, one by one, for a wave's 16 columns: the state after it; give(step, error, output) in a
 // lane a column (OUT: outputs wanted). k, q, v: the head's rows; col: the lane's column of v (in: there is one).
 template <int C, bool OUT, typename T, int KT, typename F>
-DEV void steps_forward(const InetDelta& d, int b, int h, int t0, const T* k, const T* q, const T* v, int64_t v_s, int col,
+DEV void steps_forward(SameDelta& d, int b, int h, int t0, const T* k, const T* q, const T* v, int64_t v_s, int col,
                        bool in, f32x4 (&S)[KT], int g, F&& give) {
 #pragma nounroll
     for (int t = 0; t < C && t0 + t < d.T; ++t) {
@@ -462,7 +470,7 @@ DEV void steps_forward(const InetDelta& d, int b, int h, int t0, const T* k, con
 }
 // the same backwards: S from the gradient of the state after the chunk to that before it, give(step, Z). u: the head's rows of dO
 template <int C, typename T, int KT, typename F>
-DEV void steps_backward(const InetDelta& d, int b, int h, int t0, const T* k, const T* q, const T* u, int64_t u_s, int col,
+DEV void steps_backward(SameDelta& d, int b, int h, int t0, const T* k, const T* q, const T* u, int64_t u_s, int col,
                         bool in, f32x4 (&S)[KT], int g, F&& give) {
 #pragma nounroll
     for (int t = (d.T - t0 < C ? d.T - t0 : C) - 1; t >= 0; --t) {

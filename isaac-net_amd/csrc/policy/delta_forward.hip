@@ -88,37 +88,44 @@ void delta_forward_kernel(InetDelta d) {
                 }
             }
             solve_down<C>(x, s.ln, Lds::LL, n, g);
-            if (all_finite(x, s.gates.beta, g)) {
-                if (d.err && mine) rows_store(x, d.err + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
+            const bool sound = all_finite(x, s.gates.beta, g);
+            if (d.err && mine) rows_store(x, d.err + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
+            for (int rt = 0; rt < RT; ++rt) x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
 #pragma unroll
-                for (int kp = 0; kp < RT / 2; ++kp) {
-                    const Frag<NO> xf = split_tiles<NO>(x[2 * kp], x[2 * kp + 1]);
+            for (int kp = 0; kp < RT / 2; ++kp) {
+                const Frag<NO> xf = split_tiles<NO>(x[2 * kp], x[2 * kp + 1]);
 #pragma unroll
-                    for (int rt = 2 * kp; rt < RT; ++rt)
-                        o[rt] = mma<ORD>(P.frag(rt * 16 + n, kp * 32 + 8 * g), xf, o[rt]);
-                }
+                for (int rt = 2 * kp; rt < RT; ++rt)
+                    o[rt] = mma<ORD>(P.frag(rt * 16 + n, kp * 32 + 8 * g), xf, o[rt]);
+            }
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) tile_put(s.o + rt * 16 * LV + w * 16, LV, n, g, o[rt]);
-                const float a_end = s.gates.a_end;
+            for (int rt = 0; rt < RT; ++rt) tile_put(s.o + rt * 16 * LV + w * 16, LV, n, g, o[rt]);
+            const float a_end = s.gates.a_end;
+            f32x4 old[KT];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt) {
+                old[kt] = S[kt];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
+                for (int e = 0; e < 4; ++e) S[kt][e] = a_end != 0.0f ? a_end * S[kt][e] : 0.0f;
+            }
 #pragma unroll
-                for (int kp = 0; kp < RT / 2; ++kp) {
-                    const f32x4 c0 = *(const f32x4*)(s.gates.c + kp * 32 + 4 * g),
-                                c1 = *(const f32x4*)(s.gates.c + kp * 32 + 16 + 4 * g);
-                    const Frag<3> xf = split_tiles<3>(x[2 * kp] * c0, x[2 * kp + 1] * c1);
+            for (int kp = 0; kp < RT / 2; ++kp) {
+                const f32x4 c0 = *(const f32x4*)(s.gates.c + kp * 32 + 4 * g),
+                            c1 = *(const f32x4*)(s.gates.c + kp * 32 + 16 + 4 * g);
+                const Frag<3> xf = split_tiles<3>(x[2 * kp] * c0, x[2 * kp + 1] * c1);
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), xf, S[kt]);
-                }
-            } else {
+                for (int kt = 0; kt < KT; ++kt) S[kt] = mma<2>(Kr.tr_frag(kt, kp, n, g), xf, S[kt]);
+            }
+            if (__builtin_expect(!sound, 0)) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // (the errors are stored once more)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) S[kt] = old[kt];
                 const int col = w * 16 + n;
-                steps_forward<C, true>(d, b, h, t0, k, q, v, d.v_s[1], col, mine, S, g, [&](int t, float err, float out) {
+                SameDelta& a = same_delta();
+                steps_forward<C, true>(a, b, h, t0, k, q, v, a.v_s[1], col, mine, S, g, [&](int t, float err, float out) {
                     s.o[t * LV + col] = (T)out;
-                    if (d.err && mine) d.err[rows0 + (t0 + t) * row_s + col] = err;
+                    if (a.err && mine) a.err[rows0 + (t0 + t) * row_s + col] = err;
                 });
             }
         }

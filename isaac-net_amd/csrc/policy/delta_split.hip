@@ -165,8 +165,7 @@ template <typename T, int C, int KP, bool BACK, bool VEC>
 __global__ __launch_bounds__(2 * DELTA_WG, 2) void delta_serial_kernel(InetDelta d, const float* __restrict__ first,
                                                                    float* __restrict__ last, float* __restrict__ between,
                                                                    float* __restrict__ U, SplitWork work,
-                                                                   const T* __restrict__ rhs, int64_t rhs_b,
-                                                                   int64_t rhs_t, int64_t rhs_h) {
+                                                                   const T* __restrict__ d_o) {
     constexpr int NP = Elem<T>::planes, RT = C / 16, KT = KP / 16, LK = KP + 8, WG8 = 3 * C * (KP / 8),
                   NW = (WG8 + DELTA_WG - 1) / DELTA_WG;
     extern __shared__ char lds_raw[];
@@ -276,31 +275,41 @@ __global__ __launch_bounds__(2 * DELTA_WG, 2) void delta_serial_kernel(InetDelta
                     x[rt][e] += m[e] != 0.0f ? y[rt][e] : 0.0f;
                 }
             }
-            if (all_finite(x, s.f, g)) {
-                if (mine) rows_store(x, rows + ch * C * row_s, at_row, row_s, d.T - ch * C, g);
+            if (mine) rows_store(x, rows + ch * C * row_s, at_row, row_s, d.T - ch * C, g);
+            f32x4 old[KT];
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+            for (int kt = 0; kt < KT; ++kt) {
+                old[kt] = S[kt];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        S[kt][e] = (a_end != 0.0f ? a_end * S[kt][e] : 0.0f) + (BACK ? G[kt][e] : 0.0f);
+                for (int e = 0; e < 4; ++e)
+                    S[kt][e] = (a_end != 0.0f ? a_end * S[kt][e] : 0.0f) + (BACK ? G[kt][e] : 0.0f);
+            }
 #pragma unroll
-                for (int kp = 0; kp < RT / 2; ++kp) {
-                    const f32x4 f0 = *(const f32x4*)(s.f + kp * 32 + 4 * g),
-                                f1 = *(const f32x4*)(s.f + kp * 32 + 16 + 4 * g);
-                    const Frag<3> xf = split_tiles<3>(x[2 * kp] * f0, x[2 * kp + 1] * f1);
-                    Frag<NP> kf[KT];
+            for (int kp = 0; kp < RT / 2; ++kp) {
+                const f32x4 f0 = *(const f32x4*)(s.f + kp * 32 + 4 * g), f1 = *(const f32x4*)(s.f + kp * 32 + 16 + 4 * g);
+                const Frag<3> xf = split_tiles<3>(x[2 * kp] * f0, x[2 * kp + 1] * f1);
+                Frag<NP> kf[KT];
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) kf[kt] = Kr.tr_frag(kt, kp, n, g);
-                    mma_rows<2>(kf, xf, S);
-                }
-            } else {
-                const T *q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2], *r = rhs + b * rhs_b + h * rhs_h + c0;
+                for (int kt = 0; kt < KT; ++kt) kf[kt] = Kr.tr_frag(kt, kp, n, g);
+                mma_rows<2>(kf, xf, S);
+            }
+            if (__builtin_expect(!all_finite(x, s.f, g), 0)) {       // (asked at the end: the chain does not wait for it)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // (X is stored once more)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) S[kt] = old[kt];
+                SameDelta& a = same_delta();
                 const int col = w * 16 + n;
                 auto give = [&](int t, float e, float = 0.0f) {
                     if (mine) rows[(ch * C + t) * row_s + col] = e;
                 };
-                if (BACK) steps_backward<C>(d, b, h, ch * C, k, q, r, rhs_t, col, mine && rhs, S, g, give);
-                else steps_forward<C, false>(d, b, h, ch * C, k, q, r, rhs_t, col, mine, S, g, give);
+                const T* q = (const T*)a.q + b * a.q_s[0] + hk * a.q_s[2];
+                if (BACK) {
+                    const T* u = d_o + b * (int64_t)a.T * row_s + h * a.V + c0;
+                    steps_backward<C>(a, b, h, ch * C, k, q, u, row_s, col, mine && d_o, S, g, give);
+                } else {
+                    const T* v = (const T*)a.v + b * a.v_s[0] + h * a.v_s[2] + c0;
+                    steps_forward<C, false>(a, b, h, ch * C, k, q, v, a.v_s[1], col, mine, S, g, give);
+                }
             }
         }
         __syncthreads();
@@ -356,27 +365,28 @@ __global__ __launch_bounds__(DELTA_WG, 2) void delta_after_kernel(InetDelta d) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) o[rt] = mma<ORD>(Qr.frag(rt * 16 + n, kp * 32 + 8 * g), sf, o[rt]);
         }
-        if (all_finite(x, s.gates.beta, g)) {
+        const bool sound = all_finite(x, s.gates.beta, g);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const f32x4 a = *(const f32x4*)(s.gates.a + rt * 16 + 4 * g);
-                x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
+        for (int rt = 0; rt < RT; ++rt) {
+            const f32x4 a = *(const f32x4*)(s.gates.a + rt * 16 + 4 * g);
+            x[rt] *= *(const f32x4*)(s.gates.beta + rt * 16 + 4 * g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[rt][e] = a[e] != 0.0f ? d.scale * a[e] * o[rt][e] : 0.0f;
-            }
+            for (int e = 0; e < 4; ++e) o[rt][e] = a[e] != 0.0f ? d.scale * a[e] * o[rt][e] : 0.0f;
+        }
 #pragma unroll
-            for (int kp = 0; kp < RT / 2; ++kp) {
-                const Frag<NO> xf = split_tiles<NO>(x[2 * kp], x[2 * kp + 1]);
+        for (int kp = 0; kp < RT / 2; ++kp) {
+            const Frag<NO> xf = split_tiles<NO>(x[2 * kp], x[2 * kp + 1]);
 #pragma unroll
-                for (int rt = 2 * kp; rt < RT; ++rt) o[rt] = mma<ORD>(P.frag(rt * 16 + n, kp * 32 + 8 * g), xf, o[rt]);
-            }
+            for (int rt = 2 * kp; rt < RT; ++rt) o[rt] = mma<ORD>(P.frag(rt * 16 + n, kp * 32 + 8 * g), xf, o[rt]);
+        }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) tile_put(s.o + rt * 16 * LV + w * 16, LV, n, g, o[rt]);
-        } else {
+        for (int rt = 0; rt < RT; ++rt) tile_put(s.o + rt * 16 * LV + w * 16, LV, n, g, o[rt]);
+        if (__builtin_expect(!sound, 0)) {
             const int col = w * 16 + n;
-            steps_forward<C, true>(d, b, h, t0, (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2],
-                                   (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2],
-                                   (const T*)d.v + b * d.v_s[0] + h * d.v_s[2] + c0, d.v_s[1], col, mine, S, g,
+            SameDelta& a = same_delta();
+            steps_forward<C, true>(a, b, h, t0, (const T*)a.k + b * a.k_s[0] + hk * a.k_s[2],
+                                   (const T*)a.q + b * a.q_s[0] + hk * a.q_s[2],
+                                   (const T*)a.v + b * a.v_s[0] + h * a.v_s[2] + c0, a.v_s[1], col, mine, S, g,
                                    [&](int t, float, float out) { s.o[t * LV + col] = (T)out; });
         }
     }
@@ -402,8 +412,8 @@ static int launch(const InetDelta& d, const InetDeltaGrad* g, hipStream_t st) {
                        work);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     hipLaunchKernelGGL(serial, dim3(d.B * d.H, cols), dim3(2 * DELTA_WG), sl, st, d, BACK ? g->d_state_out : d.state,
-                       BACK ? g->d_state : d.state_out, BACK ? g->chunk_grad : d.chunk_state, U, work, rhs, rs[0],
-                       rs[1], rs[2]);
+                       BACK ? g->d_state : d.state_out, BACK ? g->chunk_grad : d.chunk_state, U, work,
+                       BACK ? rhs : nullptr);
     if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
     if (!BACK) {
         auto after = delta_after_kernel<T, C, KP, VEC>;
