@@ -8,6 +8,13 @@
 
 namespace pol {
 
+// the kernels' second argument, as same_delta()
+typedef const __attribute__((address_space(4))) InetDeltaGrad SameGrad;
+DEV SameGrad& same_grad() {
+    static_assert(sizeof(InetDelta) % alignof(InetDeltaGrad) == 0, "the arguments lie one behind the other");
+    return *(SameGrad*)(&same_delta() + 1);
+}
+
 // rows of values [steps][V] into planes in their own order, zeros up to vp columns
 template <typename T, int C, bool VEC, int N>
 DEV void stage_rows(const T* __restrict__ x, int64_t row0, int64_t row_s, int steps, int V, int vp, const Planes<N>& s) {
@@ -95,7 +102,7 @@ template <typename T, int C, int KP> struct ScanLds {
 // The state's gradient. One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns. Bound as the
 // forward pass is, by its chain of products a chunk. 300 robots x 77 steps x 6 heads of 40 x 56, float32: 108 us.
 template <typename T, int C, int KP, bool VEC>
-__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
+__global__ __launch_bounds__(DELTA_WG, 3 * sizeof(ScanLds<T, C, KP>) <= LDS_MAX && KP <= 64 ? 3 : 2)
 void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
     constexpr int NP = Elem<T>::planes, RT = C / 16, KT = KP / 16;
     extern __shared__ char lds_raw[];
@@ -141,12 +148,27 @@ void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
         if (cols) {
             f32x4 z[RT] = {}, u[RT];
             column_gradients<C, KP, NP>(S, true, z, u, s.gates, s.ln, Lds::LL, Kr, P, O, w * 16, n, g);
+            const bool sound = all_finite(z, s.gates.beta, g);
             if (mine) {
                 rows_store(z, gr.err_grad + rows0 + t0 * row_s, at_err, row_s, d.T - t0, g);
                 if (ch + 1 < chunks)
                     state_store(S, gr.chunk_grad + (bh * (chunks - 1) + ch) * d.K * d.V + c0, at, d.V, d.K, g);
             }
+            f32x4 old[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) old[kt] = S[kt];
             if (ch || gr.d_state) state_gradient<C, KP, NP>(S, z, u, s.gates, d.scale, Kr, Qr, n, g);
+            if (__builtin_expect(!sound, 0)) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // (Z is stored once more)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) S[kt] = old[kt];
+                SameDelta& a = same_delta();
+                const T* d_o = (const T*)same_grad().d_o;
+                const int col = w * 16 + n;
+                float* to = same_grad().err_grad + rows0 + t0 * row_s + col;
+                steps_backward<C>(a, b, h, t0, k, q, d_o + rows0, row_s, col, mine && d_o, S, g,
+                                  [&](int t, float x) { if (mine) to[t * row_s] = x; });
+            }
         }
         __syncthreads();
     }
@@ -160,6 +182,7 @@ template <int C> struct Parts {
 };
 template <int C> struct alignas(16) Sums {
     float ez[C], ss[4];
+    int odd[4];                                          // whether a wave's errors or Z are not all finite
 };
 
 // D and M of a chunk in LDS (as P: columns in the order perm()), in the place of X, Z and dO when those are done with
@@ -186,6 +209,7 @@ template <typename T, int C, bool VEC, int NO>
 DEV void stage_errors(const InetDelta& d, const float* z_in, T* dv, int64_t row0, int64_t row_s, int steps, int vp,
                       const Gates<C>& gates, const Planes<NO>& X, const Planes<NO>& Z, Sums<C>& sums) {
     const int lanes = vp <= 32 ? 4 : vp <= 64 ? 8 : 16;             // a row
+    float sound = 0.0f;                                             // 0, or NaN
     for (int i = threadIdx.x; i < C * lanes; i += DELTA_WG) {
         const int r = i / lanes, c = i % lanes * 8;
         float e[8] = {}, z[8] = {}, x = 0.0f;
@@ -213,10 +237,15 @@ DEV void stage_errors(const InetDelta& d, const float* z_in, T* dv, int64_t row0
             X.put4(r, c + 4, beta * e[4], beta * e[5], beta * e[6], beta * e[7]);
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x += e[u] * z[u];
+        for (int u = 0; u < 8; ++u) {
+            x += e[u] * z[u];
+            sound += beta * e[u] * 0.0f + beta * z[u] * 0.0f;
+        }
         for (int o = 1; o < lanes; o <<= 1) x += __shfl_xor(x, o);
         if (c == 0) sums.ez[r] = x;
     }
+    const bool odd = __builtin_amdgcn_ballot_w64(sound != sound) != 0;
+    if ((threadIdx.x & 63) == 0) sums.odd[threadIdx.x >> 6] = odd;
 }
 
 // eight consecutive values of a 32-bit matrix's row
@@ -224,6 +253,23 @@ DEV void row8(const float* __restrict__ p, bool in, int v, int V, bool vec, floa
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.0f;
     if (in && v < V) load8(p + v, V - v, vec, x);
+}
+
+// dg and dbeta of step t, the chunk's step i, in the gates' type (D, G: InetDelta and InetDeltaGrad wherever they lie)
+template <int C, typename D, typename G>
+DEV void put_gate_gradients(D& d, G& gr, int b, int h, int t, int i, const Gates<C>& gates, float dg, float db) {
+    const int64_t at = ((int64_t)b * d.T + t) * d.H + h;
+    if (i ? gates.seg[i] != gates.seg[i - 1] : gates.seg[0] != 0) dg = 0.0f;         // (the memory was emptied)
+    if (d.gate_dtype == INET_POLICY_F32) {
+        ((float*)gr.d_g)[at] = dg;
+        ((float*)gr.d_beta)[at] = db;
+    } else if (d.gate_dtype == INET_POLICY_BF16) {
+        ((__bf16*)gr.d_g)[at] = (__bf16)dg;
+        ((__bf16*)gr.d_beta)[at] = (__bf16)db;
+    } else {
+        ((_Float16*)gr.d_g)[at] = (_Float16)dg;
+        ((_Float16*)gr.d_beta)[at] = (_Float16)db;
+    }
 }
 
 // The gradients of q, k and the gates of one chunk, from K, Q, X, Z and dO in LDS and the state S before the chunk and its
@@ -410,21 +456,91 @@ DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int
             const int sg = __shfl_down(seg, o);
             if (lane + o < C && sg == seg) x += u;
         }
-        if (lane < C && step < d.T) {
-            const bool cut = lane ? gates.seg[lane] != gates.seg[lane - 1] : gates.seg[0] != 0;
-            const int64_t at = ((int64_t)b * d.T + step) * d.H + h;
-            const float dg = cut ? 0.0f : x, db = sums.ez[lane];
-            if (d.gate_dtype == INET_POLICY_F32) {
-                ((float*)gr.d_g)[at] = dg;
-                ((float*)gr.d_beta)[at] = db;
-            } else if (d.gate_dtype == INET_POLICY_BF16) {
-                ((__bf16*)gr.d_g)[at] = (__bf16)dg;
-                ((__bf16*)gr.d_beta)[at] = (__bf16)db;
-            } else {
-                ((_Float16*)gr.d_g)[at] = (_Float16)dg;
-                ((_Float16*)gr.d_beta)[at] = (_Float16)db;
+        if (lane < C && step < d.T) put_gate_gradients<C>(d, gr, b, h, step, lane, gates, x, sums.ez[lane]);
+    }
+}
+
+// The same by single steps, where the errors or Z are not finite (what a product would carry to steps that see nothing of them):
+// the state before each step is taken anew from that before the chunk, eight lanes a key row, 16 columns each. ROWS: four rows
+// of C in LDS.
+template <typename T, int C, int NO>
+DEV void chunk_steps(int b, int h, int t0, const Planes<NO>& Z, const Gates<C>& gates, const Sums<C>& sums, float* rows) {
+    SameDelta& d = same_delta();
+    SameGrad& gr = same_grad();
+    const int chunks = (d.T + C - 1) / C, ch = t0 / C, steps = d.T - t0 < C ? d.T - t0 : C, hk = h / (d.H / d.Hk), V = d.V;
+    const int64_t bh = (int64_t)b * d.H + h, kv = (int64_t)d.K * V, at = bh * (chunks - 1) + ch, row_s = (int64_t)d.H * V;
+    const float* S0 = ch ? d.chunk_state + (at - 1) * kv : d.state ? d.state + bh * kv : nullptr;
+    const float* dS0 = ch + 1 < chunks ? gr.chunk_grad + at * kv : gr.d_state_out ? gr.d_state_out + bh * kv : nullptr;
+    const T *k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2] + t0 * d.k_s[1],
+            *q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2] + t0 * d.q_s[1], *d_o = (const T*)gr.d_o;
+    const int64_t row0 = ((int64_t)b * d.T + t0) * row_s + h * V;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c0 = (threadIdx.x & 7) * 16;
+    for (int i = threadIdx.x; i < 4 * C; i += DELTA_WG) rows[i] = 0.0f;
+    __syncthreads();
+    for (int r0 = 0; r0 < d.K; r0 += DELTA_WG / 8) {
+        const int row = r0 + (threadIdx.x >> 3);
+        const bool in = row < d.K;
+        float S[16], dS[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) dS[u] = in && dS0 && c0 + u < V ? dS0[(int64_t)row * V + c0 + u] : 0.0f;
+#pragma nounroll
+        for (int t = steps - 1; t >= 0; --t) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) S[u] = in && S0 && c0 + u < V ? S0[(int64_t)row * V + c0 + u] : 0.0f;
+            float kv1 = 0.0f, keep = 0.0f, beta = 0.0f;
+#pragma nounroll
+            for (int j = 0; j <= t; ++j) {                // to the state before step t, as far as step t keeps it
+                const StepGate gate(d, b, h, t0 + j);
+                kv1 = in ? (float)k[j * d.k_s[1] + row] : 0.0f;
+                keep = gate.keep, beta = gate.beta;
+                const float* e = d.err + row0 + j * row_s + c0;
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    S[u] = keep != 0.0f ? keep * S[u] : 0.0f;
+                    if (j < t && c0 + u < V) S[u] += kv1 * (beta * e[u]);
+                }
+            }
+            const float qv = in ? d.scale * (float)q[t * d.q_s[1] + row] : 0.0f;
+            float dq = 0.0f, dk = 0.0f, dg = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+                if (c0 + u < V) {
+                    const int64_t v = row0 + t * row_s + c0 + u;
+                    float z = 0.0f;
+#pragma unroll
+                    for (int m = 0; m < NO; ++m) z += (float)Z.p[m * Z.plane + t * Z.ld + c0 + u];
+                    const float x = beta * d.err[v], y = beta * z, o = d_o ? (float)d_o[v] : 0.0f, ds = dS[u] + qv * o;
+                    dq += (S[u] + kv1 * x) * o;
+                    dk += ds * x - S[u] * y;
+                    const float before = ds - kv1 * y;
+                    dg += S[u] * before;
+                    dS[u] = keep != 0.0f ? keep * before : 0.0f;
+                }
+            dq *= d.scale;
+            if (!in) dg = 0.0f;
+#pragma unroll
+            for (int s = 1; s < 8; s <<= 1) {
+                dq += __shfl_xor(dq, s);
+                dk += __shfl_xor(dk, s);
+            }
+            for (int s = 1; s < 64; s <<= 1) dg += __shfl_xor(dg, s);
+            if (lane == 0) rows[w * C + t] += dg;
+            if (in && c0 == 0) {
+                const int64_t to = (((int64_t)b * d.T + t0 + t) * d.H + h) * d.K + row;
+                if (d.H == d.Hk) {
+                    ((T*)gr.d_q)[to] = (T)dq;
+                    ((T*)gr.d_k)[to] = (T)dk;
+                } else {
+                    gr.head_grad[to] = dq;
+                    gr.head_grad[(int64_t)d.B * d.T * d.H * d.K + to] = dk;
+                }
             }
         }
+    }
+    __syncthreads();
+    if (w == 0 && lane < steps) {
+        const float dg = (rows[lane] + rows[C + lane]) + (rows[2 * C + lane] + rows[3 * C + lane]);
+        put_gate_gradients<C>(d, gr, b, h, t0 + lane, lane, gates, dg, sums.ez[lane]);
     }
 }
 
@@ -465,6 +581,10 @@ void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
     __syncthreads();
     stage_errors<T, C, VEC, NO>(d, gr.err_grad, (T*)gr.d_v, row0, row_s, steps, vp, gates, X, Z, sums);
     __syncthreads();
+    if (__builtin_expect(sums.odd[0] | sums.odd[1] | sums.odd[2] | sums.odd[3], 0)) {
+        chunk_steps<T, C>(b, h, t0, Z, gates, sums, (float*)X.p);
+        return;
+    }
     const int64_t kv = (int64_t)d.K * d.V, at = bh * (chunks - 1) + ch;
     const float* S = ch ? d.chunk_state + (at - 1) * kv : d.state ? d.state + bh * kv : nullptr;
     const float* dS = ch + 1 < chunks ? gr.chunk_grad + at * kv : gr.d_state_out ? gr.d_state_out + bh * kv : nullptr;
@@ -521,19 +641,36 @@ void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
             f32x4 z[RT] = {}, u[RT], S[KT] = {};
             if (mine && gr.d_state_out) state_load(S, gr.d_state_out + bh * kv + c0, at, d.V, d.K, g);
             column_gradients<C, KP, NP>(S, gr.d_state_out != nullptr, z, u, gates, ln, LL, Kr, P, O, c0 + w * 16, n, g);
+            const bool sound = all_finite(z, gates.beta, g);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) Z.put1(rt * 16 + 4 * g + e, c0 + w * 16 + n, z[rt][e]);
-            if (gr.d_state) {
-                state_gradient<C, KP, NP>(S, z, u, gates, d.scale, Kr, Qr, n, g);
-                if (mine) state_store(S, gr.d_state + bh * kv + c0, at, d.V, d.K, g);
+            f32x4 old[KT];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) old[kt] = S[kt];
+            if (gr.d_state) state_gradient<C, KP, NP>(S, z, u, gates, d.scale, Kr, Qr, n, g);
+            if (__builtin_expect(!sound, 0)) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) S[kt] = old[kt];
+                SameDelta& a = same_delta();
+                const T* d_o = (const T*)same_grad().d_o;
+                const int col = w * 16 + n;
+                for (int r = a.T + g; r < C; r += 4) Z.put1(r, c0 + col, 0.0f);
+                steps_backward<C>(a, b, h, 0, (const T*)a.k + b * a.k_s[0] + hk * a.k_s[2],
+                                  (const T*)a.q + b * a.q_s[0] + hk * a.q_s[2], d_o + row0 + c0, row_s, col, mine && d_o, S, g,
+                                  [&](int t, float x) { Z.put1(t, c0 + col, x); });
             }
+            if (mine && gr.d_state) state_store(S, gr.d_state + bh * kv + c0, at, d.V, d.K, g);
         }
     }
     __syncthreads();
     stage_errors<T, C, VEC, NO>(d, nullptr, (T*)gr.d_v, row0, row_s, d.T, vp, gates, X, Z, sums);
     __syncthreads();
+    if (__builtin_expect(sums.odd[0] | sums.odd[1] | sums.odd[2] | sums.odd[3], 0)) {
+        chunk_steps<T, C>(b, h, 0, Z, gates, sums, (float*)X.p);
+        return;
+    }
     chunk_gradients<T, C, KP, VEC, NP, NO>(d, gr, b, h, 0, d.state ? d.state + bh * kv : nullptr,
                                            gr.d_state_out ? gr.d_state_out + bh * kv : nullptr, gates, sums, Kr, Qr, X,
                                            Z, O, rows, vp);

@@ -7,7 +7,7 @@ import torch
 
 import isaac_net_amd as P
 from oracle import policy_oracle as O
-from test_gpu_policy import DEV, DT, NAMES, close, delta_inputs, rand
+from test_gpu_policy import DEV, DT, NAMES, close, delta_both, delta_inputs, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -81,12 +81,12 @@ def outputs_where_finite(ins, reset):
         close_where_finite(n, x, y, ins[0].shape[1] + ins[0].shape[3] + ins[2].shape[3])
 
 
-@pytest.mark.parametrize("what", ["state", "state_inf", "q", "k", "v", "v_inf", "g", "beta", "v_column"])
-@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
-def test_an_episode_sees_nothing_of_the_one_before(dt, B, T, K, V, what):
-    """A robot whose memory or inputs are not finite, its episode ending inside a chunk: from there on, and in the memory
-    after the window, all is as the recurrence has it, and so are the steps before the first wrong one."""
-    ins, reset, _, _ = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=34, end=0.02)
+WRONG = ["state", "state_inf", "q", "k", "v", "v_inf", "g", "beta", "v_column"]
+
+
+def gone_wrong(dt, B, T, K, V, what):
+    """A window of whose robots the first has a memory or inputs that are not finite, its episode ending inside a chunk."""
+    ins, reset, d_o, d_s = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=34, end=0.02)
     end = T - 7 if "state" not in what else 5
     at = end - 6
     reset[0] = False
@@ -106,17 +106,29 @@ def test_an_episode_sees_nothing_of_the_one_before(dt, B, T, K, V, what):
         beta[0, end - 1, 1] = math.nan                 # the episode's last step: in no later one's equation
     elif what == "v_column":
         v[0, at, :, V - 1] = math.nan
-    outputs_where_finite(ins, reset)
+    return ins, reset, d_o, d_s
+
+
+def history_that_ends(dt, B, T, K, V):
+    """The last steps hold no values."""
+    ins, reset, d_o, d_s = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=35, end=0.02)
+    for x in ins[:5]:
+        x[0, T - 5:] = math.nan
+    reset[0, T - 5:] = False
+    return ins, reset, d_o, d_s
+
+
+@pytest.mark.parametrize("what", WRONG)
+@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
+def test_an_episode_sees_nothing_of_the_one_before(dt, B, T, K, V, what):
+    """From the reset on, and in the memory after the window, all is as the recurrence has it, and so are the steps before
+    the first wrong one."""
+    outputs_where_finite(*gone_wrong(dt, B, T, K, V, what)[:2])
 
 
 @pytest.mark.parametrize("dt,B,T,K,V", WAYS)
 def test_steps_see_nothing_of_later_ones(dt, B, T, K, V):
-    """A window whose last steps hold no values (a robot's history that ends early): those before are as without them."""
-    ins, reset, _, _ = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=35, end=0.02)
-    for x in ins[:5]:
-        x[0, T - 5:] = math.nan
-    reset[0, T - 5:] = False
-    outputs_where_finite(ins, reset)
+    outputs_where_finite(*history_that_ends(dt, B, T, K, V)[:2])
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
@@ -133,3 +145,39 @@ def test_a_memory_gone_wrong_is_empty_after_its_reset(dt, T):
     assert torch.equal(o[1:], o2[1:]) and torch.equal(s[1:], s2[1:])
     close("o", o2[0, 5:], o[0, 5:], T + 64, roundings=2)
     close("state", s2[0], s[0], T + 64)
+
+
+def check_where_finite(ins, reset, d_o, d_s):
+    a, b = delta_both(ins, reset, d_o, d_s)
+    T, K, V = ins[0].shape[1], ins[0].shape[3], ins[2].shape[3]
+    terms = sum(torch.nan_to_num((ins[i].double() * b[2 + i].double()).sum(-1), 0.0, 0.0, 0.0).norm().item() for i in (0, 1))
+    for n, x, y in zip(NAMES, a, b):
+        if n == "dg":
+            close_where_finite(n, x, y, T + K + V, size=terms,
+                               products=0.0 if ins[0].dtype == torch.float32 else 2 * 2.0 ** -16)
+        else:
+            close_where_finite(n, x, y, T + K + V)
+
+
+@pytest.mark.parametrize("what", WRONG)
+@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
+def test_gradients_of_an_episode_see_nothing_of_another(dt, B, T, K, V, what):
+    check_where_finite(*gone_wrong(dt, B, T, K, V, what))
+
+
+@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
+def test_gradients_where_a_history_ends(dt, B, T, K, V):
+    check_where_finite(*history_that_ends(dt, B, T, K, V))
+
+
+@pytest.mark.parametrize("what", ["d_o", "d_state"])
+@pytest.mark.parametrize("dt,B,T,K,V", WAYS)
+def test_a_gradient_stays_in_its_episode(dt, B, T, K, V, what):
+    ins, reset, d_o, d_s = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=36, end=0.02)
+    reset[0] = False
+    reset[0, T - 9] = True
+    if what == "d_o":
+        d_o[0, T - 5, 0] = math.nan
+    else:
+        d_s[0, 0] = math.inf
+    check_where_finite(ins, reset, d_o, d_s)
