@@ -460,79 +460,96 @@ DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int
     }
 }
 
+// eight columns of a row from c on (past the last: 0), without branches
+template <typename T> DEV void columns8(const T* p, bool in, uint32_t c, int V, float (&x)[8]) {
+    keep(c);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const bool at = in && c + u < (uint32_t)V;
+        const float v = (float)p[at ? c + u : 0u];
+        x[u] = at ? v : 0.0f;
+    }
+}
+
 // The same by single steps, where the errors or Z are not finite (what a product would carry to steps that see nothing of them):
-// the state before each step is taken anew from that before the chunk, eight lanes a key row, 16 columns each. ROWS: four rows
+// the state before each step is taken anew from that before the chunk, 16 lanes a key row, eight columns each. rows: six rows
 // of C in LDS.
 template <typename T, int C, int NO>
 DEV void chunk_steps(int b, int h, int t0, const Planes<NO>& Z, const Gates<C>& gates, const Sums<C>& sums, float* rows) {
     SameDelta& d = same_delta();
     SameGrad& gr = same_grad();
-    const int chunks = (d.T + C - 1) / C, ch = t0 / C, steps = d.T - t0 < C ? d.T - t0 : C, hk = h / (d.H / d.Hk), V = d.V;
+    const int chunks = (d.T + C - 1) / C, ch = t0 / C, steps = d.T - t0 < C ? d.T - t0 : C, hk = h / (d.H / d.Hk), K = d.K, V = d.V;
     const int64_t bh = (int64_t)b * d.H + h, kv = (int64_t)d.K * V, at = bh * (chunks - 1) + ch, row_s = (int64_t)d.H * V;
     const float* S0 = ch ? d.chunk_state + (at - 1) * kv : d.state ? d.state + bh * kv : nullptr;
     const float* dS0 = ch + 1 < chunks ? gr.chunk_grad + at * kv : gr.d_state_out ? gr.d_state_out + bh * kv : nullptr;
     const T *k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2] + t0 * d.k_s[1],
-            *q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2] + t0 * d.q_s[1], *d_o = (const T*)gr.d_o;
-    const int64_t row0 = ((int64_t)b * d.T + t0) * row_s + h * V;
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c0 = (threadIdx.x & 7) * 16;
+            *q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2] + t0 * d.q_s[1];
+    const int64_t row0 = ((int64_t)b * d.T + t0) * row_s + h * V, k_s = d.k_s[1], q_s = d.q_s[1];
+    const float scale = d.scale;
+    const float* err = d.err + row0;
+    const T* d_o = gr.d_o ? (const T*)gr.d_o + row0 : nullptr;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, c0 = (threadIdx.x & 15) * 8;
+    float *keeps = rows + 4 * C, *betas = rows + 5 * C;
     for (int i = threadIdx.x; i < 4 * C; i += DELTA_WG) rows[i] = 0.0f;
+    if ((int)threadIdx.x < steps) {
+        const StepGate gate(d, b, h, t0 + threadIdx.x);
+        keeps[threadIdx.x] = gate.keep;
+        betas[threadIdx.x] = gate.beta;
+    }
     __syncthreads();
-    for (int r0 = 0; r0 < d.K; r0 += DELTA_WG / 8) {
-        const int row = r0 + (threadIdx.x >> 3);
-        const bool in = row < d.K;
-        float S[16], dS[16];
-#pragma unroll
-        for (int u = 0; u < 16; ++u) dS[u] = in && dS0 && c0 + u < V ? dS0[(int64_t)row * V + c0 + u] : 0.0f;
+#pragma nounroll
+    for (int r0 = 0; r0 < K; r0 += DELTA_WG / 16) {
+        const int row = r0 + (threadIdx.x >> 4);
+        const bool in = row < K;
+        float S[8], dS[8], e[8], o[8];
+        columns8(dS0 ? dS0 + (int64_t)(in ? row : 0) * V : err, in && dS0, c0, V, dS);
 #pragma nounroll
         for (int t = steps - 1; t >= 0; --t) {
-#pragma unroll
-            for (int u = 0; u < 16; ++u) S[u] = in && S0 && c0 + u < V ? S0[(int64_t)row * V + c0 + u] : 0.0f;
-            float kv1 = 0.0f, keep = 0.0f, beta = 0.0f;
+            columns8(S0 ? S0 + (int64_t)(in ? row : 0) * V : err, in && S0, c0, V, S);
 #pragma nounroll
-            for (int j = 0; j <= t; ++j) {                // to the state before step t, as far as step t keeps it
-                const StepGate gate(d, b, h, t0 + j);
-                kv1 = in ? (float)k[j * d.k_s[1] + row] : 0.0f;
-                keep = gate.keep, beta = gate.beta;
-                const float* e = d.err + row0 + j * row_s + c0;
+            for (int j = 0; j < t; ++j) {                 // to the state before step t
+                const float keep = keeps[j], kb = in ? (float)k[j * k_s + row] : 0.0f, beta = betas[j];
+                columns8(err + j * row_s, true, c0, V, e);
 #pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    S[u] = keep != 0.0f ? keep * S[u] : 0.0f;
-                    if (j < t && c0 + u < V) S[u] += kv1 * (beta * e[u]);
-                }
+                for (int u = 0; u < 8; ++u) S[u] = (keep != 0.0f ? keep * S[u] : 0.0f) + kb * (beta * e[u]);
             }
-            const float qv = in ? d.scale * (float)q[t * d.q_s[1] + row] : 0.0f;
+            const float keep = keeps[t], beta = betas[t], key = in ? (float)k[t * k_s + row] : 0.0f,
+                        query = in ? scale * (float)q[t * q_s + row] : 0.0f;
+            columns8(err + t * row_s, true, c0, V, e);
+            columns8(d_o ? d_o + t * row_s : (const T*)err, d_o, c0, V, o);
             float dq = 0.0f, dk = 0.0f, dg = 0.0f;
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
-                if (c0 + u < V) {
-                    const int64_t v = row0 + t * row_s + c0 + u;
-                    float z = 0.0f;
+            for (int u = 0; u < 8; ++u) {
+                float z = 0.0f;
 #pragma unroll
-                    for (int m = 0; m < NO; ++m) z += (float)Z.p[m * Z.plane + t * Z.ld + c0 + u];
-                    const float x = beta * d.err[v], y = beta * z, o = d_o ? (float)d_o[v] : 0.0f, ds = dS[u] + qv * o;
-                    dq += (S[u] + kv1 * x) * o;
-                    dk += ds * x - S[u] * y;
-                    const float before = ds - kv1 * y;
-                    dg += S[u] * before;
-                    dS[u] = keep != 0.0f ? keep * before : 0.0f;
-                }
-            dq *= d.scale;
+                for (int m = 0; m < NO; ++m) z += (float)Z.p[m * Z.plane + t * Z.ld + (c0 < V ? c0 : 0) + u];
+                z = c0 + u < V ? z : 0.0f;
+                S[u] = keep != 0.0f ? keep * S[u] : 0.0f;
+                const float x = beta * e[u], y = beta * z, after = dS[u] + query * o[u], before = after - key * y;
+                dq += (S[u] + key * x) * o[u];
+                dk += after * x - S[u] * y;
+                dg += S[u] * before;
+                dS[u] = keep != 0.0f ? keep * before : 0.0f;
+            }
+            dq *= scale;
             if (!in) dg = 0.0f;
 #pragma unroll
-            for (int s = 1; s < 8; s <<= 1) {
+            for (int s = 1; s < 16; s <<= 1) {
                 dq += __shfl_xor(dq, s);
                 dk += __shfl_xor(dk, s);
             }
             for (int s = 1; s < 64; s <<= 1) dg += __shfl_xor(dg, s);
             if (lane == 0) rows[w * C + t] += dg;
             if (in && c0 == 0) {
-                const int64_t to = (((int64_t)b * d.T + t0 + t) * d.H + h) * d.K + row;
+                SameDelta& d = same_delta();
+                SameGrad& gr = same_grad();
+                const int64_t to = (((int64_t)b * d.T + t0 + t) * d.H + h) * K + row;
                 if (d.H == d.Hk) {
                     ((T*)gr.d_q)[to] = (T)dq;
                     ((T*)gr.d_k)[to] = (T)dk;
                 } else {
                     gr.head_grad[to] = dq;
-                    gr.head_grad[(int64_t)d.B * d.T * d.H * d.K + to] = dk;
+                    gr.head_grad[(int64_t)d.B * d.T * d.H * K + to] = dk;
                 }
             }
         }
@@ -540,7 +557,7 @@ DEV void chunk_steps(int b, int h, int t0, const Planes<NO>& Z, const Gates<C>& 
     __syncthreads();
     if (w == 0 && lane < steps) {
         const float dg = (rows[lane] + rows[C + lane]) + (rows[2 * C + lane] + rows[3 * C + lane]);
-        put_gate_gradients<C>(d, gr, b, h, t0 + lane, lane, gates, dg, sums.ez[lane]);
+        put_gate_gradients<C>(same_delta(), same_grad(), b, h, t0 + lane, lane, gates, dg, sums.ez[lane]);
     }
 }
 
@@ -549,7 +566,7 @@ DEV void chunk_steps(int b, int h, int t0, const Planes<NO>& Z, const Gates<C>& 
 // planes of 32-bit grade make three to six products of one). 300 x 77 x 6 heads of 40 x 56, float32: 162 us; 2 x 4096 x 8
 // heads of 64 x 64, bfloat16: 50 us.
 template <typename T, int C, int KP, bool VEC>
-__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
+__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? (sizeof(T) == 2 ? 5 : 3) : 2)
 void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
     constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1, LK = KP + 8;
     extern __shared__ char lds_raw[];
