@@ -185,23 +185,30 @@ template <int C> struct alignas(16) Sums {
     int odd[4];                                          // whether a wave's errors or Z are not all finite
 };
 
+// The planes that the gradients' products hold X, Z, S, dS, D and M in: as many as the outputs of q's type ask for, but three
+// (WIDE) where 16-bit q, k and v have float32 gates, whose gradients are then of 32-bit grade too. 1008 x 2774 x 1 head of 24 x
+// 24, bfloat16: chunk kernel 750 us, wide 878; 16384 x 24 x 2 heads of 64 x 64: window kernel 627, wide 790.
+template <typename T, bool WIDE> struct Grade {
+    static constexpr int ord = WIDE ? 2 : Elem<T>::ord, planes = ord + 1;
+};
+
 // D and M of a chunk in LDS (as P: columns in the order perm()), in the place of X, Z and dO when those are done with
-template <typename T, int C> struct Inner {
-    static constexpr int NO = Elem<T>::ord + 1, LC = C + 8, SIZE = 2 * NO * C * LC;
+template <int NO, int C> struct Inner {
+    static constexpr int LC = C + 8, SIZE = 2 * NO * C * LC;
     Planes<NO> D, M;
     DEV explicit Inner(__bf16* p) : D{p, LC, C * LC}, M{p + NO * C * LC, LC, C * LC} {}
 };
 
 // LDS of the chunk kernel in bytes: gates and sums, K and Q, and the rows X, Z and dO (of vp + 8) with the triangles in
 // their place at the end, Z and dO in the order in which the one-chunk kernel can have its own triangles in X's place
-template <typename T, int C> constexpr size_t rows_lds(int vp, size_t triangles) {
-    const size_t row = sizeof(__bf16) * C * (vp + 8), NP = Elem<T>::planes, NO = Elem<T>::ord + 1, x = NO * row,
-                 all = (NO + NP) * row + (x > triangles ? x : triangles), in = sizeof(__bf16) * Inner<T, C>::SIZE;
+template <typename T, int C, int NO> constexpr size_t rows_lds(int vp, size_t triangles) {
+    const size_t row = sizeof(__bf16) * C * (vp + 8), NP = Elem<T>::planes, x = NO * row,
+                 all = (NO + NP) * row + (x > triangles ? x : triangles), in = sizeof(__bf16) * Inner<NO, C>::SIZE;
     return all > in ? all : in;
 }
-template <typename T, int C, int KP> constexpr size_t chunk_lds(int vp, size_t triangles = 0) {
+template <typename T, int C, int KP, int NO> constexpr size_t chunk_lds(int vp, size_t triangles = 0) {
     return sizeof(Gates<C>) + sizeof(Sums<C>) + sizeof(__bf16) * 2 * Elem<T>::planes * C * (KP + 8) +
-           rows_lds<T, C>(vp, triangles);
+           rows_lds<T, C, NO>(vp, triangles);
 }
 
 // X = beta E, dbeta's E . Z and dV = beta Z by rows; Z from memory (err_grad) where z_in, else as it is in LDS already
@@ -281,7 +288,7 @@ DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int
                          const float* __restrict__ dS, const Gates<C>& gates, Sums<C>& sums, const Planes<NP>& Kr,
                          const Planes<NP>& Qr, const Planes<NO>& X, const Planes<NO>& Z, const Planes<NP>& O,
                          __bf16* place, int vp) {
-    constexpr int ORD = Elem<T>::ord, RT = C / 16, KT = KP / 16, KW = KT < 4 ? KT : 4, TW = 4 / KW, TN = RT / TW;
+    constexpr int ORD = NO - 1, RT = C / 16, KT = KP / 16, KW = KT < 4 ? KT : 4, TW = 4 / KW, TN = RT / TW;
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, hk = h / (d.H / d.Hk);
     const T* q = (const T*)d.q + b * d.q_s[0] + hk * d.q_s[2];
     const T* k = (const T*)d.k + b * d.k_s[0] + hk * d.k_s[2];
@@ -353,7 +360,7 @@ DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int
         }
     }
     __syncthreads();                                    // X, Z and dO are done with
-    const Inner<T, C> in(place);
+    const Inner<NO, C> in(place);
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
         const int i = it * 16 + n;
@@ -419,7 +426,7 @@ DEV void chunk_gradients(const InetDelta& d, const InetDeltaGrad& gr, int b, int
             }
         }
     }
-    static_assert(sizeof(Parts<C>) <= sizeof(__bf16) * Inner<T, C>::SIZE, "the triangles' place");
+    static_assert(sizeof(Parts<C>) <= sizeof(__bf16) * Inner<NO, C>::SIZE, "the triangles' place");
     Parts<C>& parts = *(Parts<C>*)place;
     __syncthreads();
 #pragma unroll
@@ -565,10 +572,10 @@ DEV void chunk_steps(int b, int h, int t0, const Planes<NO>& Z, const Gates<C>& 
 // of 16 x 16, then a wave a tile of 16 key columns at a time. Bound by its matrix products and the LDS reads that feed them (the
 // planes of 32-bit grade make three to six products of one). 300 x 77 x 6 heads of 40 x 56, float32: 162 us; 2 x 4096 x 8
 // heads of 64 x 64, bfloat16: 50 us.
-template <typename T, int C, int KP, bool VEC>
-__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? (sizeof(T) == 2 ? 5 : 3) : 2)
+template <typename T, int C, int KP, bool VEC, bool WIDE>
+__global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? (sizeof(T) == 2 && !WIDE ? 5 : 3) : 2)
 void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
-    constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1, LK = KP + 8;
+    constexpr int NP = Elem<T>::planes, NO = Grade<T, WIDE>::planes, LK = KP + 8;
     extern __shared__ char lds_raw[];
     const int vp = (d.V + 31) & ~31, lv = vp + 8;
     Gates<C>& gates = *(Gates<C>*)lds_raw;
@@ -610,15 +617,17 @@ void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
 
 // the one-chunk kernel's triangles P and L, in X's place until that is staged
 template <int C> constexpr size_t triangles_lds() { return sizeof(__bf16) * 3 * C * (C + 8) + sizeof(float) * C * (C + 4); }
-template <typename T, int C, int KP> constexpr size_t window_lds(int vp) { return chunk_lds<T, C, KP>(vp, triangles_lds<C>()); }
+template <typename T, int C, int KP, int NO> constexpr size_t window_lds(int vp) {
+    return chunk_lds<T, C, KP, NO>(vp, triangles_lds<C>());
+}
 
 // The whole backward pass of a window of at most C steps, one workgroup a robot and head: Z and what the scan would leave
 // stay in LDS and registers, so S, dS, q, k, v and dO are read once. 16384 robots x 24 steps x 2 heads of 64 x 64, bfloat16: 692 us
 // for 1.44 GB (2.1 TB/s); its waves wait for LDS and for each other's parts, three workgroups a compute unit.
-template <typename T, int C, int KP, bool VEC>
+template <typename T, int C, int KP, bool VEC, bool WIDE>
 __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
 void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {
-    constexpr int NP = Elem<T>::planes, NO = Elem<T>::ord + 1, LK = KP + 8, LC = C + 8, LL = C + 4, RT = C / 16,
+    constexpr int NP = Elem<T>::planes, NO = Grade<T, WIDE>::planes, LK = KP + 8, LC = C + 8, LL = C + 4, RT = C / 16,
                   KT = KP / 16;
     extern __shared__ char lds_raw[];
     const int vp = (d.V + 31) & ~31, lv = vp + 8;
@@ -711,17 +720,18 @@ __global__ __launch_bounds__(256) void delta_heads_kernel(const float* __restric
     }
 }
 
-template <typename T, int C, int KP, bool VEC>
+template <typename T, int C, int KP, bool VEC, bool WIDE>
 static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
+    constexpr int NO = Grade<T, WIDE>::planes;
     const int chunks = (d.T + C - 1) / C, vp = (d.V + 31) & ~31;
-    static_assert(chunk_lds<T, C, KP>(INET_POLICY_MAX_HEAD) <= LDS_MAX, "LDS");
+    static_assert(chunk_lds<T, C, KP, NO>(INET_POLICY_MAX_HEAD) <= LDS_MAX, "LDS");
     if (d.work) {
         if (int rc = delta_split(d, &g, VEC, st)) return rc;
     } else if constexpr (C == 32) {               // (chunks of 64 are for delta_split alone)
-        static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && window_lds<T, C, KP>(INET_POLICY_MAX_HEAD) <= LDS_MAX, "LDS");
+        static_assert(sizeof(ScanLds<T, C, KP>) <= LDS_MAX && window_lds<T, C, KP, NO>(INET_POLICY_MAX_HEAD) <= LDS_MAX, "LDS");
         if (chunks == 1) {
-            auto window = delta_window_kernel<T, C, KP, VEC>;
-            const size_t lds = window_lds<T, C, KP>(vp);
+            auto window = delta_window_kernel<T, C, KP, VEC, WIDE>;
+            const size_t lds = window_lds<T, C, KP, NO>(vp);
             if (allow_lds((const void*)window, lds)) return INET_POLICY_ELAUNCH;
             hipLaunchKernelGGL(window, dim3(d.B * d.H), dim3(DELTA_WG), lds, st, d, g);
         } else {
@@ -736,8 +746,8 @@ static int launch(const InetDelta& d, const InetDeltaGrad& g, hipStream_t st) {
     }
     if (!chunks) return INET_POLICY_OK;
     if (chunks > 1) {
-        auto chunk = delta_chunk_kernel<T, C, KP, VEC>;
-        const size_t lds = chunk_lds<T, C, KP>(vp);
+        auto chunk = delta_chunk_kernel<T, C, KP, VEC, WIDE>;
+        const size_t lds = chunk_lds<T, C, KP, NO>(vp);
         if (allow_lds((const void*)chunk, lds)) return INET_POLICY_ELAUNCH;
         hipLaunchKernelGGL(chunk, dim3(d.B * d.H * chunks), dim3(DELTA_WG), lds, st, d, g);
         if (hipGetLastError() != hipSuccess) return INET_POLICY_ELAUNCH;
@@ -754,7 +764,10 @@ int delta_backward(const InetDelta& d, const InetDeltaGrad& g, bool vec, hipStre
     return delta_dispatch(d, [&](auto t, auto c, auto kp) {
         typedef typename decltype(t)::type T;
         constexpr int C = decltype(c)::value, KP = decltype(kp)::value;
-        return vec ? launch<T, C, KP, true>(d, g, st) : launch<T, C, KP, false>(d, g, st);
+        if constexpr (!std::is_same<T, float>::value)
+            if (d.gate_dtype == INET_POLICY_F32)
+                return vec ? launch<T, C, KP, true, true>(d, g, st) : launch<T, C, KP, false, true>(d, g, st);
+        return vec ? launch<T, C, KP, true, false>(d, g, st) : launch<T, C, KP, false, false>(d, g, st);
     });
 }
 

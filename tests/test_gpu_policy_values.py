@@ -181,3 +181,16 @@ def test_a_gradient_stays_in_its_episode(dt, B, T, K, V, what):
     else:
         d_s[0, 0] = math.inf
     check_where_finite(ins, reset, d_o, d_s)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("B,T,K,V", [(3, 24, 64, 64), (2, 33, 32, 40), (40, 70, 128, 128), (2, 200, 100, 64), (2, 600, 64, 128)])
+def test_gates_of_32_bits_have_gradients_of_32_bits(dt, B, T, K, V):
+    """dg and dbeta are of the gates' type: beside 16-bit q, k and v they are as exact as those of the same values in
+    float32: at most four times their distance, which is the order of sums, of other lengths in chunks of other sizes."""
+    ins, reset, d_o, d_s = delta_inputs(B, T, 1, 2, K, V, DT[dt], seed=33, end=0.02, gate_dt=torch.float32)
+    narrow, want = delta_both(ins, reset, d_o, d_s)
+    wide, _ = delta_both([t.float() for t in ins], reset, d_o.float(), d_s)
+    for i in (5, 6):
+        off = [(x[i].double().cpu() - want[i]).norm().item() for x in (narrow, wide)]
+        assert narrow[i].dtype == torch.float32 and off[0] <= 4 * off[1], (NAMES[i], off, want[i].norm().item())
