@@ -3,7 +3,8 @@
 //
 // Forward: a workgroup computes a tile of both projections from one pass over its rows of x, and the activation and the
 // product in registers; neither projection goes to memory. Backward: the same tile again from x, then da = dy u act'(a)
-// and du = dy act(a), rounded to the type; then
+// and du = dy act(a), rounded to the type (half the bytes and the matrix instructions' rate for the two products that follow,
+// for one rounding more in their sums; float16's range: Range below); then
 //     dx = [da du] [Wg; Wu]        a product over 2 F,        dWg = da^T x,  dWu = du^T x     products over N.
 // All are one product (Product): tiles of 64 along the sum go to LDS, the next one on its way from memory while the present
 // one is computed with, and a matrix whose rows lie across the sum (W for dx, x and da for dW) is transposed by the LDS
@@ -249,6 +250,32 @@ template <int ACT> DEV void activation(float a, float& h, float& dh) {
     }
 }
 
+// da and du in float16 keep to its range: each workgroup leaves the largest of its finite values, and where the largest of all
+// is past 65504, or so small (below 2^-4) that the usual ones would lose bits below 2^-14, the tiles are computed once more,
+// scaled by the power of two that takes it to 2^14 .. 2^15; the products' results are scaled back. Bfloat16 has the range of 32
+// bits. 16383 x 504 x 1352: 4.8 us for the launch that finds nothing to do, 89 for the tiles again.
+struct Range {
+    static constexpr int TOPS = 1024;        // more than a launch's workgroups: 256 that go on, or four times the fewer than 256
+                                             // tiles of the next size
+    static bool __device__ in(float top) { return top == 0.0f || (top >= 0.0625f && top <= 65504.0f); }
+    static float __device__ scale(float top) {
+        const int e = 14 - ilogbf(top);
+        return ldexpf(1.0f, e < -120 ? -120 : e > 120 ? 120 : e);
+    }
+};
+
+// the largest of a workgroup's values, in all lanes (s: a word a wave)
+template <int THREADS> DEV float workgroup_max(float x, float* s) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) x = fmaxf(x, s[w]);
+    return x;
+}
+
 struct FfnShape {
     int64_t N, y_s;
     int D8, F, F8;
@@ -262,10 +289,22 @@ struct FfnShape {
 template <typename T, typename P, int ACT, bool BACK>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __restrict__ y, const T* __restrict__ dy,
-                      int64_t dy_s, T* __restrict__ da) {
+                      int64_t dy_s, T* __restrict__ da, float* __restrict__ tops, bool again) {
     extern __shared__ char lds_raw[];
     constexpr int COLS = P::BN / 2, RT = P::RT, CT = P::CT;
+    constexpr bool RANGED = BACK && std::is_same<T, _Float16>::value;
     T* const lds = (T*)lds_raw;
+    float top = 0.0f, scale = 1.0f;
+    if constexpr (RANGED)
+        if (again) {
+            for (unsigned i = threadIdx.x; i < gridDim.x; i += P::THREADS) top = fmaxf(top, tops[i]);
+            top = workgroup_max<P::THREADS>(top, (float*)lds_raw);
+            const bool in = Range::in(top);
+            if (!in) scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, Range::scale(top))));
+            if (blockIdx.x == 0 && threadIdx.x == 0) tops[Range::TOPS] = 1.0f / scale;
+            if (in) return;
+            __syncthreads();
+        }
     const int64_t row_tiles = (p.N + P::BM - 1) / P::BM;
     const int col_tiles = (p.F + COLS - 1) / COLS, steps = (p.D8 + BK - 1) / BK;
     const int64_t total = row_tiles * col_tiles;
@@ -334,6 +373,15 @@ void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __r
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (!WHOLE && col + e >= cols) x1[e] = x2[e] = 0.0f;
+                    if constexpr (RANGED) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float m = fmaxf(fabsf(x1[e]), fabsf(x2[e]));
+                            top = m < INFINITY ? fmaxf(top, m) : top;
+                        }
+                        x1 *= scale;
+                        x2 *= scale;
+                    }
                     put_row4<WHOLE>(out + (int64_t)row * 2 * p.F8, col, cols8, true, x1);
                     put_row4<WHOLE>(out + (int64_t)row * 2 * p.F8 + p.F8, col, cols8, true, x2);
                 }
@@ -343,6 +391,11 @@ void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __r
     if (rows == P::BM && COLS <= cols && p.vec_y) finish(std::true_type{});
     else finish(std::false_type{});
     }
+    if constexpr (RANGED)
+        if (!again) {
+            top = workgroup_max<P::THREADS>(top, (float*)lds_raw);
+            if (threadIdx.x == 0) tops[blockIdx.x] = top;
+        }
 }
 
 // C [rows][cols] = a b (+ a2 b2 where there are such), or shares of the sum each to a C of its own. At the sizes above: dx
@@ -351,7 +404,8 @@ void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __r
 template <typename T, typename P, bool RA, bool CA, typename O>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, Operand<T, CA> b2, int64_t K,
-                        int64_t share, O* __restrict__ C, int64_t rows, int64_t cols, bool vec) {
+                        int64_t share, O* __restrict__ C, int64_t rows, int64_t cols, bool vec,
+                        const float* __restrict__ unscale) {
     extern __shared__ char lds_raw[];
     int64_t rt;
     int ct, part;
@@ -360,6 +414,13 @@ void ffn_product_kernel(Operand<T, RA> a, Operand<T, CA> b, Operand<T, RA> a2, O
     const int64_t from = part * share, to = from + share < K ? from + share : K;
     f32x4 acc[P::CT][P::RT] = {};
     P::run(a, b, a2, b2, r0, c0, from, to, (T*)lds_raw, acc);
+    if constexpr (std::is_same<O, _Float16>::value) {
+        const float f = *unscale;
+#pragma unroll
+        for (int c = 0; c < P::CT; ++c)
+#pragma unroll
+            for (int r = 0; r < P::RT; ++r) acc[c][r] *= f;
+    }
     C += part * rows * cols;
     const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, wr = wv / P::WC, wc = wv % P::WC;
     auto finish = [&](auto whole) {
@@ -396,12 +457,14 @@ __global__ __launch_bounds__(256) void ffn_pad_kernel(const T* __restrict__ in, 
 // weights at 131072 x 512 x 2048 (8 shares, 72 MB, from the L2s in part)
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_add_kernel(const float* __restrict__ parts, int count, int64_t stride,
-                                                      int64_t rows, int D, int cols, T* __restrict__ out) {
+                                                      int64_t rows, int D, int cols, T* __restrict__ out,
+                                                      const float* __restrict__ unscale) {
+    const float f = unscale ? *unscale : 1.0f;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * D; i += (int64_t)gridDim.x * 256) {
         const float* p = parts + i / D * cols + i % D;
         float x = 0.0f;
         for (int s = 0; s < count; ++s) x += p[s * stride];
-        out[i] = (T)x;
+        out[i] = (T)(x * f);
     }
 }
 
@@ -438,7 +501,7 @@ static int shares(int64_t N, int64_t D8, int64_t F8) {
 
 // the workspace's parts, in bytes from its start
 struct Work {
-    int64_t x, wg, wu, da, parts, bytes;
+    int64_t x, wg, wu, da, parts, tops, bytes;
     Work(int64_t N, int64_t D, int64_t F, bool back) {
         const int64_t D8 = up8(D), F8 = up8(F);
         int64_t at = 0;
@@ -453,6 +516,7 @@ struct Work {
         wu = take(pad ? F * D8 * 2 : 0);
         da = take(back ? N * 2 * F8 * 2 : 0);
         parts = take(back ? (int64_t)shares(N, D8, F8) * 2 * F8 * D8 * 4 : 0);
+        tops = take(back ? (Range::TOPS + 1) * 4 : 0);
         bytes = at;
     }
 };
@@ -469,14 +533,17 @@ static bool allow_lds(const void* kernel, int bytes) {
 
 template <typename T, int ACT, bool BACK>
 static int gates(const FfnShape& p, const Operand<T, true>& x, const Operand<T, true>& w, T* y, const T* dy, int64_t dy_s,
-                 T* da, hipStream_t st) {
+                 T* da, float* tops, hipStream_t st) {
     return by_size(size_for(p.N, 2 * (int64_t)p.F), [&](auto size) {
         typedef Sized<T, decltype(size)::value, true, true, true> P;
         auto k = ffn_gates_kernel<T, P, ACT, BACK>;
         if (!allow_lds((const void*)k, P::LDS)) return INET_POLICY_ELAUNCH;
         const int64_t all = tiles(p.N, P::BM) * tiles(p.F, P::BN / 2), grid = P::THREADS == 512 && all > 256 ? 256 : all;
-        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(P::THREADS), P::LDS, st, p, x, w, y, dy, dy_s, da);
-        LAUNCHED;
+        const bool ranged = BACK && std::is_same<T, _Float16>::value;
+        for (int again = 0; again <= (ranged ? 1 : 0); ++again) {
+            hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(P::THREADS), P::LDS, st, p, x, w, y, dy, dy_s, da, tops, again != 0);
+            LAUNCHED;
+        }
         return INET_POLICY_OK;
     });
 }
@@ -488,13 +555,14 @@ template <typename T, bool BACK, typename... A> static int gates_for(int act, co
 template <typename T, bool RA, bool CA, typename O>
 static int product(int size, const Operand<T, RA>& a, const Operand<T, CA>& b, const Operand<T, RA>& a2,
                    const Operand<T, CA>& b2, int64_t K, int count, int64_t share, O* C,
-                   int64_t rows, int64_t cols, bool vec, hipStream_t st) {
+                   int64_t rows, int64_t cols, bool vec, const float* unscale, hipStream_t st) {
     return by_size(size, [&](auto sz) {
         typedef Sized<T, decltype(sz)::value, RA, CA, false> P;
         auto k = ffn_product_kernel<T, P, RA, CA, O>;
         if (!allow_lds((const void*)k, P::LDS)) return INET_POLICY_ELAUNCH;
         const int64_t grid = tiles(rows, P::BM) * tiles(cols, P::BN);
-        hipLaunchKernelGGL(k, dim3((unsigned)(grid * count)), dim3(P::THREADS), P::LDS, st, a, b, a2, b2, K, share, C, rows, cols, vec);
+        hipLaunchKernelGGL(k, dim3((unsigned)(grid * count)), dim3(P::THREADS), P::LDS, st, a, b, a2, b2, K, share, C, rows,
+                           cols, vec, unscale);
         LAUNCHED;
         return INET_POLICY_OK;
     });
@@ -520,14 +588,16 @@ template <typename T> static int run(const InetFfn& a, const InetFfnGrad* d, hip
     }
     auto by4 = [](const void* p, int64_t s) { return (uintptr_t)p % 8 == 0 && s % 4 == 0; };
     FfnShape p{a.N, a.y_s, D8, a.F, F8, d ? by4(d->d_y, d->d_y_s) : by4(a.y, a.y_s)};
-    if (!d) return gates_for<T, false>(a.act, p, x, w, (T*)a.y, (const T*)nullptr, 0, (T*)nullptr, st);
+    if (!d) return gates_for<T, false>(a.act, p, x, w, (T*)a.y, (const T*)nullptr, 0, (T*)nullptr, (float*)nullptr, st);
     T* da = (T*)(work + at.da);
-    if (int rc = gates_for<T, true>(a.act, p, x, w, (T*)nullptr, (const T*)d->d_y, d->d_y_s, da, st)) return rc;
+    float* tops = (float*)(work + at.tops);
+    const float* unscale = std::is_same<T, _Float16>::value ? tops + Range::TOPS : nullptr;
+    if (int rc = gates_for<T, true>(a.act, p, x, w, (T*)nullptr, (const T*)d->d_y, d->d_y_s, da, tops, st)) return rc;
     if (d->d_x) {
         const Operand<T, true> dg{da, nullptr, 2 * F8, 0, a.N}, du{da + F8, nullptr, 2 * F8, 0, a.N};
         const Operand<T, false> wg{w.p, nullptr, w.st, 0, D8}, wu{w.p2, nullptr, w.st2, 0, D8};
         if (int rc = product<T, true, false, T>(size_for(a.N, D8), dg, wg, du, wu, a.F, 1, F8, (T*)d->d_x, a.N, a.D,
-                                                by4(d->d_x, a.D), st))
+                                                by4(d->d_x, a.D), unscale, st))
             return rc;
     }
     if (d->d_w_gate || d->d_w_up) {
@@ -535,13 +605,14 @@ template <typename T> static int run(const InetFfn& a, const InetFfnGrad* d, hip
         const int s = shares(a.N, D8, F8);
         const int64_t share = (tiles(a.N, s) + BK - 1) / BK * BK, one = (int64_t)2 * F8 * D8;
         float* parts = (float*)(work + at.parts);
-        if (int rc = product<T, false, false, float>(dw_size(D8, F8), dat, xt, no, no, a.N, s, share, parts, 2 * F8, D8, true, st))
+        if (int rc = product<T, false, false, float>(dw_size(D8, F8), dat, xt, no, no, a.N, s, share, parts, 2 * F8, D8, true,
+                                                      nullptr, st))
             return rc;
         for (int m = 0; m < 2; ++m) {
             T* out = (T*)(m ? d->d_w_up : d->d_w_gate);
             if (!out) continue;
             hipLaunchKernelGGL(ffn_add_kernel<T>, dim3(blocks256((int64_t)a.F * a.D)), dim3(256), 0, st,
-                               parts + (int64_t)m * F8 * D8, s, one, (int64_t)a.F, a.D, D8, out);
+                               parts + (int64_t)m * F8 * D8, s, one, (int64_t)a.F, a.D, D8, out, unscale);
             LAUNCHED;
         }
     }
@@ -579,7 +650,7 @@ template <typename T> static int zero_weights(const InetFfn& a, const InetFfnGra
     for (void* out : {d.d_w_gate, d.d_w_up})
         if (out) {
             hipLaunchKernelGGL(ffn_add_kernel<T>, dim3(blocks256(one)), dim3(256), 0, st, (const float*)nullptr, 0,
-                               (int64_t)0, (int64_t)a.F, a.D, a.D, (T*)out);
+                               (int64_t)0, (int64_t)a.F, a.D, a.D, (T*)out, (const float*)nullptr);
             LAUNCHED;
         }
     return INET_POLICY_OK;

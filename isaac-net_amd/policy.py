@@ -329,7 +329,8 @@ def gated_ffn(x, w_gate, w_up, activation="silu"):
     """The gated feed-forward: activation(x @ w_gate.T) * (x @ w_up.T) in one kernel, sums in 32 bits.
 
     x [..., D], w_gate and w_up [F, D] (torch.nn.Linear's layout), all bfloat16 or all float16; activation "silu",
-    "gelu" (the tanh form) or "relu". Returns [..., F] of x's type. The backward pass computes the projections again."""
+    "gelu" (the tanh form) or "relu". Returns [..., F] of x's type. The backward pass computes the projections again; their
+    gradients are rounded once to x's type before the products over them (float16's scaled into its range as needed)."""
     _on_gpu(x=x, w_gate=w_gate, w_up=w_up)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r}: one of {ACTIVATIONS}")

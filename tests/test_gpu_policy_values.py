@@ -194,3 +194,49 @@ def test_gates_of_32_bits_have_gradients_of_32_bits(dt, B, T, K, V):
     for i in (5, 6):
         off = [(x[i].double().cpu() - want[i]).norm().item() for x in (narrow, wide)]
         assert narrow[i].dtype == torch.float32 and off[0] <= 4 * off[1], (NAMES[i], off, want[i].norm().item())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("N,D,F", [(20, 32, 48), (33, 7, 50), (300, 72, 136), (2100, 520, 1032)])
+@pytest.mark.parametrize("of", ["x", "weights"])
+def test_ffn_float16_gradients_through_larger_ones(N, D, F, act, of):
+    """The gradients of the projections, up to eight times past 65504, between finite ones: small weights for dx, small
+    inputs for those of the weights. (gelu's and silu's gate times its own size: h is a for a > 0.)"""
+    gen = torch.Generator().manual_seed(32)
+    w_size, x_size = (2.0 ** -9, 2.0 ** 13) if of == "x" else (2.0 ** 7, 2.0 ** -8)
+    big = 64.0 * 4096.0 / (w_size * x_size * math.sqrt(D))             # |dy| |h| of 2^18 at |a| of its usual size
+    x = (x_size * rand(gen, N, D)).half()
+    w = [(w_size * rand(gen, F, D)).half() for _ in range(2)]
+    # few robots and columns with such gradients, so that their sums, rounded to float16, are finite
+    d = torch.zeros(N, F)
+    d[::max(1, N // 8), ::max(1, F // 8)] = big
+    d = d.clamp(max=60000.0).half()
+    got = []
+    for f, dev in ((P.gated_ffn, DEV), (O.gated_ffn, "cpu")):
+        leaves = [t.to(dev) for t in (x, *w)]
+        want = leaves[:1] if of == "x" else leaves[1:]
+        for t in want:
+            t.requires_grad_(True)
+        y = f(*leaves, activation=act)
+        got.append(torch.autograd.grad([y], want, [d.to(y)]))
+    for a, b in zip(*got):
+        assert b.abs().max() < 65504
+        close(of, a, b, F + D if of == "x" else N + D, roundings=3)
+
+
+@pytest.mark.parametrize("act", ["silu", "relu"])
+@pytest.mark.parametrize("N,D,F", [(20, 32, 48), (300, 72, 136), (2100, 520, 1032)])
+def test_ffn_float16_gradients_through_smaller_ones(N, D, F, act):
+    """The gradients of the projections around 2^-21, where float16 has three bits: those of the weights, of inputs around
+    2^6, have all of theirs."""
+    gen = torch.Generator().manual_seed(39)
+    x = (2.0 ** 6 * rand(gen, N, D)).half()
+    w = [(2.0 ** -6 / math.sqrt(D) * rand(gen, F, D)).half() for _ in range(2)]
+    d = (2.0 ** -20 * torch.sign(rand(gen, N, F))).half()
+    got = []
+    for f, dev in ((P.gated_ffn, DEV), (O.gated_ffn, "cpu")):
+        leaves = [x.to(dev), *(t.to(dev).requires_grad_(True) for t in w)]
+        y = f(*leaves, activation=act)
+        got.append(torch.autograd.grad([y], leaves[1:], [d.to(y)]))
+    for n, a, b in zip(("dw_gate", "dw_up"), *got):
+        close(n, a, b, N + D, roundings=3)
