@@ -399,8 +399,6 @@ class _BlockNorm(torch.autograd.Function):
         if pre is not None and d_n is None:      # (n took no part: its weight's gradient is zero)
             a.pre_weight = d.d_pre_weight = None
             dpre.zero_()
-            if f is None:
-                return d_y, None, None, None, None, dpre, None
         _call(lib.inet_policy_norm_backward, dev.index, "block_norm backward", C.byref(a), C.byref(d))
         return dx, df, dgate, dscale, dpost, dpre, None
 
