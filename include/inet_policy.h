@@ -4,8 +4,9 @@
  *
  * One robot is one row of the batch (E envs x R robots of an engine). Conventions, as inet_nr.h: the caller owns every
  * device buffer and workspace; nothing is allocated and the host never waits; work goes on `stream`; every entry point
- * returns 0 or a negative INET_POLICY_E* code, checked before any launch; no entry point throws. A batch, a window or
- * a row count of zero is valid and launches nothing.
+ * returns 0 or a negative INET_POLICY_E* code; sizes, types and pointers are checked before any launch; no entry point
+ * throws. A batch, a window or a row count of zero is valid: what is written is then the state as it was and the weights'
+ * gradients, zeros.
  */
 #ifndef INET_POLICY_H
 #define INET_POLICY_H
@@ -46,7 +47,8 @@ extern "C" {
  */
 typedef struct InetDelta {
     int32_t B, T, Hk, H, K, V;
-    int32_t dtype, gate_dtype;                  /* of q, k, v, o and their gradients; of g, beta and theirs */
+    int32_t dtype, gate_dtype;                  /* of q, k, v, o and their gradients; of g, beta and theirs (float32 ones
+                                                   are of 32-bit grade whatever dtype is) */
     float scale;
     int32_t chunk;                              /* steps a chunk: inet_policy_delta_chunk(), for both directions */
     int64_t q_s[3], k_s[3], v_s[3], g_s[3], beta_s[3], reset_s[2];

@@ -100,7 +100,7 @@ template <typename T, int C, int KP> struct ScanLds {
 };
 
 // The state's gradient. One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns. Bound as the
-// forward pass is, by its chain of products a chunk. 300 robots x 77 steps x 6 heads of 40 x 56, float32: 108 us.
+// forward pass is, by its chain of products a chunk. 300 robots x 77 steps x 6 heads of 40 x 56, float32: 113 us.
 template <typename T, int C, int KP, bool VEC>
 __global__ __launch_bounds__(DELTA_WG, 3 * sizeof(ScanLds<T, C, KP>) <= LDS_MAX && KP <= 64 ? 3 : 2)
 void delta_scan_kernel(InetDelta d, InetDeltaGrad gr) {
@@ -187,7 +187,8 @@ template <int C> struct alignas(16) Sums {
 
 // The planes that the gradients' products hold X, Z, S, dS, D and M in: as many as the outputs of q's type ask for, but three
 // (WIDE) where 16-bit q, k and v have float32 gates, whose gradients are then of 32-bit grade too. 1008 x 2774 x 1 head of 24 x
-// 24, bfloat16: chunk kernel 750 us, wide 878; 16384 x 24 x 2 heads of 64 x 64: window kernel 627, wide 790.
+// 24, bfloat16: chunk kernel 750 us, wide 878; 16384 x 24 x 2 heads of 64 x 64: window kernel 627, wide 790 (in turn, in
+// one run).
 template <typename T, bool WIDE> struct Grade {
     static constexpr int ord = WIDE ? 2 : Elem<T>::ord, planes = ord + 1;
 };
@@ -570,8 +571,8 @@ DEV void chunk_steps(int b, int h, int t0, const Planes<NO>& Z, const Gates<C>& 
 
 // The gradients of q, k and the gates, one workgroup a chunk, robot and head: X, Z and dO as planes in LDS, D and M by tiles
 // of 16 x 16, then a wave a tile of 16 key columns at a time. Bound by its matrix products and the LDS reads that feed them (the
-// planes of 32-bit grade make three to six products of one). 300 x 77 x 6 heads of 40 x 56, float32: 162 us; 2 x 4096 x 8
-// heads of 64 x 64, bfloat16: 50 us.
+// planes of 32-bit grade make three to six products of one). 300 x 77 x 6 heads of 40 x 56, float32: 169 us; 2 x 4096 x 8
+// heads of 64 x 64, bfloat16: 52 us.
 template <typename T, int C, int KP, bool VEC, bool WIDE>
 __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? (sizeof(T) == 2 && !WIDE ? 5 : 3) : 2)
 void delta_chunk_kernel(InetDelta d, InetDeltaGrad gr) {
@@ -622,8 +623,8 @@ template <typename T, int C, int KP, int NO> constexpr size_t window_lds(int vp)
 }
 
 // The whole backward pass of a window of at most C steps, one workgroup a robot and head: Z and what the scan would leave
-// stay in LDS and registers, so S, dS, q, k, v and dO are read once. 16384 robots x 24 steps x 2 heads of 64 x 64, bfloat16: 692 us
-// for 1.44 GB (2.1 TB/s); its waves wait for LDS and for each other's parts, three workgroups a compute unit.
+// stay in LDS and registers, so S, dS, q, k, v and dO are read once. 16384 robots x 24 steps x 2 heads of 64 x 64, bfloat16: 700 us
+// for 1.44 GB (2.1 TB/s); its waves wait for LDS and for each other's parts, four workgroups a compute unit.
 template <typename T, int C, int KP, bool VEC, bool WIDE>
 __global__ __launch_bounds__(DELTA_WG, C == 32 && KP <= 64 ? 3 : 2)
 void delta_window_kernel(InetDelta d, InetDeltaGrad gr) {

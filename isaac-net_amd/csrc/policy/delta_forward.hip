@@ -15,10 +15,10 @@ template <typename T, int C, int KP> struct ForwardLds {
 // One workgroup of four waves per robot, head and 64 columns; wave w owns 16 columns. Per chunk: K, Q and the gates to LDS,
 // the triangles and the diagonal blocks' inverses by the waves in parts, then each wave's own columns through products whose
 // results are the next one's operands in its registers. Chunks are short chains, so what bounds it is how many workgroups
-// share a compute unit and wait in turn: three, within 168 registers (four, within 128, spill: 608 us for the 480 below), but
+// share a compute unit and wait in turn: three, within 168 registers (four, within 128, spill: 608 us for the 485 below), but
 // two where float32's planes of 64 keys fill the LDS.
-// 16384 robots x 24 steps x 2 heads of 64 x 64, bfloat16, state in and out: 480 us for the 1.48 GB it has to move (3.1 TB/s,
-// where a copy makes 4.8) and 0.2 GB of errors kept; 300 x 77 x 6 heads of 40 x 56, float32: 109 us.
+// 16384 robots x 24 steps x 2 heads of 64 x 64, bfloat16, state in and out: 485 us for the 1.48 GB it has to move (3.1 TB/s,
+// where a copy makes 4.8) and 0.2 GB of errors kept; 300 x 77 x 6 heads of 40 x 56, float32: 116 us.
 template <typename T, int C, int KP, bool VEC>
 __global__ __launch_bounds__(DELTA_WG, 3 * sizeof(ForwardLds<T, C, KP>) <= LDS_MAX && KP <= 64 ? 3 : 2)
 void delta_forward_kernel(InetDelta d) {

@@ -9,8 +9,8 @@
 //
 // The scan is the only part that is serial: two products a chunk, its operands double-buffered in LDS; it is bound by the
 // latency of that chain, the other parts by their own products. 2 robots x 4096 steps x 8 heads of 64 x 64, bfloat16, 64 chunks,
-// us: before 24, scan 163 (2.5 a chunk), after 19; backward 46, 192 (3.0 a chunk) and the chunks' gradients 50. In one pass
-// the forward takes 607. 4 x 2048 x 8 heads of 128 x 128: 73, 133, 44; 102, 185, 190.
+// us: before 25, scan 174 (2.7 a chunk), after 20; backward 46, 198 (3.1 a chunk) and the chunks' gradients 52. In one pass
+// the forward takes 607. 4 x 2048 x 8 heads of 128 x 128: 74, 140, 45; 101, 191, 194.
 #include "delta.h"
 #include "delta_launch.h"
 

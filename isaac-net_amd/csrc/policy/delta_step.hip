@@ -3,7 +3,7 @@
 // What bounds it is the state: 8 K V bytes a head, read and written once, against 6 K V operations. A wave takes one
 // head's block of columns into its registers: LP lanes across the columns, VW each (one 16-byte load), 64 / LP rows at
 // a time, RL such loads a lane; the sums over the rows are taken in the lane and then across the row groups.
-// 131072 robots x 2 heads of 64 x 64: 1591 us for 8.73 GB, 5.5 TB/s; 512 robots x 2 heads of 32 x 32: 5.2 us, a launch and one
+// 131072 robots x 2 heads of 64 x 64: 1598 us for 8.73 GB, 5.5 TB/s; 512 robots x 2 heads of 32 x 32: 5.1 us, a launch and one
 // round trip to memory.
 #include "delta.h"
 #include "delta_launch.h"
@@ -128,16 +128,24 @@ static int check(const InetDelta* a) {
 // by chunks of 32 three share a compute unit, by 64 two. 2048 robots of 4 heads of 64 x 64, bfloat16, training, us at 32 and
 // 64 steps a chunk: 24 steps 275 and 875, 64 steps 740 and 1045, 200 steps 2534 and 3258.
 // A window of a few robots is delta_split.hip's, which takes all its chunks at once but for the state's own chain (`groups`
-// workgroups). One pass and split, us, 64 x 64, bfloat16, training:
-//     T         16 groups      64 groups      96 groups      128 groups
-//     100        64,  63        71,  72        73,  77         72,  79
-//     150        72,  65        80,  79        85,  81         84,  87
-//     400       152, 110       165, 136       179, 156        185, 179
-//     1000      344, 195       378, 265       411, 373        449, 458
-// so from five chunks on, up to 96 groups. There the chain's length counts, and chunks of 64 halve it: 168, 271 and 344 us for
-// the last line's first three, 475 for 2 x 4096 of 8 heads that take 618 by 32; at T = 400 they gain nothing (112, 141, 184).
-// Bfloat16 alone takes 64: float16's second plane makes them no faster (64 groups, T = 1000: 299 by 32, 331 by 64), and
-// float32's third does not fit the LDS.
+// workgroups). From five chunks on and up to 96 groups: one pass and split by 32, us, training, bfloat16, 64 x 64:
+//     T        16 groups      64 groups      96 groups      128 groups     256 groups
+//     100       64,  63        71,  72        73,  77        72,  79
+//     400      152, 110       165, 136       179, 156       185, 179       226, 268
+//     1000     365, 203       391, 248       410, 317       442, 377       547, 596
+//     2000     700, 320       773, 496       828, 604       873, 728      1055, 1132
+// and at T = 1000 of other sizes and types:
+//     forward alone   155,  82       160, 100       165, 113       165, 124       165, 211
+//     128 x 128       459, 272       495, 380       550, 476       594, 559       769, 917
+//     32 x 32         308, 210       331, 212       339, 218       347, 219       382, 328
+//     float32         425, 215       471, 312       507, 413       553, 496       711, 821
+//     its 128 x 128   588, 324       678, 550       758, 702       834, 853      1127, 1441
+//     float16         419, 204       452, 270       473, 341       509, 425       630, 687
+// (the two sides meet between 100 and 250 groups, the earlier the larger the heads; the rule keeps below the first). There the
+// chain's length counts, and chunks of 64 halve it: at T = 2000, 16, 64 and 96 groups, 271, 480 and 624 us for the 320, 496 and
+// 604 by 32, of 128 x 128 409, 745 and 965 for 480, 747 and 939, but of 32 x 32 218, 317 and 389 for 222, 297 and 344; up to
+// T = 600 they gain nothing. Bfloat16 alone takes 64: float16's second plane makes them no faster (64 groups, T = 1000: 299
+// by 32, 331 by 64), and float32's third does not fit the LDS.
 static int64_t groups_of(const InetDelta* a) { return (int64_t)a->B * a->H * ((a->V + 63) / 64); }
 static bool split(const InetDelta* a) {
     const int64_t chunks = ((int64_t)a->T + a->chunk - 1) / a->chunk;

@@ -284,8 +284,8 @@ struct FfnShape {
 
 // y, or (BACK) da and du side by side in da [N][2 F8]. A workgroup takes tile after tile: the next one's first step is on
 // its way, and dy has come during the last step, while the results are stored. The matrix instructions bound it, then what
-// the activation and the stores leave of their time: 131072 x 512 x 2048, bfloat16, silu: y 640 us, 859 TFLOP/s (the library's
-// product of these sizes alone 716, 8192^3 1302); da and du 1025 us with 1.6 GB of dy, da and du beside the same products.
+// the activation and the stores leave of their time: 131072 x 512 x 2048, bfloat16, silu: y 641 us, 857 TFLOP/s (the library's
+// product of these sizes alone 716, 8192^3 1302); da and du 1021 us with 1.6 GB of dy, da and du beside the same products.
 template <typename T, typename P, int ACT, bool BACK>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)
 void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __restrict__ y, const T* __restrict__ dy,
@@ -399,7 +399,7 @@ void ffn_gates_kernel(FfnShape p, Operand<T, true> x, Operand<T, true> w, T* __r
 }
 
 // C [rows][cols] = a b (+ a2 b2 where there are such), or shares of the sum each to a C of its own. At the sizes above: dx
-// 650 us, 846 TFLOP/s (the library's product 925); both dW 590 us, 932 TFLOP/s (559). An operand across the sum goes through
+// 679 us, 810 TFLOP/s (the library's product 925); both dW 606 us, 907 TFLOP/s (559). An operand across the sum goes through
 // registers and is transposed by LDS reads, which is what keeps it from the rate of 8192^3.
 template <typename T, typename P, bool RA, bool CA, typename O>
 __global__ __launch_bounds__(P::THREADS, P::THREADS == 512 ? 2 : 1)

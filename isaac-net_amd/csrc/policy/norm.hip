@@ -8,7 +8,7 @@
 // Memory bounds it: each row is read once into registers (the backward pass computes y again from x and f rather than
 // read it, so y stays unrounded) and every sum over a row goes across its lanes in 32 bits. LP lanes take a row, NJ groups
 // of 8 values each, 16 bytes at a time wherever rows start. 131072 x 512, bfloat16, full gate: forward 113 us for 0.67 GB, 5.9
-// TB/s, backward 250 us for 1.2 GB, 4.8 TB/s (a copy makes 4.8); 5001 x 999, float32, a gate a row: 20 and 39 us. Rows off the
+// TB/s, backward 262 us for 1.2 GB, 4.6 TB/s (a copy makes 4.8); 5001 x 999, float32, a gate a row: 20 and 40 us. Rows off the
 // 16-byte grid cost up to half more (62660 x 1071, float16: forward 179 us, backward 489).
 // The sums over rows for the weights stay in each workgroup's registers through all its rows, then go to the workspace
 // as one partial row a workgroup; a second kernel adds those in a fixed order, so results do not vary from run to run.

@@ -221,7 +221,12 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
     before the window (None: empty); reset [B, T] bool or uint8: an episode starts at the step, its memory empty; scale:
     K ** -0.5 by default. Any batch, step and head strides. The recurrence is stable for ||k||^2 beta <= 2: keys are
     usually of unit length and beta in 0 .. 1. A log-decay below -104, whose exponential is 0 in 32 bits, empties the
-    memory as reset does.
+    memory as reset does: whatever it held or an earlier step was given, NaN included, later steps see nothing of it, nor
+    an earlier step's gradient of a later episode's.
+
+    Errors, states and their gradients are of 32-bit grade; o and the other gradients are of their type's (float32 gates
+    beside 16-bit q, k and v have gradients of 32-bit grade). The backward pass needs `state` as it was: a
+    delta_rule_step on it in between makes it raise.
 
     Returns (o [B, T, H, V] of v's type, the memory after the window [B, H, K, V] float32)."""
     _delta_check(q, k, v, g, beta, state, reset, 2)
@@ -235,8 +240,8 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
 def delta_rule_step(q, k, v, g, beta, state, reset=None, scale=None, out=None):
     """One control step of the gated delta rule, the memory updated in place: q, k [B, Hk, K], v [B, H, V], g and beta
     [B, H], state [B, H, K, V] float32 contiguous, reset [B] (an emptied memory is empty whatever it held). Returns o
-    [B, H, V] (in `out` if given, contiguous of v's type: v itself, or over none of the inputs). No derivatives (in grad mode an input that requires grad is refused):
-    windows are trained through delta_rule."""
+    [B, H, V] (in `out` if given, contiguous of v's type: v itself, or over none of the inputs). No derivatives (in grad
+    mode an input that requires grad is refused): windows are trained through delta_rule."""
     dev = _delta_check(q, k, v, g, beta, state, reset, 1)
     if state is None or not state.is_contiguous():
         raise ValueError("state has to be a contiguous tensor: it is updated in place")

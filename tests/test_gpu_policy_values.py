@@ -184,7 +184,8 @@ def test_a_gradient_stays_in_its_episode(dt, B, T, K, V, what):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
-@pytest.mark.parametrize("B,T,K,V", [(3, 24, 64, 64), (2, 33, 32, 40), (40, 70, 128, 128), (2, 200, 100, 64), (2, 600, 64, 128)])
+@pytest.mark.parametrize("B,T,K,V", [(3, 24, 64, 64), (2, 33, 32, 40), (40, 70, 128, 128), (2, 200, 100, 64), (2, 600, 64, 128),
+                                       (1, 530, 128, 128)])
 def test_gates_of_32_bits_have_gradients_of_32_bits(dt, B, T, K, V):
     """dg and dbeta are of the gates' type: beside 16-bit q, k and v they are as exact as those of the same values in
     float32: at most four times their distance, which is the order of sums, of other lengths in chunks of other sizes."""
